@@ -522,6 +522,73 @@ int sva_top_unique(const int64_t *idx, const float *scores, const uint8_t *valid
 int64_t sva_stream_read_sink_words(int64_t bytes);
 int sva_stream_read(const void *src, int64_t bytes, uint32_t *sink, int64_t sink_words, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * A KV cache in 4 bits.  No counterpart in the reference: a quarter of the
+ * memory of a 16-bit cache, written once per row and read in place.
+ *   data    [G, rows, 2, D / 2] uint8, 16-byte aligned: row r's K codes, then
+ *           its V codes, two to a byte, the lower element in the low bits; a
+ *           code is a sign (8) and 0, 0.5, 1, 1.5, 2, 3, 4, 6 (0 to 7)
+ *   scales  [G, rows, 2, D / 32] uint8: 32 consecutive elements are their
+ *           codes times 2^(byte - 127); 255: they are NaN
+ *   D is a multiple of 32, at most 256.
+ */
+
+/*
+ * Writes rows of K and V.  Per 32 elements with largest magnitude a the scale
+ * is 2^(floor(log2 a) - 2) (byte at least 1), the codes the nearest values in
+ * units of it (ties to the even code, at most 6); a block with an infinity or
+ * a NaN becomes NaN.
+ *   keys / values  (b, g, t, d) at b*kv_seq_stride + g*kv_head_stride +
+ *                  t*kv_row_stride + d
+ *   first_rows     [n_seq] int64 on the device: token t of sequence b goes to
+ *                  cache row first_rows[b] + t; rows outside [0, rows) are
+ *                  skipped.  Two sequences must not name one row.
+ */
+int sva_cache4_write(const void *keys, const void *values, int kv_dtype, int64_t kv_seq_stride,
+                     int64_t kv_head_stride, int64_t kv_row_stride, int64_t n_seq, int64_t n_rows, int64_t G,
+                     int64_t D, const int64_t *first_rows, uint8_t *data, uint8_t *scales, int64_t rows,
+                     void *stream);
+
+/*
+ * The values of rows first_rows[b] + t, laid out as sva_cache4_write takes
+ * them (exact in bf16 and fp32; rounded to nearest in fp16).  Output rows
+ * whose cache row lies outside [0, rows) are left as they were.
+ */
+int sva_cache4_read(const uint8_t *data, const uint8_t *scales, int64_t rows, const int64_t *first_rows,
+                    int64_t n_seq, int64_t n_rows, int64_t G, int64_t D, void *keys, void *values, int kv_dtype,
+                    int64_t kv_seq_stride, int64_t kv_head_stride, int64_t kv_row_stride, void *stream);
+
+/*
+ * sva_verify over a 4-bit cache: softmax attention of each query item over
+ * the rows its budget list names (sva/llama.py:304-317), in fp32.  Entries
+ * outside [0, len) of their sequence are skipped; a list may name a row
+ * twice (it then counts twice); no row at all gives 0.
+ */
+int sva_cache4_verify(const void *q, int q_dtype, int64_t q_seq_stride, int64_t q_head_stride, int64_t q_tok_stride,
+                      const uint8_t *data, const uint8_t *scales, int64_t rows, const int64_t *seq_offsets,
+                      const int64_t *seq_lens, int64_t n_keys, const int32_t *fin_idx, const int32_t *fin_count,
+                      int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D, int64_t B, float scaling, void *out,
+                      int out_dtype, int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride,
+                      void *stream);
+
+/*
+ * Attention of the last Q tokens of every sequence over all of its rows (the
+ * causal rule: token t sees row n iff n <= len - Q + t; a token that sees no
+ * row gives 0).  n_keys is at least every seq_lens[b]; the part of a sequence
+ * behind it, or behind the cache's rows, is not read.
+ *   out (b, h, t, d) at b*out_seq_stride + h*out_head_stride + t*out_tok_stride + d
+ * workspace: sva_cache4_attention_workspace_bytes(...) bytes (no state
+ * between calls).
+ */
+size_t sva_cache4_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D,
+                                            int64_t n_keys);
+int sva_cache4_attention(const void *q, int q_dtype, int64_t q_seq_stride, int64_t q_head_stride,
+                         int64_t q_tok_stride, const uint8_t *data, const uint8_t *scales, int64_t rows,
+                         const int64_t *seq_offsets, const int64_t *seq_lens, int64_t n_keys, int64_t n_seq,
+                         int64_t H, int64_t G, int64_t Q, int64_t D, float scaling, void *out, int out_dtype,
+                         int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -774,3 +774,174 @@ def stream_read(buf: torch.Tensor, sink: torch.Tensor | None = None) -> torch.Te
         raise ValueError(f"stream_read: the sink must hold {words} int32 words on {device}")
     check(lib().sva_stream_read(ptr(buf), nbytes, ptr(sink), sink.numel(), stream_handle(device)), "sva_stream_read")
     return sink
+
+
+# ---------------------------------------------------------------------------
+# a KV cache in 4 bits
+
+
+def cache4_alloc(kv_heads: int, rows: int, head_dim: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """An empty 4-bit KV cache of one layer: data uint8 [G, rows, 2, D / 2] and
+    scales uint8 [G, rows, 2, D / 32], a row's K before its V (17 bits for 32
+    elements' 512 in bf16: K and V of a row take D + D / 16 bytes)."""
+
+    if kv_heads < 1 or rows < 1 or head_dim < 1 or head_dim > 256 or head_dim % 32 != 0:
+        raise ValueError(f"a 4-bit cache takes head_dim a multiple of 32 up to 256, got {kv_heads} x {rows} rows of "
+                         f"{head_dim}")
+    return (torch.zeros(kv_heads, rows, 2, head_dim // 2, device=device, dtype=torch.uint8),
+            torch.zeros(kv_heads, rows, 2, head_dim // 32, device=device, dtype=torch.uint8))
+
+
+def _check_cache4(data: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
+    """(G, rows, D) of a 4-bit cache."""
+
+    if data.dim() != 4 or data.dtype != torch.uint8 or data.shape[2] != 2 or not data.is_contiguous():
+        raise ValueError(f"4-bit data must be contiguous uint8 [G, rows, 2, D / 2], got {data.dtype} "
+                         f"{tuple(data.shape)}")
+    kv_heads, rows, _, half = data.shape
+    if scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (kv_heads, rows, 2,
+                                                                                            half // 16):
+        raise ValueError(f"4-bit scales must be contiguous uint8 {(kv_heads, rows, 2, half // 16)}, got "
+                         f"{scales.dtype} {tuple(scales.shape)}")
+    if half % 16 != 0 or half > 128 or half < 16:
+        raise ValueError(f"a 4-bit cache takes head_dim a multiple of 32 up to 256, got {2 * half}")
+    return kv_heads, rows, 2 * half
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """An entry point on `device`'s current stream, with `device` current."""
+
+    fn = getattr(lib(), name)
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(fn(*args, stream_handle(device)), name)
+        return
+    with torch.cuda.device(device):
+        check(fn(*args, stream_handle(device)), name)
+
+
+def _seq_tensor(name: str, t, n_seq: int, device: torch.device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        t = torch.tensor([t] if isinstance(t, int) else list(t), device=device, dtype=torch.int64)
+    if t.dtype != torch.int64 or tuple(t.shape) != (n_seq,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be int64 [{n_seq}], got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def cache4_write(keys: torch.Tensor, values: torch.Tensor, data: torch.Tensor, scales: torch.Tensor,
+                 first_rows) -> None:
+    """Writes keys / values [n_seq, G, T, D] (or [G, T, D]) into a 4-bit cache
+    (cache4_alloc): token t of sequence b into row first_rows[b] + t.
+    first_rows: int64 [n_seq] on the device, or an int or ints (copied there).
+    Rows outside the cache are skipped; two sequences must not name one row."""
+
+    kv_heads, rows, dim = _check_cache4(data, scales)
+    if keys.dim() == 3:
+        keys, values = keys.unsqueeze(0), values.unsqueeze(0)
+    if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != values.dtype or keys.shape[1] != kv_heads or \
+            keys.shape[3] != dim:
+        raise ValueError(f"keys / values must be [n_seq, {kv_heads}, T, {dim}] of one dtype, got {keys.dtype} "
+                         f"{tuple(keys.shape)} and {values.dtype} {tuple(values.shape)}")
+    device = require_device(keys, values, data, scales, first_rows if isinstance(first_rows, torch.Tensor) else None)
+    n_seq, _, n_rows, _ = keys.shape
+    first = _seq_tensor("first_rows", first_rows, n_seq, device)
+    dtype = dtype_code(keys)
+    if n_seq == 0 or n_rows == 0:
+        return
+    if keys.stride(-1) != 1 or values.stride() != keys.stride():
+        keys, values = keys.contiguous(), values.contiguous()
+    _call(device, "sva_cache4_write", ptr(keys), ptr(values), dtype, keys.stride(0), keys.stride(1), keys.stride(2),
+          n_seq, n_rows, kv_heads, dim, ptr(first), ptr(data), ptr(scales), rows)
+
+
+def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: int,
+                dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows first_rows[b] + t, t < n_rows, of a 4-bit cache as keys and values
+    [n_seq, G, n_rows, D] of `dtype` (exact in bf16 and fp32).  The rows must
+    lie inside the cache: the outputs of others are undefined."""
+
+    kv_heads, rows, dim = _check_cache4(data, scales)
+    device = require_device(data, scales, first_rows if isinstance(first_rows, torch.Tensor) else None)
+    n_seq = first_rows.shape[0] if isinstance(first_rows, torch.Tensor) and first_rows.dim() else (
+        1 if isinstance(first_rows, (int, torch.Tensor)) else len(first_rows))
+    first = _seq_tensor("first_rows", first_rows, n_seq, device)
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {dtype}; expected float32, bfloat16 or float16")
+    if n_rows < 0 or n_rows > rows:
+        raise ValueError(f"{n_rows} rows of a cache of {rows}")
+    keys = torch.empty(n_seq, kv_heads, n_rows, dim, device=device, dtype=dtype)
+    values = torch.empty_like(keys)
+    if n_seq and n_rows:
+        _call(device, "sva_cache4_read", ptr(data), ptr(scales), rows, ptr(first), n_seq, n_rows, kv_heads, dim,
+              ptr(keys), ptr(values), dtype_code(keys), keys.stride(0), keys.stride(1), keys.stride(2))
+    return keys, values
+
+
+def _cache4_query(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, n_keys: int, seq_offsets, seq_lens):
+    kv_heads, rows, dim = _check_cache4(data, scales)
+    q = _as_query(q)
+    n_seq, heads, q_len, head_dim = q.shape
+    if head_dim != dim or heads == 0 or heads % kv_heads != 0:
+        raise ValueError(f"query {tuple(q.shape)} does not fit a cache of {kv_heads} KV heads of {dim}")
+    if (seq_offsets is None) != (seq_lens is None):
+        raise ValueError("seq_offsets and seq_lens go together")
+    if seq_offsets is None:
+        if n_seq != 1:
+            raise ValueError("several sequences need seq_offsets and seq_lens")
+        if n_keys > rows:
+            raise ValueError(f"{n_keys} keys of a cache of {rows} rows")
+    else:
+        seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq, q.device)
+        seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq, q.device)
+    device = require_device(q, data, scales, seq_offsets, seq_lens)
+    return q, device, kv_heads, rows, seq_offsets, seq_lens
+
+
+def cache4_attention(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, n_keys: int, scaling: float,
+                     out_dtype: torch.dtype | None = None, seq_offsets: torch.Tensor | None = None,
+                     seq_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention [n_seq, H, Q, D] of the last Q tokens of every sequence over
+    all its rows of a 4-bit cache: token t sees row n iff n <= len - Q + t (0
+    where it sees none).  One sequence of n_keys rows at row 0, or seq_offsets
+    / seq_lens with n_keys at least the longest."""
+
+    q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query(q, data, scales, n_keys, seq_offsets, seq_lens)
+    n_seq, heads, q_len, dim = q.shape
+    out = torch.empty(n_seq, heads, q_len, dim, device=device, dtype=out_dtype or q.dtype)
+    if out.numel() == 0:
+        return out
+    if n_keys <= 0:
+        return out.zero_()
+    # a buffer of the call's own: calls on other streams and captured graphs never share one
+    ws = torch.empty(int(lib().sva_cache4_attention_workspace_bytes(n_seq, heads, kv_heads, q_len, dim, n_keys)),
+                     device=device, dtype=torch.uint8)
+    _call(device, "sva_cache4_attention", ptr(q), dtype_code(q), q.stride(0), q.stride(1), q.stride(2), ptr(data),
+          ptr(scales), rows, ptr(seq_offsets), ptr(seq_lens), n_keys, n_seq, heads, kv_heads, q_len, dim,
+          float(scaling), ptr(out), dtype_code(out), out.stride(0), out.stride(1), out.stride(2), ptr(ws), ws.numel())
+    return out
+
+
+def cache4_verify(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, fin_idx: torch.Tensor,
+                  fin_count: torch.Tensor, n_keys: int, scaling: float, out_dtype: torch.dtype | None = None,
+                  seq_offsets: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """verify() over a 4-bit cache: attention [n_seq, H, Q, D] of every query
+    item over the rows its budget list names (fin_idx [items, B], fin_count
+    [items], as budget_select gives them)."""
+
+    q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query(q, data, scales, n_keys, seq_offsets, seq_lens)
+    n_seq, heads, q_len, dim = q.shape
+    items = n_seq * heads * q_len
+    if fin_idx.dim() != 2 or fin_idx.dtype != torch.int32 or not fin_idx.is_contiguous() or fin_idx.shape[0] != items \
+            or fin_count.dtype != torch.int32 or tuple(fin_count.shape) != (items,) or not fin_count.is_contiguous():
+        raise ValueError(f"fin_idx must be contiguous int32 [{items}, B] and fin_count int32 [{items}]")
+    require_device(q, fin_idx, fin_count)
+    budget = fin_idx.shape[1]
+    out = torch.empty(n_seq, heads, q_len, dim, device=device, dtype=out_dtype or q.dtype)
+    if out.numel() == 0:
+        return out
+    if n_keys <= 0 or budget == 0:
+        return out.zero_()
+    _call(device, "sva_cache4_verify", ptr(q), dtype_code(q), q.stride(0), q.stride(1), q.stride(2), ptr(data),
+          ptr(scales), rows, ptr(seq_offsets), ptr(seq_lens), n_keys, ptr(fin_idx), ptr(fin_count), n_seq, heads,
+          kv_heads, q_len, dim, budget, float(scaling), ptr(out), dtype_code(out), out.stride(0), out.stride(1),
+          out.stride(2))
+    return out

@@ -1,0 +1,301 @@
+"""The KV cache in 4 bits on the GPU against the definition in 64 bits: codes and scales bit for bit, read rows exactly,
+attention and verifier within bounds of their arithmetic."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from .cache4_reference import attend, decode, encode
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+WEIGHTS = 2.0 ** -17  # a weight as two bf16 terms is within 2^-9 2^-9; twice that
+
+
+def rows_of(rng, shape, dtype, device):
+    """Rows of every kind: normal values at many magnitudes, ties, saturating values, zeros, tiny and huge blocks."""
+    x = rng.standard_normal(shape) * np.exp2(rng.integers(-8, 8, (*shape[:-1], 1)))
+    flat = x.reshape(-1, 32)
+    n = len(flat)
+    ties = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 4.0, 0.0, -0.25, -2.5, -5.0, -7.5, 3.0])
+    flat[0 % n] = np.tile(ties, 2)
+    flat[1 % n, :] = 0.0
+    if n > 4:
+        flat[2] *= 1e-30 if dtype != torch.float16 else 1e-3
+        flat[3] = np.where(np.arange(32) == 5, 60000.0, flat[3])
+        flat[4] = -0.0
+    return torch.from_numpy(x.astype(np.float32)).to(device, dtype)
+
+
+def make_cache(rng, G, rows, D, device):
+    from sva_amd import kernels
+
+    k = torch.from_numpy(rng.standard_normal((G, rows, D)).astype(np.float32)).to(device)
+    v = torch.from_numpy(rng.standard_normal((G, rows, D)).astype(np.float32)).to(device)
+    data, scales = kernels.cache4_alloc(G, rows, D, device)
+    kernels.cache4_write(k, v, data, scales, 0)
+    return data, scales
+
+
+def decoded(data, scales):
+    kv = decode(data.cpu().numpy(), scales.cpu().numpy())
+    return kv[:, :, 0], kv[:, :, 1]
+
+
+@pytest.mark.parametrize("n_seq,G,T,D,dtype", [
+    (1, 1, 1, 32, torch.float32), (3, 2, 5, 64, torch.bfloat16), (2, 3, 33, 128, torch.float16),
+    (1, 2, 70, 96, torch.bfloat16), (2, 1, 9, 256, torch.float32), (1, 3, 2000, 64, torch.bfloat16)])
+def test_write_and_read(device, n_seq, G, T, D, dtype):
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(T + D)
+    k, v = (rows_of(rng, (n_seq, G, T, D), dtype, device) for _ in range(2))
+    rows = n_seq * (T + 3) + 2
+    data, scales = kernels.cache4_alloc(G, rows, D, device)
+    data.fill_(0xAB)
+    scales.fill_(7)
+    first = [b * (T + 3) + 1 + b % 2 for b in range(n_seq)]
+    kernels.cache4_write(k, v, data, scales, first)
+    got_d, got_s = data.cpu().numpy(), scales.cpu().numpy()
+    touched = np.zeros(rows, bool)
+    for b in range(n_seq):
+        at = slice(first[b], first[b] + T)
+        touched[at] = True
+        for i, x in enumerate((k, v)):
+            codes, bytes_ = encode(x[b].float().cpu().numpy())
+            assert np.array_equal(got_s[:, at, i], bytes_)
+            assert np.array_equal(got_d[:, at, i], codes)
+    assert (got_d[:, ~touched] == 0xAB).all() and (got_s[:, ~touched] == 7).all()
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        back = kernels.cache4_read(data, scales, torch.tensor(first, device=device), T, out)
+        for i, x in enumerate(back):
+            for b in range(n_seq):
+                at = slice(first[b], first[b] + T)
+                ref = decode(got_d[:, at, i], got_s[:, at, i])
+                want = torch.from_numpy(ref).to(torch.float32).to(out)
+                assert torch.equal(x[b].cpu(), want)
+
+
+def test_write_takes_strides_and_alignment(device):
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(3)
+    T, G, D = 7, 2, 64
+    wide = rows_of(rng, (1, T, 2 * G, D), torch.bfloat16, device)
+    heads = wide.transpose(1, 2)                       # [1, 2 G, T, D], rows not neighbours
+    odd = torch.zeros(1 + T * G * D, device=device, dtype=torch.bfloat16)[1:].view(1, G, T, D)
+    odd.copy_(heads[:, :G])                            # rows at odd addresses
+    results = []
+    for k, v in ((heads[:, :G], heads[:, G:]), (odd, heads[:, G:]), (heads[:, :G].contiguous(),
+                                                                      heads[:, G:].contiguous())):
+        data, scales = kernels.cache4_alloc(G, T, D, device)
+        kernels.cache4_write(k, v, data, scales, 0)
+        results.append((data, scales))
+    for data, scales in results[:-1]:
+        assert torch.equal(data, results[-1][0]) and torch.equal(scales, results[-1][1])
+    o2 = torch.empty(1 + T * G * D, device=device, dtype=torch.bfloat16)[1:].view(1, G, T, D)
+    kernels.cache4_write(odd, o2.copy_(heads[:, G:]), data, scales, 0)  # both odd: element by element
+    assert torch.equal(data, results[-1][0]) and torch.equal(scales, results[-1][1])
+
+
+def test_write_skips_rows_outside_and_marks_blocks_that_are_not_finite(device):
+    from sva_amd import kernels
+
+    k = torch.ones(2, 1, 4, 64, device=device)
+    k[0, 0, 1, 3] = float("nan")
+    k[0, 0, 2, 40] = float("-inf")
+    v = k.clone()
+    data, scales = kernels.cache4_alloc(1, 6, 64, device)
+    scales.fill_(9)
+    kernels.cache4_write(k, v, data, scales, [-1, 4])  # rows -1 .. 2 and 4 .. 7: rows -1, 6 and 7 are not there
+    s = scales[0].cpu().tolist()
+    assert s[0] == [[255, 125]] * 2 and s[1] == [[125, 255]] * 2 and s[2] == [[125, 125]] * 2
+    assert s[3] == [[9, 9]] * 2 and s[4] == s[5] == [[125, 125]] * 2
+    keys, _ = kernels.cache4_read(data, scales, 0, 3)
+    assert torch.isnan(keys[0, 0, 0, :32]).all() and (keys[0, 0, 0, 32:] == 1).all() and (keys[0, 0, 2] == 1).all()
+    before = data.clone()
+    kernels.cache4_write(k[:, :, :0], v[:, :, :0], data, scales, [0, 0])
+    assert torch.equal(before, data)
+
+
+def attention_case(device, lens, H, G, Q, D, dtype, seed=0, pad=0):
+    rng = np.random.default_rng(seed + sum(lens) + Q)
+    starts = np.concatenate([[0], np.cumsum([n + pad for n in lens])])
+    rows = max(int(starts[-1]), 1)
+    data, scales = make_cache(rng, G, rows, D, device)
+    q = torch.from_numpy(rng.standard_normal((len(lens), H, Q, D)).astype(np.float32)).to(device, dtype)
+    off = torch.tensor(starts[:-1], device=device)
+    return q, data, scales, off, torch.tensor(lens, device=device)
+
+
+def close(got, ref, bound, weights=WEIGHTS, scale=None):
+    """|got - ref| <= the bound, the weights' rounding of the sums' size, and half a step of the output's type."""
+    g = got.double().cpu().numpy()
+    extra = weights * scale if scale is not None else 0.0
+    assert (np.abs(g - ref) <= bound + extra + HALF_STEP[got.dtype] * np.abs(ref) + 1e-30).all(), \
+        np.nanmax(np.abs(g - ref) - bound - extra - HALF_STEP[got.dtype] * np.abs(ref))
+
+
+@pytest.mark.parametrize("lens,H,G,Q,D,dtype", [
+    ([1], 1, 1, 1, 64, torch.float32), ([5], 3, 1, 1, 32, torch.float32), ([33, 0, 1, 64], 4, 2, 1, 64, torch.bfloat16),
+    ([300, 129, 31], 9, 3, 2, 64, torch.float16), ([700], 16, 1, 3, 128, torch.float32),  # 48 query rows: three tiles
+    ([1000, 3], 32, 8, 1, 128, torch.bfloat16), ([257, 513], 2, 1, 5, 96, torch.float32),
+    ([640], 4, 4, 7, 256, torch.float16), ([90], 2, 2, 1, 160, torch.bfloat16), ([5000], 3, 1, 1, 64, torch.float32),
+    ([2, 3], 6, 2, 4, 64, torch.float32)])  # tokens before the first row see nothing
+def test_attention(device, lens, H, G, Q, D, dtype):
+    from sva_amd import kernels
+
+    q, data, scales, off, ln = attention_case(device, lens, H, G, Q, D, dtype, pad=3)
+    K, V = decoded(data, scales)
+    got = kernels.cache4_attention(q, data, scales, max(lens), D ** -0.5, seq_offsets=off, seq_lens=ln)
+    assert got.shape == q.shape and got.dtype == dtype
+    for out_dtype in {dtype, torch.float32}:
+        got = kernels.cache4_attention(q, data, scales, max(lens), D ** -0.5, out_dtype, off, ln)
+        for b, n in enumerate(lens):
+            at = slice(int(off[b]), int(off[b]) + n)
+            allowed = np.arange(n) <= n - Q + np.arange(Q)[:, None]
+            for h in range(H):
+                g = h // (H // G)
+                x = q[b, h].double().cpu().numpy()
+                ref, bound = attend(x, K[g, at], V[g, at], allowed, D ** -0.5)
+                size, _ = attend(x, K[g, at], np.abs(V[g, at]), allowed, D ** -0.5)
+                close(got[b, h], ref, bound, scale=size)
+
+
+def test_attention_of_one_sequence_needs_no_offsets(device):
+    from sva_amd import kernels
+
+    q, data, scales, off, ln = attention_case(device, [777], 9, 3, 1, 64, torch.bfloat16)
+    a = kernels.cache4_attention(q, data, scales, 777, 0.125)
+    b = kernels.cache4_attention(q, data, scales, 1500, 0.125, seq_offsets=off, seq_lens=ln)
+    assert torch.equal(a, kernels.cache4_attention(q[0], data, scales, 777, 0.125))
+    assert (a.float() - b.float()).abs().max() <= 2.0 ** -7 * a.float().abs().max()  # other ranges, one step of bf16
+    strided = torch.zeros(1, 1, 9, 64, device=device, dtype=torch.bfloat16).transpose(1, 2).copy_(q)
+    assert torch.equal(a, kernels.cache4_attention(strided, data, scales, 777, 0.125))
+    # a length behind the cache's end, or behind n_keys, is cut there
+    c = kernels.cache4_attention(q, data, scales, 777, 0.125, seq_offsets=off, seq_lens=ln * 100)
+    assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("Q", [1, 3])
+def test_attention_nan_rows_reach_only_who_sees_them(device, Q):
+    from sva_amd import kernels
+
+    lens = [200]
+    q, data, scales, off, ln = attention_case(device, lens, 2, 1, Q, 64, torch.float32, pad=50)
+    clean = kernels.cache4_attention(q, data, scales, 200, 0.125, seq_offsets=off, seq_lens=ln)
+    scales[0, 200:] = 255  # rows behind the sequence
+    assert torch.equal(clean, kernels.cache4_attention(q, data, scales, 200, 0.125, seq_offsets=off, seq_lens=ln))
+    scales[0, 199, 1, 1] = 255  # half of the last row's V: the last token alone sees it
+    got = kernels.cache4_attention(q, data, scales, 200, 0.125, seq_offsets=off, seq_lens=ln)
+    assert torch.isnan(got[:, :, -1, 32:]).all()
+    assert torch.equal(got[:, :, -1, :32], clean[:, :, -1, :32]) and torch.equal(got[:, :, :-1], clean[:, :, :-1])
+    scales[0, 199, 0, 0] = 255  # and of its K
+    got = kernels.cache4_attention(q, data, scales, 200, 0.125, seq_offsets=off, seq_lens=ln)
+    assert torch.isnan(got[:, :, -1]).all() and torch.equal(got[:, :, :-1], clean[:, :, :-1])
+
+
+@pytest.mark.parametrize("lens,H,G,Q,D,B,dtype", [
+    ([1], 1, 1, 1, 64, 1, torch.float32), ([300, 0, 9], 6, 2, 2, 64, 40, torch.bfloat16),
+    ([1000], 9, 3, 1, 64, 512, torch.float32), ([500, 400], 8, 8, 1, 128, 333, torch.float16),
+    ([300], 2, 1, 3, 32, 100, torch.float32), ([300], 3, 1, 1, 96, 64, torch.bfloat16),
+    ([300], 2, 1, 1, 256, 200, torch.float32)])
+def test_verify(device, lens, H, G, Q, D, B, dtype):
+    from sva_amd import kernels
+
+    q, data, scales, off, ln = attention_case(device, lens, H, G, Q, D, dtype)
+    K, V = decoded(data, scales)
+    rng = np.random.default_rng(B)
+    items = len(lens) * H * Q
+    idx = np.full((items, B), -1, np.int32)
+    cnt = np.zeros(items, np.int32)
+    for i in range(items):
+        n = lens[i // (H * Q)]
+        cnt[i] = rng.integers(0, min(B, n) + 1) if i % 5 == 0 else min(B, n)
+        idx[i, :cnt[i]] = np.sort(rng.choice(n, cnt[i], replace=False)) if n else []
+    if lens[0] >= 4:
+        idx[0, 0:2], cnt[0] = [-5, lens[0]], max(cnt[0], 2)  # entries outside the sequence are skipped
+    got = kernels.cache4_verify(q, data, scales, torch.from_numpy(idx).to(device), torch.from_numpy(cnt).to(device),
+                                max(lens), D ** -0.5, None, off, ln)
+    assert got.dtype == dtype
+    for i in range(items):
+        b, h, t = i // (H * Q), i // Q % H, i % Q
+        at = idx[i, :cnt[i]]
+        at = at[(at >= 0) & (at < lens[b])] + int(off[b])
+        g = h // (H // G)
+        x = q[b, h, t:t + 1].double().cpu().numpy()
+        ref, bound = attend(x, K[g, at], V[g, at], np.ones((1, len(at)), bool), D ** -0.5)
+        close(got[b, h, t:t + 1], ref, 2 * bound)  # (twice: the slots' and waves' rescaling)
+
+
+def test_verify_of_every_row_equals_attention(device):
+    from sva_amd import kernels
+
+    q, data, scales, off, ln = attention_case(device, [600], 9, 3, 1, 64, torch.float32)
+    idx = torch.arange(600, device=device, dtype=torch.int32).expand(9, 600).contiguous()
+    a = kernels.cache4_verify(q, data, scales, idx, torch.full((9,), 600, device=device, dtype=torch.int32), 600, 0.125)
+    b = kernels.cache4_attention(q, data, scales, 600, 0.125)
+    assert (a - b).abs().max() <= 2.0 ** -16 * a.abs().max() + 2.0 ** -16
+
+
+def test_calls_on_another_stream_and_in_a_graph(device):
+    """Two streams at once, and replays with eager work between them: each equals the eager result."""
+    from sva_amd import kernels
+
+    q, data, scales, off, ln = attention_case(device, [9000, 4000], 9, 3, 1, 64, torch.bfloat16)
+    q2 = q.flip(1).contiguous()
+
+    def call(x):
+        return kernels.cache4_attention(x, data, scales, 9000, 0.125, seq_offsets=off, seq_lens=ln)
+
+    want, want2 = call(q), call(q2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            a = call(q)
+        b = call(q2)
+    torch.cuda.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want2)
+    static = q.clone()
+    with torch.cuda.stream(side):
+        call(static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(static)
+    for x, w in ((q2, want2), (q, want), (q2, want2)):
+        static.copy_(x)
+        graph.replay()
+        assert torch.equal(call(q), want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, w)
+
+
+def test_offsets_past_32_bits(device):
+    """Rows whose code bytes lie past 2^31 and whose elements lie past 2^32."""
+    from sva_amd import kernels
+
+    rows, D = 20_000_000, 128  # 2.56 GB of codes a KV head
+    data = torch.zeros(2, rows, 2, D // 2, device=device, dtype=torch.uint8)
+    scales = torch.full((2, rows, 2, D // 32), 127, device=device, dtype=torch.uint8)
+    g = torch.Generator(device=device).manual_seed(0)
+    k, v = (torch.randn(2, 300, D, device=device, generator=g) for _ in range(2))
+    q = torch.randn(1, 4, 1, D, device=device, generator=g)
+    first = rows - 300
+    kernels.cache4_write(k, v, data, scales, first)
+    small, small_s = kernels.cache4_alloc(2, 300, D, device)
+    kernels.cache4_write(k, v, small, small_s, 0)
+    assert torch.equal(data[:, first:], small) and torch.equal(scales[:, first:], small_s)
+    off, ln = torch.tensor([first], device=device), torch.tensor([300], device=device)
+    want = kernels.cache4_attention(q, small, small_s, 300, 0.1)
+    assert torch.equal(kernels.cache4_attention(q, data, scales, 300, 0.1, seq_offsets=off, seq_lens=ln), want)
+    idx = torch.arange(300, device=device, dtype=torch.int32).expand(4, 300).contiguous()
+    cnt = torch.full((4,), 300, device=device, dtype=torch.int32)
+    assert torch.equal(kernels.cache4_verify(q, data, scales, idx, cnt, 300, 0.1, None, off, ln),
+                       kernels.cache4_verify(q, small, small_s, idx, cnt, 300, 0.1))
+    assert all(torch.equal(a, b) for a, b in zip(kernels.cache4_read(data, scales, first, 300),
+                                                 kernels.cache4_read(small, small_s, 0, 300)))
