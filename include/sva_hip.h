@@ -589,6 +589,40 @@ int sva_cache4_attention(const void *q, int q_dtype, int64_t q_seq_stride, int64
                          int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride, void *workspace,
                          size_t workspace_bytes, void *stream);
 
+/*
+ * Dense attention of whole prompts: softmax attention of the last Q tokens of
+ * every sequence over all of its keys, without a shortlist.  No counterpart
+ * in the reference, whose patched layers summon for prompt tokens too
+ * (sva/llama.py:226-328); its unpatched layers use the model's own attention.
+ *   q, out   (b, h, t, d) at b*seq_stride + h*head_stride + t*tok_stride + d;
+ *            with q_offsets / q_lens (int64 [n_seq], device; both or neither)
+ *            packed tokens: token t of sequence b is row q_offsets[b] + t of
+ *            q_rows, t < q_lens[b] <= Q, at h*head_stride + row*tok_stride.
+ *            Rows of no sequence are left as they were.
+ *   keys / values  of q's dtype, key n of sequence b at row seq_offsets[b] + n
+ *            of kv_rows; n_keys is at least every seq_lens[b], and what lies
+ *            behind it, or behind kv_rows, is not read
+ *   mask     NULL: token t sees key n iff n <= len - Q + t (its sequence's Q);
+ *            otherwise (t, n) of sequence b at b*mask_seq_stride +
+ *            t*mask_tok_stride + n decides alone: a float > -1e4 allows (it is
+ *            not added), a bool byte allows where it is not 0 (unlike the
+ *            lookup's SVA_MASK_BOOL).  Not with packed tokens.
+ *   A token that sees no key gives 0.  What an unseen key holds, NaN and
+ *   infinities included, reaches no output.  head_dim <= 256.
+ * workspace: sva_prompt_attention_workspace_bytes(...) bytes (no state
+ * between calls).
+ */
+size_t sva_prompt_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D,
+                                            int64_t n_keys);
+int sva_prompt_attention(const void *q, int dtype, int64_t q_seq_stride, int64_t q_head_stride, int64_t q_tok_stride,
+                         const int64_t *q_offsets, const int64_t *q_lens, int64_t q_rows, const void *keys,
+                         const void *values, int64_t kv_head_stride, int64_t kv_row_stride, int64_t kv_rows,
+                         const int64_t *seq_offsets, const int64_t *seq_lens, int64_t n_keys, int64_t n_seq, int64_t H,
+                         int64_t G, int64_t Q, int64_t D, float scaling, const void *mask, int mask_type,
+                         int64_t mask_seq_stride, int64_t mask_tok_stride, void *out, int out_dtype,
+                         int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

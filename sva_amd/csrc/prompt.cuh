@@ -1,0 +1,436 @@
+// Dense attention of whole prompts: the kernel.
+//
+// out[r] = sum_n p[n] V[n] / sum_n p[n], p[n] = 2^(s (q[r] . K[n]) - m), over
+// the keys row r may see, in one pass over the keys with a running reference
+// m.  The query rows of a KV head are (token, head of its group) pairs,
+// token-major, so one K / V tile serves every head of the group.  Four waves
+// of 32 * NQ query rows each share tiles of BN keys in LDS (two buffers: the
+// next tile is loaded into registers while this one is used).
+//  * S^T = K Q^T (rows: keys) leaves each lane with half of the tile's scores
+//    of one query row, and exactly the elements of P^T that the second
+//    product O^T = V^T P^T wants from it: weights stay in registers, a row's
+//    maximum takes one exchange between the wave's halves.
+//  * The reference m only moves when a tile's maximum passes it by 2^8: the
+//    sums are then rescaled.  Weights are at most 2^8 (fp16: 2^12, and 2^8 at
+//    the maximum, which keeps small ones out of fp16's subnormals).
+//  * Weights are rounded to the type of V for the product (2^-9 of each, of
+//    random sign, as V's own rounding); m, the sum of weights and the sums are
+//    fp32.  fp32 inputs use the fp32 matrix instructions throughout.
+//  * A masked key's V meets a weight of 0, which a NaN or an infinity
+//    survives: a wave whose sums are not finite does its rows again, key by
+//    key, over the keys they may see alone.
+#pragma once
+#include "cache4.h"
+#include "join.h"
+
+namespace sva {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+struct PromptParams {
+  const void* q;
+  int64_t q_bs, q_hs, q_ts;
+  const int64_t* q_offsets;
+  const int64_t* q_lens;
+  int64_t q_rows;
+  const void* keys;
+  const void* values;
+  int64_t kv_hs, kv_rs, kv_rows;
+  const int64_t* offs;
+  const int64_t* lens;
+  int64_t N;
+  int n_seq, H, G, Q, D, row_tiles, splits;
+  int chunk;     // keys per workgroup, a multiple of 64
+  bool vec;      // K, V and Q rows are whole aligned 16-byte words
+  float scaling;
+  const void* mask;
+  int mask_type;
+  int64_t mask_bs, mask_ts;
+  float* part;
+  void* out;
+  int out_dtype;
+  int64_t o_bs, o_hs, o_ts;
+};
+
+template <int DT>
+struct PromptType {
+  static constexpr int ES = DT == F32 ? 4 : 2;
+  static constexpr int BN = DT == F32 ? 32 : 64;
+};
+
+SVA_DEV bool prompt_mask_allows(const void* mask, int64_t i, int mtype) {
+  return mtype == MASK_BOOL ? ((const uint8_t*)mask)[i] != 0 : mask_allows(mask, i, mtype);
+}
+
+template <int DT, int DP, int NQ, bool MASK>
+__global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
+  constexpr int ES = PromptType<DT>::ES, BN = PromptType<DT>::BN;
+  constexpr int KT = BN / 32;            // 32-key blocks of a tile
+  constexpr int CPR = DP * ES / 16;      // 16-byte chunks of a row
+  constexpr int CH = BN * CPR / 256;     // chunks per thread
+  constexpr int EC = 16 / ES;            // elements of a chunk
+  constexpr int BM = 4 * 32 * NQ;        // query rows of a workgroup
+  constexpr int TB = BN * DP * ES;       // bytes of a K or V tile
+  constexpr int NO = DP / 32;            // 32-element blocks of the sums
+  constexpr float kLog2e = 1.44269504088896340736f;
+  constexpr float kSlack = DT == F16 ? 12.0f : 8.0f;   // how far a score may pass the reference
+  constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;    // how far below the maximum a new reference lies
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int tid = (int)threadIdx.x, lane = lane_id(), w = tid / WAVE;
+  const int l32 = lane & 31, hf = lane >> 5, m16 = lane & 15;
+
+  // KV heads fastest (8 of them: one XCD's L2 each), then the row tiles, the longest first
+  int64_t id = blockIdx.x;
+  const int g = (int)(id % p.G);
+  id /= p.G;
+  const int rt = p.row_tiles - 1 - (int)(id % p.row_tiles);
+  id /= p.row_tiles;
+  const int split = (int)(id % p.splits);
+  const int b = (int)(id / p.splits);
+  const int grp = p.H / p.G;
+  int64_t q_first;
+  const int q_len = seq_tokens(p.q_lens, p.q_offsets, p.q_rows, p.Q, b, q_first);
+  const int rows = q_len * grp;
+  if (rt * BM >= rows) return;
+  const int64_t off = p.offs ? p.offs[b] : 0;
+  int64_t len64 = min(min(p.lens ? p.lens[b] : p.N, p.N), p.kv_rows - off);
+  const int len = off < 0 || len64 < 0 ? 0 : (int)len64;
+  const int shift = len - q_len;  // token t sees keys n <= t + shift
+  const int last_tok = (min(rows, (rt + 1) * BM) - 1) / grp;
+  const int kbeg = split * p.chunk;
+  const int kend = min(min(len, kbeg + p.chunk), MASK ? len : last_tok + shift + 1);
+
+  // this wave's rows, and per lane NQ of them
+  const int wrow = rt * BM + w * 32 * NQ;
+  const int wend = min(rows, wrow + 32 * NQ);
+  const bool busy = wrow < rows;
+  const int wfull = MASK ? 0 : min(len, wrow / grp + shift + 1);                  // keys below are seen by all rows
+  const int wlast = busy ? (MASK ? kend : min(kend, (wend - 1) / grp + shift + 1)) : 0;  // keys from here by none
+  int lim[NQ];                    // last key of the lane's row
+  const unsigned char* mrow[NQ];  // its mask row
+  const int64_t kvb = (int64_t)g * p.kv_hs + off * p.kv_rs;  // element offset of key 0
+  auto q_at = [&](int r, int64_t bs, int64_t hs, int64_t ts) {
+    const int tok = r / grp, head = g * grp + r % grp;
+    return (p.q_lens ? (q_first + tok) * ts : (int64_t)b * bs + (int64_t)tok * ts) + (int64_t)head * hs;
+  };
+  using frag = typename std::conditional<DT == BF16, bf16x8, typename std::conditional<DT == F16, f16x8, f32x4>::type>::type;
+  constexpr int NF = DT == F32 ? DP / 8 : DP / 16;  // fragments of a row per lane
+  constexpr int FE = DT == F32 ? 4 : 8;             // elements of one: d = 2 FE f + FE hf + i
+  frag bq[NQ][NF];
+  const float sgn = p.scaling < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = wrow + 32 * n + l32;
+    const bool live = r < rows;
+    lim[n] = live ? (MASK ? kend - 1 : min(kend - 1, r / grp + shift)) : -1;
+    if constexpr (MASK) {
+      const int64_t at = (int64_t)b * p.mask_bs + (int64_t)(live ? r / grp : 0) * p.mask_ts;
+      mrow[n] = (const unsigned char*)p.mask + at * (p.mask_type == MASK_F32 ? 4 : (p.mask_type == MASK_BOOL ? 1 : 2));
+    }
+    const int64_t at = q_at(live ? r : 0, p.q_bs, p.q_hs, p.q_ts);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      const int d = 2 * FE * f + FE * hf;
+      if (live && p.vec) {
+        union {
+          uint4 u;
+          frag v;
+        } x;
+        x.u = *(const uint4*)((const unsigned char*)p.q + (at + d) * ES);
+        bq[n][f] = x.v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < FE; ++i) {
+          const float x = live && d + i < p.D ? load_elem(p.q, at + d + i, DT) : 0.0f;
+          if constexpr (DT == BF16) bq[n][f][i] = (__bf16)x;
+          else if constexpr (DT == F16) bq[n][f][i] = (_Float16)x;
+          else bq[n][f][i] = x;
+        }
+      }
+      if (sgn < 0.0f) bq[n][f] = -bq[n][f];
+    }
+  }
+  // (a scale of 0: the smallest normal one gives the same weights, and -inf times it stays -inf)
+  const float sl = fmaxf(fabsf(p.scaling) * kLog2e, 1.17549435e-38f);
+
+  f32x16 o[NQ][NO];
+  float mref[NQ], z[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    mref[n] = -3.0e38f;
+    z[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o[n][i][k] = 0.0f;
+  }
+
+  uint4 kr[CH], vr[CH];
+  auto fetch = [&](int n0) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int idx = tid + 256 * c;
+      const int row = idx / CPR, ch = idx % CPR;
+      const int64_t e = kvb + (int64_t)min(n0 + row, len - 1) * p.kv_rs + ch * EC;  // past the end: the last key
+      if (p.vec) {
+        kr[c] = *(const uint4*)((const unsigned char*)p.keys + e * ES);
+        vr[c] = *(const uint4*)((const unsigned char*)p.values + e * ES);
+      } else {
+        union {
+          uint4 u;
+          uint16_t h[8];
+          uint32_t x[4];
+        } a, v;
+#pragma unroll
+        for (int i = 0; i < EC; ++i) {
+          const bool in = ch * EC + i < p.D;
+          if constexpr (ES == 4) {
+            a.x[i] = in ? ((const uint32_t*)p.keys)[e + i] : 0u;
+            v.x[i] = in ? ((const uint32_t*)p.values)[e + i] : 0u;
+          } else {
+            a.h[i] = in ? ((const uint16_t*)p.keys)[e + i] : (uint16_t)0;
+            v.h[i] = in ? ((const uint16_t*)p.values)[e + i] : (uint16_t)0;
+          }
+        }
+        kr[c] = a.u;
+        vr[c] = v.u;
+      }
+    }
+  };
+  // chunk ch of row r lies at ch ^ (r % 8) (K: eight rows' chunks of one
+  // column meet no bank twice) and ch ^ 2 (r % 4) (V: as do the four rows of
+  // a transposed read)
+  auto place = [&](unsigned char* buf) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int idx = tid + 256 * c;
+      const int row = idx / CPR, ch = idx % CPR;
+      *(uint4*)(buf + (row * CPR + (ch ^ (row & 7))) * 16) = kr[c];
+      *(uint4*)(buf + TB + (row * CPR + (ES == 2 ? ch ^ ((row & 3) * 2) : ch)) * 16) = vr[c];
+    }
+  };
+
+  int cur = 0;
+  if (kbeg < kend) {
+    fetch(kbeg);
+    place(lds);
+  }
+  __syncthreads();
+  for (int n0 = kbeg; n0 < kend; n0 += BN) {
+    const bool more = n0 + BN < kend;
+    if (more) fetch(n0 + BN);
+    if (n0 < wlast) {
+      const unsigned char* kb = lds + cur * 2 * TB;
+      const unsigned char* vb = kb + TB;
+      f32x16 s[NQ][KT];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) s[n][kt][k] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const frag a = *(const frag*)(kb + ((32 * kt + l32) * CPR + ((2 * f + hf) ^ (l32 & 7))) * 16);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            if constexpr (DT == BF16) {
+              s[n][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, bq[n][f], s[n][kt], 0, 0, 0);
+            } else if constexpr (DT == F16) {
+              s[n][kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bq[n][f], s[n][kt], 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                s[n][kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], bq[n][f][i], s[n][kt], 0, 0, 0);
+            }
+          }
+        }
+      }
+      // a lane's score k of block kt is key n0 + 32 kt + 8 (k / 4) + 4 hf + k % 4
+      if (MASK || n0 + BN > wfull) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int key = n0 + 32 * kt + 8 * (k / 4) + 4 * hf + k % 4;
+              bool ok = key <= lim[n];
+              if constexpr (MASK) {
+                if (ok) ok = prompt_mask_allows(mrow[n], key, p.mask_type);
+              }
+              s[n][kt][k] = ok ? s[n][kt][k] : -INFINITY;
+            }
+      }
+      using pfrag = typename std::conditional<DT == F32, f32x4, frag>::type;
+      pfrag pw[NQ][KT][2];  // (unused for fp32, whose weights stay in s)
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        float top = s[n][0][0];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) top = fmaxf(top, s[n][kt][k]);
+        {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+          top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        }
+        top *= sl;
+        if (__any(top > mref[n] + kSlack)) {
+          const float mn = fmaxf(mref[n], top - kBelow);
+          const float corr = __builtin_amdgcn_exp2f(mref[n] - mn);
+          mref[n] = mn;
+          z[n] *= corr;
+#pragma unroll
+          for (int i = 0; i < NO; ++i) o[n][i] *= corr;
+        }
+        float zs = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k], sl, -mref[n]));
+            zs += e;
+            if constexpr (DT == BF16) pw[n][kt][k / 8][k % 8] = (__bf16)e;
+            else if constexpr (DT == F16) pw[n][kt][k / 8][k % 8] = (_Float16)e;
+            else s[n][kt][k] = e;
+          }
+        z[n] += zs;
+      }
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        if constexpr (DT == F32) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float* vrow = (const float*)(vb + (32 * kt + 8 * (k / 4) + 4 * hf + k % 4) * CPR * 16);
+#pragma unroll
+            for (int i = 0; i < NO; ++i) {
+              const float a = vrow[32 * i + l32];
+#pragma unroll
+              for (int n = 0; n < NQ; ++n)
+                o[n][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[n][kt][k], o[n][i], 0, 0, 0);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+#pragma unroll
+            for (int i = 0; i < NO; ++i) {
+              union {
+                s16x4 half[2];
+                frag v;
+              } a;
+              const int row = 32 * kt + 16 * st + 4 * hf + m16 / 4;
+              const int ch = (4 * i + 2 * (lane >> 4 & 1) + (m16 & 3) / 2) ^ (m16 / 4 * 2);
+              const unsigned char* at = vb + (row * CPR + ch) * 16 + (m16 & 1) * 8;
+              a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+              a.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) s16x4*)(at + 8 * CPR * 16));
+#pragma unroll
+              for (int n = 0; n < NQ; ++n) {
+                if constexpr (DT == BF16)
+                  o[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, pw[n][kt][st], o[n][i], 0, 0, 0);
+                else
+                  o[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.v, pw[n][kt][st], o[n][i], 0, 0, 0);
+              }
+            }
+          }
+        }
+      }
+    }
+    cur ^= 1;
+    if (more) place(lds + cur * 2 * TB);
+    __syncthreads();
+  }
+  if (!busy) return;
+
+  // the two halves of the wave hold a row's keys
+  bool odd = false;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(z[n]), __float_as_uint(z[n]), false, false);
+    z[n] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) odd = odd || !(fabsf(o[n][i][k]) <= 3.40282347e38f);
+  }
+  auto part_at = [&](int r) {
+    const int tok = r / grp, head = g * grp + r % grp;
+    return p.part + ((((int64_t)b * p.H + head) * p.Q + tok) * p.splits + split) * (p.D + 2);
+  };
+  if (__any(odd)) {
+    // again, key by key: lanes take 64 keys' scores, then the row's elements
+    for (int r = wrow; r < wend; ++r) {
+      const int end = MASK ? kend : min(kend, r / grp + shift + 1);
+      const int64_t qa = q_at(r, p.q_bs, p.q_hs, p.q_ts);
+      float m = -INFINITY, zz = 0.0f, acc[DP / 64];
+#pragma unroll
+      for (int k = 0; k < DP / 64; ++k) acc[k] = 0.0f;
+      for (int n0 = kbeg; n0 < end; n0 += WAVE) {
+        const int key = n0 + lane;
+        bool ok = key < end;
+        if constexpr (MASK)
+          ok = ok && prompt_mask_allows(p.mask, (int64_t)b * p.mask_bs + (int64_t)(r / grp) * p.mask_ts + key,
+                                        p.mask_type);
+        float sc = -INFINITY;
+        if (ok) {
+          sc = 0.0f;
+          const int64_t ka = kvb + (int64_t)key * p.kv_rs;
+          for (int d = 0; d < p.D; ++d)
+            sc = __builtin_fmaf(load_elem(p.q, qa + d, DT), load_elem(p.keys, ka + d, DT), sc);
+          sc *= p.scaling * kLog2e;
+        }
+        const float mn = fmaxf(m, wave_max(sc));
+        const float corr = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        const float e = ok ? __builtin_amdgcn_exp2f(sc - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
+        m = mn;
+        zz = zz * corr + wave_sum(e);
+#pragma unroll
+        for (int k = 0; k < DP / 64; ++k) acc[k] *= corr;
+        const uint64_t seen = __ballot(ok);
+        for (int j = 0; j < min(WAVE, end - n0); ++j) {
+          if (!(seen >> j & 1ull)) continue;
+          const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e), j));
+          const int64_t va = kvb + (int64_t)(n0 + j) * p.kv_rs;
+#pragma unroll
+          for (int k = 0; k < DP / 64; ++k) {
+            const int d = lane + 64 * k;
+            if (d < p.D) acc[k] = __builtin_fmaf(pj, load_elem(p.values, va + d, DT), acc[k]);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < DP / 64; ++k) {
+        const int d = lane + 64 * k;
+        if (d >= p.D) continue;
+        if (p.splits > 1)
+          part_at(r)[2 + d] = acc[k];
+        else
+          store_elem(p.out, q_at(r, p.o_bs, p.o_hs, p.o_ts) + d, p.out_dtype, zz == 0.0f ? 0.0f : acc[k] / zz);
+      }
+      if (p.splits > 1 && lane == 0) part_at(r)[0] = m, part_at(r)[1] = zz;
+    }
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = wrow + 32 * n + l32;
+    if (r >= rows) continue;
+    float* part = p.splits > 1 ? part_at(r) : nullptr;
+    const int64_t at = q_at(r, p.o_bs, p.o_hs, p.o_ts);
+    const float f = part ? 1.0f : (z[n] == 0.0f ? 0.0f : 1.0f / z[n]);
+    if (part && hf == 0) part[0] = mref[n], part[1] = z[n];
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int d = 32 * i + 8 * (k / 4) + 4 * hf + k % 4;
+        if (d >= p.D) continue;
+        if (part) part[2 + d] = o[n][i][k];
+        else store_elem(p.out, at + d, p.out_dtype, o[n][i][k] * f);
+      }
+  }
+}
+
+}  // namespace sva

@@ -1,0 +1,147 @@
+// Dense attention of whole prompts (sva_prompt_attention): argument checks,
+// the choice of tile and of key ranges, launches.  The kernel: prompt.cuh.
+#include <algorithm>
+#include <type_traits>
+
+#include "prompt.cuh"
+
+#include "capi_internal.h"
+#include "summon.h"
+
+using namespace sva;
+
+namespace {
+
+constexpr int BM = 128;  // query rows of a workgroup
+
+int64_t row_tiles(int64_t H, int64_t G, int64_t Q) { return (H / G * Q + BM - 1) / BM; }
+
+// Keys per workgroup: all of them where the row tiles alone fill the card,
+// otherwise ranges of at least 512.
+int64_t chunk_keys(int64_t tiles, int64_t n_keys) {
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(64, 768 / tiles));
+  return std::max<int64_t>(512, ((n_keys + want - 1) / want + 63) / 64 * 64);
+}
+
+template <int DT, int DP, bool MASK>
+int launch(const PromptParams& p, hipStream_t stream) {
+  constexpr int lds = 4 * PromptType<DT>::BN * DP * PromptType<DT>::ES;
+  constexpr auto fn = prompt_kernel<DT, DP, 1, MASK>;
+  SVA_SET_MAX_LDS_ONCE(fn, sva::kMaxLds, "hipFuncSetAttribute(prompt_kernel)");
+  const int64_t blocks = (int64_t)p.G * p.row_tiles * p.splits * p.n_seq;
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), lds, stream, p);
+  SVA_CHECK_LAUNCH("prompt_kernel");
+  return SVA_OK;
+}
+
+template <int DT>
+int launch_dim(const PromptParams& p, hipStream_t stream) {
+  if (p.mask) {
+    if (p.D <= 64) return launch<DT, 64, true>(p, stream);
+    if (p.D <= 128) return launch<DT, 128, true>(p, stream);
+    return launch<DT, 256, true>(p, stream);
+  }
+  if (p.D <= 64) return launch<DT, 64, false>(p, stream);
+  if (p.D <= 128) return launch<DT, 128, false>(p, stream);
+  return launch<DT, 256, false>(p, stream);
+}
+
+}  // namespace
+
+extern "C" size_t sva_prompt_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D,
+                                                       int64_t n_keys) {
+  if (n_seq <= 0 || H <= 0 || G <= 0 || Q <= 0 || D <= 0 || n_keys <= 0 || H % G != 0) return 0;
+  const int64_t chunk = chunk_keys(n_seq * G * row_tiles(H, G, Q), n_keys);
+  const int64_t splits = (n_keys + chunk - 1) / chunk;
+  return splits == 1 ? 256 : sizeof(float) * (size_t)(n_seq * H * Q) * (size_t)splits * (size_t)(D + 2) + 256;
+}
+
+extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stride, int64_t q_head_stride,
+                                    int64_t q_tok_stride, const int64_t* q_offsets, const int64_t* q_lens,
+                                    int64_t q_rows, const void* keys, const void* values, int64_t kv_head_stride,
+                                    int64_t kv_row_stride, int64_t kv_rows, const int64_t* seq_offsets,
+                                    const int64_t* seq_lens, int64_t n_keys, int64_t n_seq, int64_t H, int64_t G,
+                                    int64_t Q, int64_t D, float scaling, const void* mask, int mask_type,
+                                    int64_t mask_seq_stride, int64_t mask_tok_stride, void* out, int out_dtype,
+                                    int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  sva::clear_error();
+  SVA_REQUIRE(q && keys && values && out, "sva_prompt_attention: null pointer");
+  SVA_REQUIRE((seq_offsets == nullptr) == (seq_lens == nullptr) && (q_offsets == nullptr) == (q_lens == nullptr),
+              "sva_prompt_attention: offsets and lengths go together");
+  SVA_REQUIRE(seq_offsets || n_seq == 1, "sva_prompt_attention: several sequences need offsets and lengths");
+  SVA_REQUIRE(n_seq > 0 && H > 0 && G > 0 && Q > 0 && n_keys > 0 && kv_rows > 0 && H % G == 0 &&
+                  (!q_lens || q_rows > 0),
+              "sva_prompt_attention: bad sizes");
+  SVA_REQUIRE(D > 0 && D <= 256, "sva_prompt_attention: head_dim %lld out of range (at most 256)", (long long)D);
+  SVA_REQUIRE(dtype >= 0 && dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, "sva_prompt_attention: bad dtype");
+  SVA_REQUIRE((mask == nullptr) == (mask_type == SVA_MASK_NONE) && mask_type >= 0 && mask_type <= 4,
+              "sva_prompt_attention: bad mask type");
+  SVA_REQUIRE(!mask || !q_lens, "sva_prompt_attention: packed tokens take no mask");
+  SVA_REQUIRE(n_keys < (1ll << 31) - 1024 && n_seq < (1ll << 31) && H < (1ll << 20) && Q < (1ll << 31) &&
+                  H * Q < (1ll << 31) && n_seq * H < (1ll << 31) && n_seq * H * Q < (1ll << 31),
+              "sva_prompt_attention: too many items or keys");
+  const size_t need = sva_prompt_attention_workspace_bytes(n_seq, H, G, Q, D, n_keys);
+  SVA_REQUIRE(workspace != nullptr && workspace_bytes >= need, "sva_prompt_attention: workspace of %zu bytes required",
+              need);
+  const int64_t word = dtype == F32 ? 4 : 8;  // elements of 16 bytes
+  PromptParams p;
+  p.q = q;
+  p.q_bs = q_seq_stride;
+  p.q_hs = q_head_stride;
+  p.q_ts = q_tok_stride;
+  p.q_offsets = q_offsets;
+  p.q_lens = q_lens;
+  p.q_rows = q_rows;
+  p.keys = keys;
+  p.values = values;
+  p.kv_hs = kv_head_stride;
+  p.kv_rs = kv_row_stride;
+  p.kv_rows = kv_rows;
+  p.offs = seq_offsets;
+  p.lens = seq_lens;
+  p.N = n_keys;
+  p.n_seq = (int)n_seq;
+  p.H = (int)H;
+  p.G = (int)G;
+  p.Q = (int)Q;
+  p.D = (int)D;
+  p.row_tiles = (int)row_tiles(H, G, Q);
+  p.chunk = (int)chunk_keys(n_seq * G * p.row_tiles, n_keys);
+  p.splits = (int)((n_keys + p.chunk - 1) / p.chunk);
+  p.vec = (D == 64 || D == 128 || D == 256) && (((uintptr_t)q | (uintptr_t)keys | (uintptr_t)values) & 15u) == 0 &&
+          q_seq_stride % word == 0 && q_head_stride % word == 0 && q_tok_stride % word == 0 &&
+          kv_head_stride % word == 0 && kv_row_stride % word == 0;
+  p.scaling = scaling;
+  p.mask = mask;
+  p.mask_type = mask_type;
+  p.mask_bs = mask_seq_stride;
+  p.mask_ts = mask_tok_stride;
+  p.part = (float*)workspace;
+  p.out = out;
+  p.out_dtype = out_dtype;
+  p.o_bs = out_seq_stride;
+  p.o_hs = out_head_stride;
+  p.o_ts = out_tok_stride;
+  SVA_REQUIRE((int64_t)p.G * p.row_tiles * p.splits * n_seq < (1ll << 31), "sva_prompt_attention: too many items");
+  int rc;
+  if (dtype == F32) rc = launch_dim<F32>(p, (hipStream_t)stream);
+  else if (dtype == BF16) rc = launch_dim<BF16>(p, (hipStream_t)stream);
+  else rc = launch_dim<F16>(p, (hipStream_t)stream);
+  if (rc != SVA_OK || p.splits == 1) return rc;
+  JoinParams j;
+  j.part = p.part;
+  j.splits = p.splits;
+  j.H = p.H;
+  j.Q = p.Q;
+  j.D = p.D;
+  j.q_lens = q_lens;
+  j.q_offsets = q_offsets;
+  j.q_rows = q_rows;
+  j.out = out;
+  j.out_dtype = out_dtype;
+  j.o_bs = out_seq_stride;
+  j.o_hs = out_head_stride;
+  j.o_ts = out_tok_stride;
+  return sva::launch_join(j, n_seq, (hipStream_t)stream);
+}

@@ -808,6 +808,11 @@ def _check_cache4(data: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, i
     return kv_heads, rows, 2 * half
 
 
+def _inference_only(name: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} runs inference only: call it under torch.no_grad()")
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """An entry point on `device`'s current stream, with `device` current."""
 
@@ -842,6 +847,7 @@ def cache4_write(keys: torch.Tensor, values: torch.Tensor, data: torch.Tensor, s
         raise ValueError(f"keys / values must be [n_seq, {kv_heads}, T, {dim}] of one dtype, got {keys.dtype} "
                          f"{tuple(keys.shape)} and {values.dtype} {tuple(values.shape)}")
     device = require_device(keys, values, data, scales, first_rows if isinstance(first_rows, torch.Tensor) else None)
+    _inference_only("cache4_write", keys, values)
     n_seq, _, n_rows, _ = keys.shape
     first = _seq_tensor("first_rows", first_rows, n_seq, device)
     dtype = dtype_code(keys)
@@ -905,6 +911,7 @@ def cache4_attention(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, 
     / seq_lens with n_keys at least the longest."""
 
     q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query(q, data, scales, n_keys, seq_offsets, seq_lens)
+    _inference_only("cache4_attention", q)
     n_seq, heads, q_len, dim = q.shape
     out = torch.empty(n_seq, heads, q_len, dim, device=device, dtype=out_dtype or q.dtype)
     if out.numel() == 0:
@@ -928,6 +935,7 @@ def cache4_verify(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, fin
     [items], as budget_select gives them)."""
 
     q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query(q, data, scales, n_keys, seq_offsets, seq_lens)
+    _inference_only("cache4_verify", q)
     n_seq, heads, q_len, dim = q.shape
     items = n_seq * heads * q_len
     if fin_idx.dim() != 2 or fin_idx.dtype != torch.int32 or not fin_idx.is_contiguous() or fin_idx.shape[0] != items \
@@ -944,4 +952,122 @@ def cache4_verify(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, fin
           ptr(scales), rows, ptr(seq_offsets), ptr(seq_lens), n_keys, ptr(fin_idx), ptr(fin_count), n_seq, heads,
           kv_heads, q_len, dim, budget, float(scaling), ptr(out), dtype_code(out), out.stride(0), out.stride(1),
           out.stride(2))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# dense attention of whole prompts
+
+
+def _prompt_mask(mask: torch.Tensor, n_seq: int, q_len: int, n_keys: int):
+    """(mask, type, sequence stride, token stride) of a mask [Q, N], [1 or n_seq, Q, N] or [1 or n_seq, 1, Q, N]."""
+
+    m = mask
+    if m.dim() == 4:
+        if m.shape[1] != 1 and m.stride(1) != 0:
+            raise ValueError(f"prompt_attention takes one mask for every head, got {tuple(mask.shape)}")
+        m = m[:, 0]
+    if m.dim() == 2:
+        m = m.unsqueeze(0)
+    if m.dim() != 3 or m.shape[0] not in (1, n_seq) or m.shape[1] < q_len or m.shape[2] < n_keys:
+        raise ValueError(f"mask {tuple(mask.shape)} does not cover {n_seq} sequences of {q_len} tokens over {n_keys} "
+                         f"keys")
+    m = m[:, :q_len, :n_keys]
+    if m.dtype not in _lib.MASK_TYPES:
+        raise TypeError(f"unsupported mask dtype {m.dtype}; expected bool, float32, bfloat16 or float16")
+    if m.stride(-1) != 1:
+        m = m.contiguous()
+    return m, _lib.MASK_TYPES[m.dtype], m.stride(0) if m.shape[0] > 1 else 0, m.stride(1)
+
+
+def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, n_keys: int, scaling: float,
+                     mask: torch.Tensor | None = None, seq_offsets: torch.Tensor | None = None,
+                     seq_lens: torch.Tensor | None = None, q_offsets: torch.Tensor | None = None,
+                     q_lens: torch.Tensor | None = None, max_q: int = 0, out: torch.Tensor | None = None,
+                     out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Dense softmax attention of the last tokens of every sequence over all of
+    its keys: token t of Q sees key n iff n <= len - Q + t (0 where it sees none).
+
+    q: [n_seq, H, Q, D] (or [H, Q, D]), every sequence with Q tokens; or, with
+    q_offsets and q_lens (int64 [n_seq] on the device), packed tokens
+    [H, T, D], sequence b's rows q_offsets[b] + t, t < q_lens[b] <= max_q.
+    keys / values: [G, rows, D] of q's dtype; one sequence of n_keys rows, or
+    seq_offsets / seq_lens (int64 [n_seq]), n_keys at least the longest.
+    mask (not with packed tokens): [Q, N], [1 or n_seq, Q, N] or
+    [1 or n_seq, 1, Q, N] in place of the causal rule; a float mask allows
+    where it is > -1e4 (its value is not added), a bool mask where it is true.
+    What a masked key holds, NaN and infinities included, reaches no output.
+
+    Returns q's shape in out_dtype (or `out`, of q's shape); packed rows of no
+    sequence are left as they were (undefined in a new output).  Inference
+    only: no gradient."""
+
+    packed = q_offsets is not None
+    if packed != (q_lens is not None) or (seq_offsets is None) != (seq_lens is None):
+        raise ValueError("offsets and lengths go together")
+    shape = q.shape
+    if packed:
+        if q.dim() != 3:
+            raise ValueError(f"packed tokens must be [H, T, D], got {tuple(q.shape)}")
+        if mask is not None:
+            raise ValueError("packed tokens take no mask")
+        heads, n_rows, dim = q.shape
+        n_seq = q_offsets.shape[0] if q_offsets.dim() == 1 else 0
+        q_len = min(int(max_q), n_rows)
+        if max_q < 1:
+            raise ValueError("packed tokens need max_q, the longest sequence's tokens")
+        q4 = q.unsqueeze(0)
+    else:
+        q4 = q.unsqueeze(0) if q.dim() == 3 else q
+        if q4.dim() != 4:
+            raise ValueError(f"query must be [n_seq, H, Q, D] or [H, Q, D], got {tuple(q.shape)}")
+        n_seq, heads, q_len, dim = q4.shape
+        n_rows = 0
+    if keys.dim() != 3 or keys.shape != values.shape or keys.dtype != values.dtype or keys.dtype != q.dtype or \
+            keys.shape[2] != dim:
+        raise ValueError(f"keys / values must be [G, rows, {dim}] of {q.dtype}, got {keys.dtype} {tuple(keys.shape)} "
+                         f"and {values.dtype} {tuple(values.shape)}")
+    kv_heads, rows = keys.shape[0], keys.shape[1]
+    if dim < 1 or dim > 256 or kv_heads < 1 or heads < 1 or heads % kv_heads != 0:
+        raise ValueError(f"{heads} query heads over {kv_heads} KV heads of {dim} unsupported (head_dim at most 256)")
+    if seq_offsets is None and (n_seq != 1 or n_keys > rows):
+        raise ValueError(f"{n_seq} sequences of up to {n_keys} keys need seq_offsets and seq_lens, or rows for them")
+    if out is not None and (out.shape != shape or out.stride(-1) != 1 or (out_dtype or out.dtype) != out.dtype):
+        raise ValueError(f"out must be {tuple(shape)} with contiguous rows, got {out.dtype} {tuple(out.shape)}")
+    device = require_device(q, keys, values, mask, seq_offsets, seq_lens, q_offsets, q_lens, out)
+    _inference_only("prompt_attention", q, keys, values)
+    dtype = dtype_code(q)
+    if seq_offsets is not None:
+        seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq, device)
+        seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq, device)
+    if packed:
+        q_offsets = _seq_tensor("q_offsets", q_offsets, n_seq, device)
+        q_lens = _seq_tensor("q_lens", q_lens, n_seq, device)
+    if q4.stride(-1) != 1:
+        q4 = q4.contiguous()
+    if keys.stride(-1) != 1 or values.stride() != keys.stride():
+        keys, values = keys.contiguous(), values.contiguous()
+    if out is None:
+        # tokens before heads: the model's projection takes the result without a copy
+        order = (q4.shape[0], q4.shape[2], heads, dim)
+        out = torch.empty(order, device=device, dtype=out_dtype or q.dtype).transpose(1, 2).view(shape)
+    if out.numel() == 0 or n_seq == 0 or q_len == 0:
+        return out
+    if n_keys <= 0:
+        if packed:
+            n_keys = 1  # (every length is 0: the rows of sequences become 0)
+            if rows == 0:
+                keys = values = keys.new_zeros(kv_heads, 1, dim)
+                rows = 1
+        else:
+            return out.zero_()
+    m, mtype, mseq, mtok = (None, 0, 0, 0) if mask is None else _prompt_mask(mask, n_seq, q_len, n_keys)
+    o4 = out if out.dim() == 4 else out.unsqueeze(0)
+    # a buffer of the call's own: calls on other streams and captured graphs never share one
+    ws = torch.empty(int(lib().sva_prompt_attention_workspace_bytes(n_seq, heads, kv_heads, q_len, dim, n_keys)),
+                     device=device, dtype=torch.uint8)
+    _call(device, "sva_prompt_attention", ptr(q4), dtype, q4.stride(0), q4.stride(1), q4.stride(2), ptr(q_offsets),
+          ptr(q_lens), n_rows, ptr(keys), ptr(values), keys.stride(0), keys.stride(1), rows, ptr(seq_offsets),
+          ptr(seq_lens), n_keys, n_seq, heads, kv_heads, q_len, dim, float(scaling), ptr(m), mtype, mseq, mtok, ptr(out),
+          dtype_code(out), o4.stride(0), o4.stride(1), o4.stride(2), ptr(ws), ws.numel())
     return out
