@@ -41,7 +41,6 @@ struct PromptParams {
   int64_t N;
   int n_seq, H, G, Q, D, row_tiles, splits;
   int chunk;     // keys per workgroup, a multiple of 64
-  bool vec;      // K, V and Q rows are whole aligned 16-byte words
   float scaling;
   const void* mask;
   int mask_type;
@@ -56,14 +55,22 @@ template <int DT>
 struct PromptType {
   static constexpr int ES = DT == F32 ? 4 : 2;
   static constexpr int BN = DT == F32 ? 32 : 64;
+  // waves per SIMD that the registers are kept to
+  static constexpr int waves(int dp, int nq) { return DT == F32 || dp * nq > 128 ? 1 : (dp * nq > 64 ? 2 : 3); }
 };
 
 SVA_DEV bool prompt_mask_allows(const void* mask, int64_t i, int mtype) {
   return mtype == MASK_BOOL ? ((const uint8_t*)mask)[i] != 0 : mask_allows(mask, i, mtype);
 }
 
-template <int DT, int DP, int NQ, bool MASK>
-__global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
+// How a call's rows are read and masked: whole aligned rows of DP elements
+// under the causal rule, the same under a mask, anything else.
+enum PromptMode : int { PROMPT_CAUSAL = 0, PROMPT_MASK = 1, PROMPT_ANY = 2 };
+
+template <int DT, int DP, int NQ, int MODE>
+__global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_kernel(PromptParams p) {
+  constexpr bool VEC = MODE != PROMPT_ANY;
+  const bool MASK = MODE == PROMPT_MASK || (MODE == PROMPT_ANY && p.mask != nullptr);
   constexpr int ES = PromptType<DT>::ES, BN = PromptType<DT>::BN;
   constexpr int KT = BN / 32;            // 32-key blocks of a tile
   constexpr int CPR = DP * ES / 16;      // 16-byte chunks of a row
@@ -76,7 +83,7 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
   constexpr float kSlack = DT == F16 ? 12.0f : 8.0f;   // how far a score may pass the reference
   constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;    // how far below the maximum a new reference lies
   extern __shared__ __align__(16) unsigned char lds[];
-  const int tid = (int)threadIdx.x, lane = lane_id(), w = tid / WAVE;
+  const int tid = (int)threadIdx.x, lane = lane_id(), w = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int l32 = lane & 31, hf = lane >> 5, m16 = lane & 15;
 
   // KV heads fastest (8 of them: one XCD's L2 each), then the row tiles, the longest first
@@ -107,7 +114,7 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
   const int wfull = MASK ? 0 : min(len, wrow / grp + shift + 1);                  // keys below are seen by all rows
   const int wlast = busy ? (MASK ? kend : min(kend, (wend - 1) / grp + shift + 1)) : 0;  // keys from here by none
   int lim[NQ];                    // last key of the lane's row
-  const unsigned char* mrow[NQ];  // its mask row
+  const unsigned char* mrow[NQ] = {};  // its mask row
   const int64_t kvb = (int64_t)g * p.kv_hs + off * p.kv_rs;  // element offset of key 0
   auto q_at = [&](int r, int64_t bs, int64_t hs, int64_t ts) {
     const int tok = r / grp, head = g * grp + r % grp;
@@ -123,7 +130,7 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
     const int r = wrow + 32 * n + l32;
     const bool live = r < rows;
     lim[n] = live ? (MASK ? kend - 1 : min(kend - 1, r / grp + shift)) : -1;
-    if constexpr (MASK) {
+    if (MASK) {
       const int64_t at = (int64_t)b * p.mask_bs + (int64_t)(live ? r / grp : 0) * p.mask_ts;
       mrow[n] = (const unsigned char*)p.mask + at * (p.mask_type == MASK_F32 ? 4 : (p.mask_type == MASK_BOOL ? 1 : 2));
     }
@@ -131,13 +138,13 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const int d = 2 * FE * f + FE * hf;
-      if (live && p.vec) {
+      if (VEC) {
         union {
-          uint4 u;
+          u32x4 u;
           frag v;
         } x;
-        x.u = *(const uint4*)((const unsigned char*)p.q + (at + d) * ES);
-        bq[n][f] = x.v;
+        x.u = *(const u32x4*)((const unsigned char*)p.q + (at + d) * ES);
+        bq[n][f] = live ? x.v : frag{};
       } else {
 #pragma unroll
         for (int i = 0; i < FE; ++i) {
@@ -165,19 +172,19 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
       for (int k = 0; k < 16; ++k) o[n][i][k] = 0.0f;
   }
 
-  uint4 kr[CH], vr[CH];
+  u32x4 kr[CH], vr[CH];
   auto fetch = [&](int n0) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int idx = tid + 256 * c;
       const int row = idx / CPR, ch = idx % CPR;
       const int64_t e = kvb + (int64_t)min(n0 + row, len - 1) * p.kv_rs + ch * EC;  // past the end: the last key
-      if (p.vec) {
-        kr[c] = *(const uint4*)((const unsigned char*)p.keys + e * ES);
-        vr[c] = *(const uint4*)((const unsigned char*)p.values + e * ES);
+      if constexpr (VEC) {
+        kr[c] = *(const u32x4*)((const unsigned char*)p.keys + e * ES);
+        vr[c] = *(const u32x4*)((const unsigned char*)p.values + e * ES);
       } else {
         union {
-          uint4 u;
+          u32x4 u;
           uint16_t h[8];
           uint32_t x[4];
         } a, v;
@@ -205,8 +212,8 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
     for (int c = 0; c < CH; ++c) {
       const int idx = tid + 256 * c;
       const int row = idx / CPR, ch = idx % CPR;
-      *(uint4*)(buf + (row * CPR + (ch ^ (row & 7))) * 16) = kr[c];
-      *(uint4*)(buf + TB + (row * CPR + (ES == 2 ? ch ^ ((row & 3) * 2) : ch)) * 16) = vr[c];
+      *(u32x4*)(buf + (row * CPR + (ch ^ (row & 7))) * 16) = kr[c];
+      *(u32x4*)(buf + TB + (row * CPR + (ES == 2 ? ch ^ ((row & 3) * 2) : ch)) * 16) = vr[c];
     }
   };
 
@@ -256,7 +263,7 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
             for (int k = 0; k < 16; ++k) {
               const int key = n0 + 32 * kt + 8 * (k / 4) + 4 * hf + k % 4;
               bool ok = key <= lim[n];
-              if constexpr (MASK) {
+              if (MASK) {
                 if (ok) ok = prompt_mask_allows(mrow[n], key, p.mask_type);
               }
               s[n][kt][k] = ok ? s[n][kt][k] : -INFINITY;
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(256) prompt_kernel(PromptParams p) {
       for (int n0 = kbeg; n0 < end; n0 += WAVE) {
         const int key = n0 + lane;
         bool ok = key < end;
-        if constexpr (MASK)
+        if (MASK)
           ok = ok && prompt_mask_allows(p.mask, (int64_t)b * p.mask_bs + (int64_t)(r / grp) * p.mask_ts + key,
                                         p.mask_type);
         float sc = -INFINITY;

@@ -23,10 +23,10 @@ int64_t chunk_keys(int64_t tiles, int64_t n_keys) {
   return std::max<int64_t>(512, ((n_keys + want - 1) / want + 63) / 64 * 64);
 }
 
-template <int DT, int DP, bool MASK>
+template <int DT, int DP, int MODE>
 int launch(const PromptParams& p, hipStream_t stream) {
   constexpr int lds = 4 * PromptType<DT>::BN * DP * PromptType<DT>::ES;
-  constexpr auto fn = prompt_kernel<DT, DP, 1, MASK>;
+  constexpr auto fn = prompt_kernel<DT, DP, 1, MODE>;
   SVA_SET_MAX_LDS_ONCE(fn, sva::kMaxLds, "hipFuncSetAttribute(prompt_kernel)");
   const int64_t blocks = (int64_t)p.G * p.row_tiles * p.splits * p.n_seq;
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), lds, stream, p);
@@ -34,16 +34,17 @@ int launch(const PromptParams& p, hipStream_t stream) {
   return SVA_OK;
 }
 
-template <int DT>
+template <int DT, int MODE>
 int launch_dim(const PromptParams& p, hipStream_t stream) {
-  if (p.mask) {
-    if (p.D <= 64) return launch<DT, 64, true>(p, stream);
-    if (p.D <= 128) return launch<DT, 128, true>(p, stream);
-    return launch<DT, 256, true>(p, stream);
-  }
-  if (p.D <= 64) return launch<DT, 64, false>(p, stream);
-  if (p.D <= 128) return launch<DT, 128, false>(p, stream);
-  return launch<DT, 256, false>(p, stream);
+  if (p.D <= 64) return launch<DT, 64, MODE>(p, stream);
+  if (p.D <= 128) return launch<DT, 128, MODE>(p, stream);
+  return launch<DT, 256, MODE>(p, stream);
+}
+
+template <int DT>
+int launch_mode(const PromptParams& p, bool vec, hipStream_t stream) {
+  if (!vec) return launch_dim<DT, PROMPT_ANY>(p, stream);
+  return p.mask ? launch_dim<DT, PROMPT_MASK>(p, stream) : launch_dim<DT, PROMPT_CAUSAL>(p, stream);
 }
 
 }  // namespace
@@ -109,9 +110,9 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   p.row_tiles = (int)row_tiles(H, G, Q);
   p.chunk = (int)chunk_keys(n_seq * G * p.row_tiles, n_keys);
   p.splits = (int)((n_keys + p.chunk - 1) / p.chunk);
-  p.vec = (D == 64 || D == 128 || D == 256) && (((uintptr_t)q | (uintptr_t)keys | (uintptr_t)values) & 15u) == 0 &&
-          q_seq_stride % word == 0 && q_head_stride % word == 0 && q_tok_stride % word == 0 &&
-          kv_head_stride % word == 0 && kv_row_stride % word == 0;
+  const bool vec = (D == 64 || D == 128 || D == 256) && (((uintptr_t)q | (uintptr_t)keys | (uintptr_t)values) & 15u) == 0 &&
+                   q_seq_stride % word == 0 && q_head_stride % word == 0 && q_tok_stride % word == 0 &&
+                   kv_head_stride % word == 0 && kv_row_stride % word == 0;
   p.scaling = scaling;
   p.mask = mask;
   p.mask_type = mask_type;
@@ -125,9 +126,9 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   p.o_ts = out_tok_stride;
   SVA_REQUIRE((int64_t)p.G * p.row_tiles * p.splits * n_seq < (1ll << 31), "sva_prompt_attention: too many items");
   int rc;
-  if (dtype == F32) rc = launch_dim<F32>(p, (hipStream_t)stream);
-  else if (dtype == BF16) rc = launch_dim<BF16>(p, (hipStream_t)stream);
-  else rc = launch_dim<F16>(p, (hipStream_t)stream);
+  if (dtype == F32) rc = launch_mode<F32>(p, vec, (hipStream_t)stream);
+  else if (dtype == BF16) rc = launch_mode<BF16>(p, vec, (hipStream_t)stream);
+  else rc = launch_mode<F16>(p, vec, (hipStream_t)stream);
   if (rc != SVA_OK || p.splits == 1) return rc;
   JoinParams j;
   j.part = p.part;
