@@ -10,9 +10,11 @@
 //    of one query row, and exactly the elements of P^T that the second
 //    product O^T = V^T P^T wants from it: weights stay in registers, a row's
 //    maximum takes one exchange between the wave's halves.
-//  * The reference m only moves when a tile's maximum passes it by 2^8: the
-//    sums are then rescaled.  Weights are at most 2^8 (fp16: 2^12, and 2^8 at
-//    the maximum, which keeps small ones out of fp16's subnormals).
+//  * The reference m is a maximum of the row's first keys and only moves when
+//    a lane's weights of a tile sum to more than 2^16 (fp16: 2^15): the tile's
+//    maximum is then taken, the sums rescaled and the weights done again.  The
+//    sum is needed anyway, so an ordinary tile looks for no maximum.  (fp16
+//    weights are 2^8 at a new reference, to keep small ones normal.)
 //  * Weights are rounded to the type of V for the product (2^-9 of each, of
 //    random sign, as V's own rounding); m, the sum of weights and the sums are
 //    fp32.  fp32 inputs use the fp32 matrix instructions throughout.
@@ -51,8 +53,29 @@ struct PromptParams {
   int64_t o_bs, o_hs, o_ts;
 };
 
+// Where 16-byte chunk ch of row r of a tile lies in LDS: ch ^ k_chunk(r) (K:
+// the rows of one column, 16 at a time, meet no bank twice) and ch ^
+// v_chunk(r) (V: nor do the four 64-byte row pieces of half a wave's
+// transposed read).  CPR: chunks of a row, 8 of them half of the banks.
+template <int CPR>
+SVA_DEV int k_chunk(int r) {
+  return CPR == 8 ? (r & 7) ^ (r >> 3 & 1) : r & 15;
+}
+template <int CPR>
+SVA_DEV int v_chunk(int r) {
+  return CPR == 8 ? 2 * (r & 3) : (4 * (r & 3)) ^ (r & 2);
+}
+
 template <int DT>
 struct PromptType {
+  using type = typename std::conditional<DT == BF16, __bf16, _Float16>::type;
+  typedef type pair __attribute__((ext_vector_type(2)));
+  // z + e[0] + e[1]: the sum of the weights as the second product takes them
+  static SVA_DEV float sum2(pair e, float z) {
+    const pair one = {(type)1.0f, (type)1.0f};
+    if constexpr (DT == BF16) return __builtin_amdgcn_fdot2_f32_bf16(e, one, z, false);
+    else return __builtin_amdgcn_fdot2(e, one, z, false);
+  }
   static constexpr int ES = DT == F32 ? 4 : 2;
   static constexpr int BN = DT == F32 ? 32 : 64;
   // waves per SIMD that the registers are kept to
@@ -80,8 +103,10 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
   constexpr int TB = BN * DP * ES;       // bytes of a K or V tile
   constexpr int NO = DP / 32;            // 32-element blocks of the sums
   constexpr float kLog2e = 1.44269504088896340736f;
-  constexpr float kSlack = DT == F16 ? 12.0f : 8.0f;   // how far a score may pass the reference
-  constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;    // how far below the maximum a new reference lies
+  constexpr float kMost = DT == F16 ? 32768.0f : 65536.0f;  // a lane's weights of a tile may sum to
+  constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;         // how far below the maximum a new reference lies
+  using Elem = PromptType<DT>;
+  using pair = typename Elem::pair;
   extern __shared__ __align__(16) unsigned char lds[];
   const int tid = (int)threadIdx.x, lane = lane_id(), w = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int l32 = lane & 31, hf = lane >> 5, m16 = lane & 15;
@@ -173,15 +198,19 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
   }
 
   u32x4 kr[CH], vr[CH];
+  // a thread's chunks lie 32-bit byte offsets from the tile's first row (checked by the host)
+  const uint32_t rowb = (uint32_t)p.kv_rs * ES;
   auto fetch = [&](int n0) {
+    const unsigned char* kp = (const unsigned char*)p.keys + (kvb + (int64_t)n0 * p.kv_rs) * ES;
+    const unsigned char* vp = (const unsigned char*)p.values + (kvb + (int64_t)n0 * p.kv_rs) * ES;
+    const int most = len - 1 - n0;  // rows past the end: the last key
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int idx = tid + 256 * c;
-      const int row = idx / CPR, ch = idx % CPR;
-      const int64_t e = kvb + (int64_t)min(n0 + row, len - 1) * p.kv_rs + ch * EC;  // past the end: the last key
+      const int row = min(idx / CPR, most), ch = idx % CPR;
       if constexpr (VEC) {
-        kr[c] = *(const u32x4*)((const unsigned char*)p.keys + e * ES);
-        vr[c] = *(const u32x4*)((const unsigned char*)p.values + e * ES);
+        kr[c] = *(const u32x4*)(kp + (row * rowb + ch * 16));
+        vr[c] = *(const u32x4*)(vp + (row * rowb + ch * 16));
       } else {
         union {
           u32x4 u;
@@ -191,12 +220,13 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
 #pragma unroll
         for (int i = 0; i < EC; ++i) {
           const bool in = ch * EC + i < p.D;
+          const uint32_t at = row * rowb + (ch * EC + i) * ES;
           if constexpr (ES == 4) {
-            a.x[i] = in ? ((const uint32_t*)p.keys)[e + i] : 0u;
-            v.x[i] = in ? ((const uint32_t*)p.values)[e + i] : 0u;
+            a.x[i] = in ? *(const uint32_t*)(kp + at) : 0u;
+            v.x[i] = in ? *(const uint32_t*)(vp + at) : 0u;
           } else {
-            a.h[i] = in ? ((const uint16_t*)p.keys)[e + i] : (uint16_t)0;
-            v.h[i] = in ? ((const uint16_t*)p.values)[e + i] : (uint16_t)0;
+            a.h[i] = in ? *(const uint16_t*)(kp + at) : (uint16_t)0;
+            v.h[i] = in ? *(const uint16_t*)(vp + at) : (uint16_t)0;
           }
         }
         kr[c] = a.u;
@@ -204,16 +234,13 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
       }
     }
   };
-  // chunk ch of row r lies at ch ^ (r % 8) (K: eight rows' chunks of one
-  // column meet no bank twice) and ch ^ 2 (r % 4) (V: as do the four rows of
-  // a transposed read)
   auto place = [&](unsigned char* buf) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int idx = tid + 256 * c;
       const int row = idx / CPR, ch = idx % CPR;
-      *(u32x4*)(buf + (row * CPR + (ch ^ (row & 7))) * 16) = kr[c];
-      *(u32x4*)(buf + TB + (row * CPR + (ES == 2 ? ch ^ ((row & 3) * 2) : ch)) * 16) = vr[c];
+      *(u32x4*)(buf + (row * CPR + (ch ^ k_chunk<CPR>(row))) * 16) = kr[c];
+      *(u32x4*)(buf + TB + (row * CPR + (ES == 2 ? ch ^ v_chunk<CPR>(row) : ch)) * 16) = vr[c];
     }
   };
 
@@ -238,7 +265,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
           for (int k = 0; k < 16; ++k) s[n][kt][k] = 0.0f;
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-          const frag a = *(const frag*)(kb + ((32 * kt + l32) * CPR + ((2 * f + hf) ^ (l32 & 7))) * 16);
+          const frag a = *(const frag*)(kb + ((32 * kt + l32) * CPR + ((2 * f + hf) ^ k_chunk<CPR>(l32))) * 16);
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
             if constexpr (DT == BF16) {
@@ -269,39 +296,50 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
               s[n][kt][k] = ok ? s[n][kt][k] : -INFINITY;
             }
       }
-      using pfrag = typename std::conditional<DT == F32, f32x4, frag>::type;
-      pfrag pw[NQ][KT][2];  // (unused for fp32, whose weights stay in s)
+      typename std::conditional<DT == F32, f32x16, frag[2]>::type pw[NQ][KT];  // the weights
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        float top = s[n][0][0];
+        auto weigh = [&]() {
+          float zs = 0.0f;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+          for (int kt = 0; kt < KT; ++kt) {
+            if constexpr (DT == F32) {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) top = fmaxf(top, s[n][kt][k]);
-        {
+              for (int k = 0; k < 16; ++k) {
+                pw[n][kt][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k], sl, -mref[n]));
+                zs += pw[n][kt][k];
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k], sl, -mref[n]));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k + 1], sl, -mref[n]));
+                pair e;
+                e[0] = (typename Elem::type)e0, e[1] = (typename Elem::type)e1;
+                pw[n][kt][k / 8][k % 8] = e[0], pw[n][kt][k / 8][k % 8 + 1] = e[1];
+                zs = Elem::sum2(e, zs);
+              }
+            }
+          }
+          return zs;
+        };
+        float zs = weigh();
+        if (__any(zs > kMost)) {  // (the first tile with a key always: the reference starts below every score)
+          float top = s[n][0][0];
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) top = fmaxf(top, s[n][kt][k]);
           const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-          top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-        }
-        top *= sl;
-        if (__any(top > mref[n] + kSlack)) {
+          top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * sl;
           const float mn = fmaxf(mref[n], top - kBelow);
           const float corr = __builtin_amdgcn_exp2f(mref[n] - mn);
           mref[n] = mn;
           z[n] *= corr;
 #pragma unroll
           for (int i = 0; i < NO; ++i) o[n][i] *= corr;
+          zs = weigh();
         }
-        float zs = 0.0f;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k], sl, -mref[n]));
-            zs += e;
-            if constexpr (DT == BF16) pw[n][kt][k / 8][k % 8] = (__bf16)e;
-            else if constexpr (DT == F16) pw[n][kt][k / 8][k % 8] = (_Float16)e;
-            else s[n][kt][k] = e;
-          }
         z[n] += zs;
       }
 #pragma unroll
@@ -315,7 +353,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
               const float a = vrow[32 * i + l32];
 #pragma unroll
               for (int n = 0; n < NQ; ++n)
-                o[n][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[n][kt][k], o[n][i], 0, 0, 0);
+                o[n][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pw[n][kt][k], o[n][i], 0, 0, 0);
             }
           }
         } else {
@@ -328,7 +366,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
                 frag v;
               } a;
               const int row = 32 * kt + 16 * st + 4 * hf + m16 / 4;
-              const int ch = (4 * i + 2 * (lane >> 4 & 1) + (m16 & 3) / 2) ^ (m16 / 4 * 2);
+              const int ch = (4 * i + 2 * (lane >> 4 & 1) + (m16 & 3) / 2) ^ v_chunk<CPR>(m16 / 4);
               const unsigned char* at = vb + (row * CPR + ch) * 16 + (m16 & 1) * 8;
               a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
               a.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(

@@ -82,6 +82,7 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   SVA_REQUIRE(n_keys < (1ll << 31) - 1024 && n_seq < (1ll << 31) && H < (1ll << 20) && Q < (1ll << 31) &&
                   H * Q < (1ll << 31) && n_seq * H < (1ll << 31) && n_seq * H * Q < (1ll << 31),
               "sva_prompt_attention: too many items or keys");
+  SVA_REQUIRE(kv_row_stride >= 0 && kv_row_stride < (1ll << 23), "sva_prompt_attention: row stride out of range");
   const size_t need = sva_prompt_attention_workspace_bytes(n_seq, H, G, Q, D, n_keys);
   SVA_REQUIRE(workspace != nullptr && workspace_bytes >= need, "sva_prompt_attention: workspace of %zu bytes required",
               need);
