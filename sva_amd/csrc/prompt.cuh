@@ -4,7 +4,7 @@
 // the keys row r may see, in one pass over the keys with a running reference
 // m.  The query rows of a KV head are (token, head of its group) pairs,
 // token-major, so one K / V tile serves every head of the group.  Four waves
-// of 32 * NQ query rows each share tiles of BN keys in LDS (two buffers: the
+// of 32 query rows each share tiles of BN keys in LDS (two buffers: the
 // next tile is loaded into registers while this one is used).
 //  * S^T = K Q^T (rows: keys) leaves each lane with half of the tile's scores
 //    of one query row, and exactly the elements of P^T that the second
@@ -79,7 +79,7 @@ struct PromptType {
   static constexpr int ES = DT == F32 ? 4 : 2;
   static constexpr int BN = DT == F32 ? 32 : 64;
   // waves per SIMD that the registers are kept to
-  static constexpr int waves(int dp, int nq) { return DT == F32 || dp * nq > 128 ? 1 : (dp * nq > 64 ? 2 : 3); }
+  static constexpr int waves(int dp) { return dp > 128 || (DT == F32 && dp > 64) ? 1 : 2; }
 };
 
 SVA_DEV bool prompt_mask_allows(const void* mask, int64_t i, int mtype) {
@@ -90,8 +90,8 @@ SVA_DEV bool prompt_mask_allows(const void* mask, int64_t i, int mtype) {
 // under the causal rule, the same under a mask, anything else.
 enum PromptMode : int { PROMPT_CAUSAL = 0, PROMPT_MASK = 1, PROMPT_ANY = 2 };
 
-template <int DT, int DP, int NQ, int MODE>
-__global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_kernel(PromptParams p) {
+template <int DT, int DP, int MODE>
+__global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(PromptParams p) {
   constexpr bool VEC = MODE != PROMPT_ANY;
   const bool MASK = MODE == PROMPT_MASK || (MODE == PROMPT_ANY && p.mask != nullptr);
   constexpr int ES = PromptType<DT>::ES, BN = PromptType<DT>::BN;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
   constexpr int CPR = DP * ES / 16;      // 16-byte chunks of a row
   constexpr int CH = BN * CPR / 256;     // chunks per thread
   constexpr int EC = 16 / ES;            // elements of a chunk
-  constexpr int BM = 4 * 32 * NQ;        // query rows of a workgroup
+  constexpr int BM = 4 * 32;             // query rows of a workgroup
   constexpr int TB = BN * DP * ES;       // bytes of a K or V tile
   constexpr int NO = DP / 32;            // 32-element blocks of the sums
   constexpr float kLog2e = 1.44269504088896340736f;
@@ -132,34 +132,36 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
   const int kbeg = split * p.chunk;
   const int kend = min(min(len, kbeg + p.chunk), MASK ? len : last_tok + shift + 1);
 
-  // this wave's rows, and per lane NQ of them
-  const int wrow = rt * BM + w * 32 * NQ;
-  const int wend = min(rows, wrow + 32 * NQ);
+  // this wave's rows, one per lane and half
+  const int wrow = rt * BM + w * 32;
+  const int wend = min(rows, wrow + 32);
   const bool busy = wrow < rows;
-  const int wfull = MASK ? 0 : min(len, wrow / grp + shift + 1);                  // keys below are seen by all rows
-  const int wlast = busy ? (MASK ? kend : min(kend, (wend - 1) / grp + shift + 1)) : 0;  // keys from here by none
-  int lim[NQ];                    // last key of the lane's row
-  const unsigned char* mrow[NQ] = {};  // its mask row
+  const int wfull = min(len, wrow / grp + shift + 1);  // keys below are seen by every row of the wave
   const int64_t kvb = (int64_t)g * p.kv_hs + off * p.kv_rs;  // element offset of key 0
   auto q_at = [&](int r, int64_t bs, int64_t hs, int64_t ts) {
     const int tok = r / grp, head = g * grp + r % grp;
     return (p.q_lens ? (q_first + tok) * ts : (int64_t)b * bs + (int64_t)tok * ts) + (int64_t)head * hs;
   };
   using frag = typename std::conditional<DT == BF16, bf16x8, typename std::conditional<DT == F16, f16x8, f32x4>::type>::type;
+  struct frag_pair {
+    frag v[2];
+    SVA_DEV frag& operator[](int i) { return v[i]; }
+    SVA_DEV const frag& operator[](int i) const { return v[i]; }
+  };
+  using weights = typename std::conditional<DT == F32, f32x16, frag_pair>::type;  // of 32 keys
   constexpr int NF = DT == F32 ? DP / 8 : DP / 16;  // fragments of a row per lane
   constexpr int FE = DT == F32 ? 4 : 8;             // elements of one: d = 2 FE f + FE hf + i
-  frag bq[NQ][NF];
-  const float sgn = p.scaling < 0.0f ? -1.0f : 1.0f;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = wrow + 32 * n + l32;
-    const bool live = r < rows;
-    lim[n] = live ? (MASK ? kend - 1 : min(kend - 1, r / grp + shift)) : -1;
-    if (MASK) {
-      const int64_t at = (int64_t)b * p.mask_bs + (int64_t)(live ? r / grp : 0) * p.mask_ts;
-      mrow[n] = (const unsigned char*)p.mask + at * (p.mask_type == MASK_F32 ? 4 : (p.mask_type == MASK_BOOL ? 1 : 2));
-    }
-    const int64_t at = q_at(live ? r : 0, p.q_bs, p.q_hs, p.q_ts);
+  const int row = wrow + l32;
+  const bool live = row < rows;
+  const int lim = live ? (MASK ? kend - 1 : min(kend - 1, row / grp + shift)) : -1;  // the last key of the row
+  const unsigned char* mrow = nullptr;                                                 // its mask row
+  if (MASK) {
+    const int64_t at = (int64_t)b * p.mask_bs + (int64_t)(live ? row / grp : 0) * p.mask_ts;
+    mrow = (const unsigned char*)p.mask + at * (p.mask_type == MASK_F32 ? 4 : (p.mask_type == MASK_BOOL ? 1 : 2));
+  }
+  frag bq[NF];
+  {
+    const int64_t at = q_at(live ? row : 0, p.q_bs, p.q_hs, p.q_ts);
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       const int d = 2 * FE * f + FE * hf;
@@ -169,237 +171,256 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
           frag v;
         } x;
         x.u = *(const u32x4*)((const unsigned char*)p.q + (at + d) * ES);
-        bq[n][f] = live ? x.v : frag{};
+        bq[f] = live ? x.v : frag{};
       } else {
 #pragma unroll
         for (int i = 0; i < FE; ++i) {
           const float x = live && d + i < p.D ? load_elem(p.q, at + d + i, DT) : 0.0f;
-          if constexpr (DT == BF16) bq[n][f][i] = (__bf16)x;
-          else if constexpr (DT == F16) bq[n][f][i] = (_Float16)x;
-          else bq[n][f][i] = x;
+          if constexpr (DT == BF16) bq[f][i] = (__bf16)x;
+          else if constexpr (DT == F16) bq[f][i] = (_Float16)x;
+          else bq[f][i] = x;
         }
       }
-      if (sgn < 0.0f) bq[n][f] = -bq[n][f];
+      if (p.scaling < 0.0f) bq[f] = -bq[f];
     }
   }
   // (a scale of 0: the smallest normal one gives the same weights, and -inf times it stays -inf)
   const float sl = fmaxf(fabsf(p.scaling) * kLog2e, 1.17549435e-38f);
 
-  f32x16 o[NQ][NO];
-  float mref[NQ], z[NQ];
+  f32x16 o[NO];
+  float mref = -3.0e38f, z = 0.0f;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    mref[n] = -3.0e38f;
-    z[n] = 0.0f;
+  for (int i = 0; i < NO; ++i)
 #pragma unroll
-    for (int i = 0; i < NO; ++i)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) o[n][i][k] = 0.0f;
-  }
+    for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
 
-  u32x4 kr[CH], vr[CH];
-  // a thread's chunks lie 32-bit byte offsets from the tile's first row (checked by the host)
+  // Tiles go to LDS as the loads return (whole aligned rows: 16 bytes a lane,
+  // a wave's 64 one after another; otherwise element by element through
+  // registers).  Slot i of a tile holds chunk i % CPR ^ swizzle(row) of row
+  // i / CPR: a lane's source lies a 32-bit byte offset from the tile's first
+  // row (checked by the host), the same for every tile but the last.
   const uint32_t rowb = (uint32_t)p.kv_rs * ES;
-  auto fetch = [&](int n0) {
-    const unsigned char* kp = (const unsigned char*)p.keys + (kvb + (int64_t)n0 * p.kv_rs) * ES;
-    const unsigned char* vp = (const unsigned char*)p.values + (kvb + (int64_t)n0 * p.kv_rs) * ES;
-    const int most = len - 1 - n0;  // rows past the end: the last key
+  auto swizzle = [&](int r, bool v) { return v ? (ES == 2 ? v_chunk<CPR>(r) : 0) : k_chunk<CPR>(r); };
+  uint32_t from[2][CH];
+#pragma unroll
+  for (int v = 0; v < 2; ++v)
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int idx = tid + 256 * c;
-      const int row = min(idx / CPR, most), ch = idx % CPR;
-      if constexpr (VEC) {
-        kr[c] = *(const u32x4*)(kp + (row * rowb + ch * 16));
-        vr[c] = *(const u32x4*)(vp + (row * rowb + ch * 16));
-      } else {
+      const int i = tid + 256 * c;
+      from[v][c] = i / CPR * rowb + (i % CPR ^ swizzle(i / CPR, v)) * 16;
+    }
+  auto load = [&](int v, int n0, unsigned char* buf) {
+    const unsigned char* tile =
+        (const unsigned char*)(v ? p.values : p.keys) + (kvb + (int64_t)n0 * p.kv_rs) * ES;
+    const int most = len - 1 - n0;  // rows past the end: the last key
+    if constexpr (VEC) {
+      const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)buf + w * 1024;
+      const bool last = most < BN - 1;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        uint32_t o = from[v][c];
+        if (last) {
+          const int r = (tid + 256 * c) / CPR;
+          if (r > most) o -= (uint32_t)(r - most) * rowb;
+        }
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                     :
+                     : "v"(o), "s"(tile), "s"(at + c * 4096)
+                     : "memory", "m0");
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int i = tid + 256 * c;
+        const int r = i / CPR, ch = i % CPR ^ swizzle(r, v);
+        const uint32_t o = min(r, most) * rowb + ch * 16;
         union {
           u32x4 u;
           uint16_t h[8];
-          uint32_t x[4];
-        } a, v;
+          uint32_t w[4];
+        } a;
 #pragma unroll
-        for (int i = 0; i < EC; ++i) {
-          const bool in = ch * EC + i < p.D;
-          const uint32_t at = row * rowb + (ch * EC + i) * ES;
-          if constexpr (ES == 4) {
-            a.x[i] = in ? *(const uint32_t*)(kp + at) : 0u;
-            v.x[i] = in ? *(const uint32_t*)(vp + at) : 0u;
-          } else {
-            a.h[i] = in ? *(const uint16_t*)(kp + at) : (uint16_t)0;
-            v.h[i] = in ? *(const uint16_t*)(vp + at) : (uint16_t)0;
-          }
+        for (int k = 0; k < EC; ++k) {
+          const bool in = ch * EC + k < p.D;
+          if constexpr (ES == 4) a.w[k] = in ? *(const uint32_t*)(tile + o + 4 * k) : 0u;
+          else a.h[k] = in ? *(const uint16_t*)(tile + o + 2 * k) : (uint16_t)0;
         }
-        kr[c] = a.u;
-        vr[c] = v.u;
+        *(u32x4*)(buf + i * 16) = a.u;
       }
     }
   };
-  auto place = [&](unsigned char* buf) {
+  // every load of this wave is in LDS, then every wave's
+  auto arrive = [&]() {
+    if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  // the steps of a tile: scores, masking, weights, sums
+  auto scores = [&](const unsigned char* kb, f32x16 (&s)[KT]) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      const int idx = tid + 256 * c;
-      const int row = idx / CPR, ch = idx % CPR;
-      *(u32x4*)(buf + (row * CPR + (ch ^ k_chunk<CPR>(row))) * 16) = kr[c];
-      *(u32x4*)(buf + TB + (row * CPR + (ES == 2 ? ch ^ v_chunk<CPR>(row) : ch)) * 16) = vr[c];
+    for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s[kt][k] = 0.0f;
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const frag a = *(const frag*)(kb + ((32 * kt + l32) * CPR + ((2 * f + hf) ^ k_chunk<CPR>(l32))) * 16);
+        if constexpr (DT == BF16) {
+          s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, bq[f], s[kt], 0, 0, 0);
+        } else if constexpr (DT == F16) {
+          s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bq[f], s[kt], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], bq[f][i], s[kt], 0, 0, 0);
+        }
+      }
+    }
+  };
+  // a lane's score k of block kt is key n0 + 32 kt + 8 (k / 4) + 4 hf + k % 4
+  auto hide = [&](int n0, f32x16 (&s)[KT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int key = n0 + 32 * kt + 8 * (k / 4) + 4 * hf + k % 4;
+        bool ok = key <= lim;
+        if (MASK) {
+          if (ok) ok = prompt_mask_allows(mrow, key, p.mask_type);
+        }
+        s[kt][k] = ok ? s[kt][k] : -INFINITY;
+      }
+  };
+  auto weigh = [&](const f32x16 (&s)[KT], weights (&pw)[KT]) {
+    float zs = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      if constexpr (DT == F32) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          pw[kt][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][k], sl, -mref));
+          zs += pw[kt][k];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][k], sl, -mref));
+          const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][k + 1], sl, -mref));
+          pair e;
+          e[0] = (typename Elem::type)e0, e[1] = (typename Elem::type)e1;
+          pw[kt][k / 8][k % 8] = e[0], pw[kt][k / 8][k % 8 + 1] = e[1];
+          zs = Elem::sum2(e, zs);
+        }
+      }
+    }
+    return zs;
+  };
+  // where a tile's weights sum to more than kMost (the first one's with a key
+  // always: the reference starts below every score), the reference moves to
+  // its maximum
+  auto settle = [&](float zs, const f32x16 (&s)[KT], weights (&pw)[KT]) {
+    if (__any(zs > kMost)) {
+      float top = s[0][0];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) top = fmaxf(top, s[kt][k]);
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * sl;
+      const float mn = fmaxf(mref, top - kBelow);
+      const float corr = __builtin_amdgcn_exp2f(mref - mn);
+      mref = mn;
+      z *= corr;
+#pragma unroll
+      for (int i = 0; i < NO; ++i) o[i] *= corr;
+      zs = weigh(s, pw);
+    }
+    z += zs;
+  };
+  auto sums = [&](const unsigned char* vb, const weights (&pw)[KT]) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      if constexpr (DT == F32) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float* vrow = (const float*)(vb + (32 * kt + 8 * (k / 4) + 4 * hf + k % 4) * CPR * 16);
+#pragma unroll
+          for (int i = 0; i < NO; ++i)
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[32 * i + l32], pw[kt][k], o[i], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+#pragma unroll
+          for (int i = 0; i < NO; ++i) {
+            union {
+              s16x4 half[2];
+              frag v;
+            } a;
+            const int row = 32 * kt + 16 * st + 4 * hf + m16 / 4;
+            const int ch = (4 * i + 2 * (lane >> 4 & 1) + (m16 & 3) / 2) ^ v_chunk<CPR>(m16 / 4);
+            const unsigned char* at = vb + (row * CPR + ch) * 16 + (m16 & 1) * 8;
+            a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+            a.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(at + 8 * CPR * 16));
+            if constexpr (DT == BF16) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, pw[kt][st], o[i], 0, 0, 0);
+            else o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.v, pw[kt][st], o[i], 0, 0, 0);
+          }
+        }
+      }
     }
   };
 
-  int cur = 0;
-  if (kbeg < kend) {
-    fetch(kbeg);
-    place(lds);
-  }
-  __syncthreads();
-  for (int n0 = kbeg; n0 < kend; n0 += BN) {
-    const bool more = n0 + BN < kend;
-    if (more) fetch(n0 + BN);
-    if (n0 < wlast) {
-      const unsigned char* kb = lds + cur * 2 * TB;
-      const unsigned char* vb = kb + TB;
-      f32x16 s[NQ][KT];
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int k = 0; k < 16; ++k) s[n][kt][k] = 0.0f;
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const frag a = *(const frag*)(kb + ((32 * kt + l32) * CPR + ((2 * f + hf) ^ k_chunk<CPR>(l32))) * 16);
-#pragma unroll
-          for (int n = 0; n < NQ; ++n) {
-            if constexpr (DT == BF16) {
-              s[n][kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, bq[n][f], s[n][kt], 0, 0, 0);
-            } else if constexpr (DT == F16) {
-              s[n][kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bq[n][f], s[n][kt], 0, 0, 0);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                s[n][kt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], bq[n][f][i], s[n][kt], 0, 0, 0);
-            }
-          }
-        }
+  // Tile t's scores are taken while tile t - 1 is weighed and tile t - 2's
+  // sums are added: the matrix and the vector instructions of one step do not
+  // wait for one another.  K is a tile ahead of that, V two behind it.
+  unsigned char* const kbuf = lds;
+  unsigned char* const vbuf = lds + 2 * TB;
+  const int nt = (kend - kbeg + BN - 1) / BN;
+  if (nt > 0) {
+    f32x16 s[KT], s2[KT];
+    weights pw[KT], pw2[KT];
+    auto step = [&](int t, f32x16 (&sc)[KT], f32x16 (&sn)[KT], weights (&pc)[KT], weights (&pp)[KT], bool first) {
+      // weigh tile t (scores sc) into pc, add tile t - 1 (weights pp), score tile t + 1 into sn
+      const int n0 = kbeg + t * BN;
+      if (t + 2 < nt) load(0, n0 + 2 * BN, kbuf + (t & 1) * TB);
+      load(1, n0, vbuf + (t & 1) * TB);
+      if (busy) {
+        if (MASK || n0 + BN > wfull) hide(n0, sc);
+        scores(kbuf + ((t + 1) & 1) * TB, sn);  // (behind the last tile: not used)
+        if (!first) sums(vbuf + ((t + 1) & 1) * TB, pp);
+        const float zs = weigh(sc, pc);
+        settle(zs, sc, pc);
       }
-      // a lane's score k of block kt is key n0 + 32 kt + 8 (k / 4) + 4 hf + k % 4
-      if (MASK || n0 + BN > wfull) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int key = n0 + 32 * kt + 8 * (k / 4) + 4 * hf + k % 4;
-              bool ok = key <= lim[n];
-              if (MASK) {
-                if (ok) ok = prompt_mask_allows(mrow[n], key, p.mask_type);
-              }
-              s[n][kt][k] = ok ? s[n][kt][k] : -INFINITY;
-            }
-      }
-      typename std::conditional<DT == F32, f32x16, frag[2]>::type pw[NQ][KT];  // the weights
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        auto weigh = [&]() {
-          float zs = 0.0f;
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            if constexpr (DT == F32) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                pw[n][kt][k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k], sl, -mref[n]));
-                zs += pw[n][kt][k];
-              }
-            } else {
-#pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k], sl, -mref[n]));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][kt][k + 1], sl, -mref[n]));
-                pair e;
-                e[0] = (typename Elem::type)e0, e[1] = (typename Elem::type)e1;
-                pw[n][kt][k / 8][k % 8] = e[0], pw[n][kt][k / 8][k % 8 + 1] = e[1];
-                zs = Elem::sum2(e, zs);
-              }
-            }
-          }
-          return zs;
-        };
-        float zs = weigh();
-        if (__any(zs > kMost)) {  // (the first tile with a key always: the reference starts below every score)
-          float top = s[n][0][0];
-#pragma unroll
-          for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) top = fmaxf(top, s[n][kt][k]);
-          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-          top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * sl;
-          const float mn = fmaxf(mref[n], top - kBelow);
-          const float corr = __builtin_amdgcn_exp2f(mref[n] - mn);
-          mref[n] = mn;
-          z[n] *= corr;
-#pragma unroll
-          for (int i = 0; i < NO; ++i) o[n][i] *= corr;
-          zs = weigh();
-        }
-        z[n] += zs;
-      }
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        if constexpr (DT == F32) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float* vrow = (const float*)(vb + (32 * kt + 8 * (k / 4) + 4 * hf + k % 4) * CPR * 16);
-#pragma unroll
-            for (int i = 0; i < NO; ++i) {
-              const float a = vrow[32 * i + l32];
-#pragma unroll
-              for (int n = 0; n < NQ; ++n)
-                o[n][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, pw[n][kt][k], o[n][i], 0, 0, 0);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int st = 0; st < 2; ++st) {
-#pragma unroll
-            for (int i = 0; i < NO; ++i) {
-              union {
-                s16x4 half[2];
-                frag v;
-              } a;
-              const int row = 32 * kt + 16 * st + 4 * hf + m16 / 4;
-              const int ch = (4 * i + 2 * (lane >> 4 & 1) + (m16 & 3) / 2) ^ v_chunk<CPR>(m16 / 4);
-              const unsigned char* at = vb + (row * CPR + ch) * 16 + (m16 & 1) * 8;
-              a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-              a.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) s16x4*)(at + 8 * CPR * 16));
-#pragma unroll
-              for (int n = 0; n < NQ; ++n) {
-                if constexpr (DT == BF16)
-                  o[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, pw[n][kt][st], o[n][i], 0, 0, 0);
-                else
-                  o[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.v, pw[n][kt][st], o[n][i], 0, 0, 0);
-              }
-            }
-          }
-        }
-      }
+      arrive();
+    };
+    load(0, kbeg, kbuf);
+    if (nt > 1) load(0, kbeg + BN, kbuf + TB);
+    arrive();
+    if (busy) scores(kbuf, s);
+    __syncthreads();  // (tile 2 takes tile 0's place)
+    step(0, s, s2, pw, pw2, true);
+    int t = 1;
+    for (; t + 1 < nt; t += 2) {
+      step(t, s2, s, pw2, pw, false);
+      step(t + 1, s, s2, pw, pw2, false);
     }
-    cur ^= 1;
-    if (more) place(lds + cur * 2 * TB);
-    __syncthreads();
+    if (t < nt) {
+      step(t, s2, s, pw2, pw, false);
+      if (busy) sums(vbuf + (t & 1) * TB, pw2);
+    } else if (busy) {
+      sums(vbuf + ((t - 1) & 1) * TB, pw);
+    }
   }
   if (!busy) return;
 
   // the two halves of the wave hold a row's keys
+  {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(z), __float_as_uint(z), false, false);
+    z = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
   bool odd = false;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(z[n]), __float_as_uint(z[n]), false, false);
-    z[n] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  for (int i = 0; i < NO; ++i)
 #pragma unroll
-    for (int i = 0; i < NO; ++i)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) odd = odd || !(fabsf(o[n][i][k]) <= 3.40282347e38f);
-  }
+    for (int k = 0; k < 16; ++k) odd = odd || !(fabsf(o[i][k]) <= 3.40282347e38f);
   auto part_at = [&](int r) {
     const int tok = r / grp, head = g * grp + r % grp;
     return p.part + ((((int64_t)b * p.H + head) * p.Q + tok) * p.splits + split) * (p.D + 2);
@@ -458,24 +479,20 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP, NQ)) prompt_ker
     }
     return;
   }
+  if (!live) return;
+  float* part = p.splits > 1 ? part_at(row) : nullptr;
+  const int64_t at = q_at(row, p.o_bs, p.o_hs, p.o_ts);
+  const float f = part ? 1.0f : (z == 0.0f ? 0.0f : 1.0f / z);
+  if (part && hf == 0) part[0] = mref, part[1] = z;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int r = wrow + 32 * n + l32;
-    if (r >= rows) continue;
-    float* part = p.splits > 1 ? part_at(r) : nullptr;
-    const int64_t at = q_at(r, p.o_bs, p.o_hs, p.o_ts);
-    const float f = part ? 1.0f : (z[n] == 0.0f ? 0.0f : 1.0f / z[n]);
-    if (part && hf == 0) part[0] = mref[n], part[1] = z[n];
+  for (int i = 0; i < NO; ++i)
 #pragma unroll
-    for (int i = 0; i < NO; ++i)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const int d = 32 * i + 8 * (k / 4) + 4 * hf + k % 4;
-        if (d >= p.D) continue;
-        if (part) part[2 + d] = o[n][i][k];
-        else store_elem(p.out, at + d, p.out_dtype, o[n][i][k] * f);
-      }
-  }
+    for (int k = 0; k < 16; ++k) {
+      const int d = 32 * i + 8 * (k / 4) + 4 * hf + k % 4;
+      if (d >= p.D) continue;
+      if (part) part[2 + d] = o[i][k];
+      else store_elem(p.out, at + d, p.out_dtype, o[i][k] * f);
+    }
 }
 
 }  // namespace sva

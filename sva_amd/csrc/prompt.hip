@@ -26,7 +26,7 @@ int64_t chunk_keys(int64_t tiles, int64_t n_keys) {
 template <int DT, int DP, int MODE>
 int launch(const PromptParams& p, hipStream_t stream) {
   constexpr int lds = 4 * PromptType<DT>::BN * DP * PromptType<DT>::ES;
-  constexpr auto fn = prompt_kernel<DT, DP, 1, MODE>;
+  constexpr auto fn = prompt_kernel<DT, DP, MODE>;
   SVA_SET_MAX_LDS_ONCE(fn, sva::kMaxLds, "hipFuncSetAttribute(prompt_kernel)");
   const int64_t blocks = (int64_t)p.G * p.row_tiles * p.splits * p.n_seq;
   hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), lds, stream, p);
