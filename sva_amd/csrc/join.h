@@ -8,15 +8,28 @@
 namespace sva {
 
 struct JoinParams {
-  const float* part;  // [n_seq * H * Q, splits, D + 2]: m, z, sums; z = 0: no key in the range, the sums are not read
-  int splits, H, Q, D;
+  const float* sums;   // [n_seq * H * Q, splits, D]
+  const float* stats;  // [n_seq * H * Q, splits, 2]: m, z; z = 0: the range has no key, its sums are not read
+  int splits, H, G, Q, D;
   const int64_t* q_lens;     // packed tokens: sequence b's are rows q_offsets[b] + t, t < q_lens[b], of q_rows;
   const int64_t* q_offsets;  // NULL: Q tokens of every sequence
   int64_t q_rows;
+  const int64_t* lens;  // keys: seq_keys
+  const int64_t* offs;
+  int64_t N, rows;
+  int tile_rows;  // query rows that one workgroup takes
+  int chunk;      // keys of a range
+  bool causal;
   void* out;
   int out_dtype;
   int64_t o_bs, o_hs, o_ts;
 };
+
+// Bytes of the sums and stats of `items` items, the stats' first.
+inline size_t join_bytes(int64_t items, int64_t splits, int64_t D) {
+  return sizeof(float) * (size_t)(items * splits) * (size_t)(D + 2) + 256;
+}
+inline int64_t join_stats_floats(int64_t items, int64_t splits) { return (items * splits * 2 + 3) / 4 * 4; }
 
 int launch_join(const JoinParams& p, int64_t n_seq, hipStream_t stream);
 
@@ -31,6 +44,32 @@ __device__ inline int seq_tokens(const int64_t* q_lens, const int64_t* q_offsets
   n = n < q_rows - first ? n : q_rows - first;
   n = n < Q ? n : Q;
   return n > 0 ? (int)n : 0;
+}
+
+// Keys of sequence b and the cache row of its first, inside [0, rows) and no
+// more than N.
+__device__ inline int64_t seq_keys(const int64_t* lens, const int64_t* offs, int64_t N, int64_t rows, int b,
+                                   int64_t& off) {
+  off = offs ? offs[b] : 0;
+  if (off < 0 || off >= rows) return 0;
+  int64_t n = lens ? lens[b] : N;
+  n = n < N ? n : N;
+  n = n < rows - off ? n : rows - off;
+  return n > 0 ? n : 0;
+}
+
+// The end of the keys that some row of tile rt sees, of q_len tokens x grp
+// heads over len keys, and the ranges of `chunk` keys up to it (at least 1).
+// A tile of one range writes its outputs itself; the others are joined.
+__device__ inline int64_t tile_keys(int rt, int tile_rows, int q_len, int grp, int64_t len, bool causal) {
+  if (!causal) return len;
+  const int64_t rows = (int64_t)q_len * grp, end = (int64_t)(rt + 1) * tile_rows;
+  const int64_t last_token = ((end < rows ? end : rows) - 1) / grp;
+  const int64_t keys = last_token + len - q_len + 1;
+  return keys < 0 ? 0 : (keys < len ? keys : len);
+}
+__device__ inline int tile_ranges(int64_t keys, int64_t chunk) {
+  return keys <= chunk ? 1 : (int)((keys + chunk - 1) / chunk);
 }
 
 }  // namespace sva

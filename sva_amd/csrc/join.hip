@@ -7,35 +7,71 @@
 namespace sva {
 namespace {
 
-constexpr int JB = 256;  // 32 elements x 8 ranges at a time
+constexpr int JB = 512;  // 32 elements x 16 ranges
+constexpr int RB = 256;
 
+struct JoinItem {
+  const float* sums;   // [ranges, D]
+  const float* stats;  // [ranges, 2]
+  int ranges;          // 1: nothing to join
+  int64_t at;          // its output
+};
+
+SVA_DEV JoinItem join_item(const JoinParams& p, int item) {
+  JoinItem x;
+  const int t = item % p.Q, h = item / p.Q % p.H, b = item / (p.Q * p.H);
+  int64_t first, off;
+  const int q_len = seq_tokens(p.q_lens, p.q_offsets, p.q_rows, p.Q, b, first);
+  x.ranges = 1;
+  if (t >= q_len) return x;
+  const int64_t len = seq_keys(p.lens, p.offs, p.N, p.rows, b, off);
+  const int grp = p.H / p.G;
+  const int rt = (int)(((int64_t)t * grp + h % grp) / p.tile_rows);
+  x.ranges = tile_ranges(tile_keys(rt, p.tile_rows, q_len, grp, len, p.causal), p.chunk);
+  x.sums = p.sums + (int64_t)item * p.splits * p.D;
+  x.stats = p.stats + (int64_t)item * p.splits * 2;
+  x.at = (p.q_lens ? (first + t) * p.o_ts : (int64_t)b * p.o_bs + (int64_t)t * p.o_ts) + (int64_t)h * p.o_hs;
+  return x;
+}
+
+// A range's share of the joined sums: 2^(m - M).  (A range without a key has
+// sums of 0; one done again whose scores are all NaN has m = -inf and z NaN.)
+SVA_DEV float join_share(float m, float M) { return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M); }
+
+// Few items of many ranges (decode): a workgroup takes 32 elements of one
+// item, 16 ranges at a time, eight rounds of loads in flight: 256 ranges are
+// two round trips.
 __global__ void __launch_bounds__(JB) join_kernel(JoinParams p) {
   __shared__ float red[2][JB];
   __shared__ float top[JB / WAVE];
-  const int item = (int)blockIdx.x, d = (int)blockIdx.y * 32 + (int)threadIdx.x % 32, lane8 = (int)threadIdx.x / 32;
-  const int t = item % p.Q, h = item / p.Q % p.H, b = item / (p.Q * p.H);
-  int64_t first;
-  if (t >= seq_tokens(p.q_lens, p.q_offsets, p.q_rows, p.Q, b, first)) return;
-  const float* src = p.part + (int64_t)item * p.splits * (p.D + 2);
+  const JoinItem x = join_item(p, (int)blockIdx.x);
+  const int d = (int)blockIdx.y * 32 + (int)threadIdx.x % 32, part = (int)threadIdx.x / 32;
+  if (x.ranges == 1) return;
+  constexpr int U = 8, PARTS = JB / 32;
   float M = -INFINITY;
-  for (int s = (int)threadIdx.x; s < p.splits; s += JB) {
-    const float* f = src + (int64_t)s * (p.D + 2);
-    if (f[1] != 0.0f) M = fmaxf(M, f[0]);
-  }
+  for (int s = (int)threadIdx.x; s < x.ranges; s += JB) M = fmaxf(M, x.stats[2 * s]);
   M = wave_max(M);
   if (lane_id() == 0) top[threadIdx.x / WAVE] = M;
   __syncthreads();
 #pragma unroll
   for (int v = 0; v < JB / WAVE; ++v) M = fmaxf(M, top[v]);
   float Z = 0.0f, a = 0.0f;
-#pragma unroll 4
-  for (int s = lane8; s < p.splits; s += JB / 32) {
-    const float* f = src + (int64_t)s * (p.D + 2);
-    const float m = f[0], z = f[1];
-    if (z != 0.0f) {  // (a NaN counts)
-      const float c = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
-      Z += z * c;
-      if (d < p.D) a += f[2 + d] * c;
+  for (int s0 = part; s0 < x.ranges; s0 += U * PARTS) {
+    float2 st[U];
+    float sm[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = min(s0 + u * PARTS, x.ranges - 1);
+      st[u] = *(const float2*)(x.stats + 2 * s);
+      sm[u] = x.sums[(int64_t)s * p.D + min(d, p.D - 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float c = s0 + u * PARTS < x.ranges ? join_share(st[u].x, M) : 0.0f;
+      if (c != 0.0f) {
+        Z += st[u].y * c;
+        a += sm[u] * c;
+      }
     }
   }
   red[0][threadIdx.x] = a;
@@ -48,18 +84,42 @@ __global__ void __launch_bounds__(JB) join_kernel(JoinParams p) {
       a += red[0][32 * v + threadIdx.x];
       Z += red[1][32 * v + threadIdx.x];
     }
-    const int64_t at = (p.q_lens ? (first + t) * p.o_ts : (int64_t)b * p.o_bs + (int64_t)t * p.o_ts) +
-                       (int64_t)h * p.o_hs + d;
-    store_elem(p.out, at, p.out_dtype, Z == 0.0f ? 0.0f : a / Z);
+    store_elem(p.out, x.at + d, p.out_dtype, Z == 0.0f ? 0.0f : a / Z);
+  }
+}
+
+// Many items of few ranges (prompts): a wave an item, 64 elements at a time.
+__global__ void __launch_bounds__(RB) join_rows_kernel(JoinParams p, int items) {
+  const int item = (int)blockIdx.x * (RB / WAVE) + (int)threadIdx.x / WAVE;
+  if (item >= items) return;
+  const JoinItem x = join_item(p, item);
+  if (x.ranges == 1) return;
+  float M = -INFINITY, Z = 0.0f;
+  for (int s = 0; s < x.ranges; ++s) M = fmaxf(M, x.stats[2 * s]);
+  for (int s = 0; s < x.ranges; ++s) Z += x.stats[2 * s + 1] * join_share(x.stats[2 * s], M);
+  for (int d = lane_id(); d < p.D; d += WAVE) {
+    float a = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < x.ranges; ++s) {
+      const float c = join_share(x.stats[2 * s], M);
+      a += c == 0.0f ? 0.0f : x.sums[(int64_t)s * p.D + d] * c;
+    }
+    store_elem(p.out, x.at + d, p.out_dtype, Z == 0.0f ? 0.0f : a / Z);
   }
 }
 
 }  // namespace
 
 int launch_join(const JoinParams& p, int64_t n_seq, hipStream_t stream) {
-  hipLaunchKernelGGL(join_kernel, dim3((unsigned)(n_seq * p.H * p.Q), (unsigned)((p.D + 31) / 32)), dim3(JB), 0,
-                     stream, p);
-  SVA_CHECK_LAUNCH("join_kernel");
+  const int64_t items = n_seq * p.H * p.Q;
+  if (items <= 1024) {
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)items, (unsigned)((p.D + 31) / 32)), dim3(JB), 0, stream, p);
+    SVA_CHECK_LAUNCH("join_kernel");
+  } else {
+    hipLaunchKernelGGL(join_rows_kernel, dim3((unsigned)((items + RB / WAVE - 1) / (RB / WAVE))), dim3(RB), 0, stream, p,
+                       (int)items);
+    SVA_CHECK_LAUNCH("join_rows_kernel");
+  }
   return SVA_OK;
 }
 

@@ -22,6 +22,8 @@
 //    survives: a wave whose sums are not finite does its rows again, key by
 //    key, over the keys they may see alone.
 #pragma once
+// (loads to LDS name m0 among what they change)
+#pragma clang diagnostic ignored "-Winline-asm"
 #include "cache4.h"
 #include "join.h"
 
@@ -47,9 +49,11 @@ struct PromptParams {
   const void* mask;
   int mask_type;
   int64_t mask_bs, mask_ts;
-  float* part;
+  float* sums;   // join.h
+  float* stats;
   void* out;
   int out_dtype;
+  bool out_vec;  // four elements of an output row are one aligned store
   int64_t o_bs, o_hs, o_ts;
 };
 
@@ -124,13 +128,15 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   const int q_len = seq_tokens(p.q_lens, p.q_offsets, p.q_rows, p.Q, b, q_first);
   const int rows = q_len * grp;
   if (rt * BM >= rows) return;
-  const int64_t off = p.offs ? p.offs[b] : 0;
-  int64_t len64 = min(min(p.lens ? p.lens[b] : p.N, p.N), p.kv_rows - off);
-  const int len = off < 0 || len64 < 0 ? 0 : (int)len64;
+  int64_t off;
+  const int len = (int)seq_keys(p.lens, p.offs, p.N, p.kv_rows, b, off);
   const int shift = len - q_len;  // token t sees keys n <= t + shift
-  const int last_tok = (min(rows, (rt + 1) * BM) - 1) / grp;
+  const int keys = (int)tile_keys(rt, BM, q_len, grp, len, !MASK);
+  const int ranges = tile_ranges(keys, p.chunk);
+  if (split >= ranges) return;
+  const bool partial = ranges > 1;  // joined by a second kernel
   const int kbeg = split * p.chunk;
-  const int kend = min(min(len, kbeg + p.chunk), MASK ? len : last_tok + shift + 1);
+  const int kend = min(keys, kbeg + p.chunk);
 
   // this wave's rows, one per lane and half
   const int wrow = rt * BM + w * 32;
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
     for (int k = 0; k < 16; ++k) odd = odd || !(fabsf(o[i][k]) <= 3.40282347e38f);
   auto part_at = [&](int r) {
     const int tok = r / grp, head = g * grp + r % grp;
-    return p.part + ((((int64_t)b * p.H + head) * p.Q + tok) * p.splits + split) * (p.D + 2);
+    return (((int64_t)b * p.H + head) * p.Q + tok) * p.splits + split;
   };
   if (__any(odd)) {
     // again, key by key: lanes take 64 keys' scores, then the row's elements
@@ -470,28 +476,45 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
       for (int k = 0; k < DP / 64; ++k) {
         const int d = lane + 64 * k;
         if (d >= p.D) continue;
-        if (p.splits > 1)
-          part_at(r)[2 + d] = acc[k];
+        if (partial)
+          p.sums[part_at(r) * p.D + d] = acc[k];
         else
           store_elem(p.out, q_at(r, p.o_bs, p.o_hs, p.o_ts) + d, p.out_dtype, zz == 0.0f ? 0.0f : acc[k] / zz);
       }
-      if (p.splits > 1 && lane == 0) part_at(r)[0] = m, part_at(r)[1] = zz;
+      if (partial && lane == 0) p.stats[2 * part_at(r)] = m, p.stats[2 * part_at(r) + 1] = zz;
     }
     return;
   }
   if (!live) return;
-  float* part = p.splits > 1 ? part_at(row) : nullptr;
-  const int64_t at = q_at(row, p.o_bs, p.o_hs, p.o_ts);
-  const float f = part ? 1.0f : (z == 0.0f ? 0.0f : 1.0f / z);
-  if (part && hf == 0) part[0] = mref, part[1] = z;
+  // four consecutive elements at a time
+  void* dst = partial ? (void*)p.sums : p.out;
+  const int type = partial ? (int)F32 : p.out_dtype;
+  const int64_t at = partial ? part_at(row) * p.D : q_at(row, p.o_bs, p.o_hs, p.o_ts);
+  const float f = partial ? 1.0f : (z == 0.0f ? 0.0f : 1.0f / z);
+  if (partial && hf == 0) p.stats[2 * part_at(row)] = mref, p.stats[2 * part_at(row) + 1] = z;
+  const bool whole = partial ? p.D % 4 == 0 : p.out_vec;
 #pragma unroll
   for (int i = 0; i < NO; ++i)
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int d = 32 * i + 8 * (k / 4) + 4 * hf + k % 4;
+    for (int k = 0; k < 16; k += 4) {
+      const int d = 32 * i + 2 * k + 4 * hf;
       if (d >= p.D) continue;
-      if (part) part[2 + d] = o[i][k];
-      else store_elem(p.out, at + d, p.out_dtype, o[i][k] * f);
+      const float x[4] = {o[i][k] * f, o[i][k + 1] * f, o[i][k + 2] * f, o[i][k + 3] * f};
+      if (whole) {
+        if (type == F32) {
+          *(f32x4*)((float*)dst + at + d) = f32x4{x[0], x[1], x[2], x[3]};
+        } else {
+          uint16_t h[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) store_elem(h, j, type, x[j]);
+          *(uint2*)((uint16_t*)dst + at + d) =
+              make_uint2((uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (d + j < p.D) store_elem(dst, at + d + j, type, x[j]);
+      }
     }
 }
 

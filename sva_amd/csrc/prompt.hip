@@ -16,11 +16,22 @@ constexpr int BM = 128;  // query rows of a workgroup
 
 int64_t row_tiles(int64_t H, int64_t G, int64_t Q) { return (H / G * Q + BM - 1) / BM; }
 
-// Keys per workgroup: all of them where the row tiles alone fill the card,
-// otherwise ranges of at least 512.
-int64_t chunk_keys(int64_t tiles, int64_t n_keys) {
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(64, 768 / tiles));
-  return std::max<int64_t>(512, ((n_keys + want - 1) / want + 63) / 64 * 64);
+// Keys per workgroup: all of them, or ranges of at least 256.  The row tiles
+// of whole prompts are of every length, and dispatch evens them out: they are
+// split only where they do not fill the card once.  Tokens over a cache that
+// is much longer make row tiles of one length: about five workgroups for each
+// of the two places of a CU, so that a last round of them is a small part.
+// Ranges cost a second launch and their sums' way through memory.  (9 x 64
+// bf16: 8192 whole tokens 120 us in one range, 145 with a second behind key
+// 4736; 512 tokens each over 8 x 32768 keys 530 us in two ranges, 450 in
+// seven, 520 in 16; a token each of 32 sequences of up to 131072 keys 376 us
+// in eight, 289 in 28, 318 in 64; 12 x 64 fp32, 1001 tokens 77 us in one, 54 in
+// two.)
+int64_t chunk_keys(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t n_keys) {
+  const int64_t tiles = n_seq * G * row_tiles(H, G, Q), cus = sva::device_cu_count();
+  const int64_t want = 2 * Q > n_keys ? (cus + tiles - 1) / tiles : (10 * cus + tiles / 2) / tiles;
+  const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(64, want));
+  return std::max<int64_t>(256, ((n_keys + ranges - 1) / ranges + 63) / 64 * 64);
 }
 
 template <int DT, int DP, int MODE>
@@ -52,9 +63,9 @@ int launch_mode(const PromptParams& p, bool vec, hipStream_t stream) {
 extern "C" size_t sva_prompt_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D,
                                                        int64_t n_keys) {
   if (n_seq <= 0 || H <= 0 || G <= 0 || Q <= 0 || D <= 0 || n_keys <= 0 || H % G != 0) return 0;
-  const int64_t chunk = chunk_keys(n_seq * G * row_tiles(H, G, Q), n_keys);
+  const int64_t chunk = chunk_keys(n_seq, H, G, Q, n_keys);
   const int64_t splits = (n_keys + chunk - 1) / chunk;
-  return splits == 1 ? 256 : sizeof(float) * (size_t)(n_seq * H * Q) * (size_t)splits * (size_t)(D + 2) + 256;
+  return splits == 1 ? 256 : join_bytes(n_seq * H * Q, splits, D);
 }
 
 extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stride, int64_t q_head_stride,
@@ -109,7 +120,7 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   p.Q = (int)Q;
   p.D = (int)D;
   p.row_tiles = (int)row_tiles(H, G, Q);
-  p.chunk = (int)chunk_keys(n_seq * G * p.row_tiles, n_keys);
+  p.chunk = (int)chunk_keys(n_seq, H, G, Q, n_keys);
   p.splits = (int)((n_keys + p.chunk - 1) / p.chunk);
   const bool vec = (D == 64 || D == 128 || D == 256) && (((uintptr_t)q | (uintptr_t)keys | (uintptr_t)values) & 15u) == 0 &&
                    q_seq_stride % word == 0 && q_head_stride % word == 0 && q_tok_stride % word == 0 &&
@@ -119,9 +130,12 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   p.mask_type = mask_type;
   p.mask_bs = mask_seq_stride;
   p.mask_ts = mask_tok_stride;
-  p.part = (float*)workspace;
+  p.stats = (float*)workspace;
+  p.sums = p.stats + join_stats_floats(n_seq * H * Q, p.splits);
   p.out = out;
   p.out_dtype = out_dtype;
+  p.out_vec = D % 4 == 0 && ((uintptr_t)out & 15u) == 0 && out_seq_stride % 4 == 0 && out_head_stride % 4 == 0 &&
+              out_tok_stride % 4 == 0;
   p.o_bs = out_seq_stride;
   p.o_hs = out_head_stride;
   p.o_ts = out_tok_stride;
@@ -132,9 +146,18 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   else rc = launch_mode<F16>(p, vec, (hipStream_t)stream);
   if (rc != SVA_OK || p.splits == 1) return rc;
   JoinParams j;
-  j.part = p.part;
+  j.sums = p.sums;
+  j.stats = p.stats;
   j.splits = p.splits;
   j.H = p.H;
+  j.G = p.G;
+  j.lens = seq_lens;
+  j.offs = seq_offsets;
+  j.N = n_keys;
+  j.rows = kv_rows;
+  j.tile_rows = BM;
+  j.chunk = p.chunk;
+  j.causal = mask == nullptr;
   j.Q = p.Q;
   j.D = p.D;
   j.q_lens = q_lens;
