@@ -11,6 +11,7 @@ from __future__ import annotations
 import importlib
 
 _EXPORTS = {
+    "FourBitCache": "cache4",
     "SVAArtifactBundle": "artifacts",
     "SVALayerArtifacts": "artifacts",
     "load_sva_artifact_bundle": "artifacts",

@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(WPI * WAVE) cache4_verify_kernel(Verify4Params
 
 template <int LPR>
 int launch_verify(const Verify4Params& p, int64_t items, hipStream_t stream) {
-  hipLaunchKernelGGL((cache4_verify_kernel<LPR, 8>), dim3((unsigned)items), dim3(8 * WAVE), 0, stream, p);
+  hipLaunchKernelGGL((cache4_verify_kernel<LPR, 16>), dim3((unsigned)items), dim3(16 * WAVE), 0, stream, p);
   SVA_CHECK_LAUNCH("cache4_verify_kernel");
   return SVA_OK;
 }

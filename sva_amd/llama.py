@@ -28,11 +28,12 @@ import torch
 from torch import nn
 from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
 
-from . import inverted, kernels
+from . import cache4, inverted, kernels
 from .artifacts import SVAArtifactBundle, SVALayerArtifacts, load_sva_artifact_bundle
 from .stats import SVAStats
 
 SUMMON_MODES = ("scan", "inverted", "inverted_static")
+PROMPT_MODES = ("summon", "dense")
 
 
 @dataclass(frozen=True)
@@ -52,6 +53,7 @@ class SVALlamaServingConfig:
     adaptive_high_margin: float = 0.70
     profile_components: bool = False
     static_tail_rebuild_interval: int = 64
+    prompt_attention: str = "summon"
 
 
 def _code_dtype(codewords: int) -> torch.dtype:
@@ -70,6 +72,8 @@ class SVALlamaAttention(nn.Module):
         super().__init__()
         if serving.summon_mode not in SUMMON_MODES:
             raise ValueError(f"Unknown SVA summon_mode: {serving.summon_mode!r}")
+        if serving.prompt_attention not in PROMPT_MODES:
+            raise ValueError(f"Unknown SVA prompt_attention: {serving.prompt_attention!r}")
         self.original = original
         self.config = original.config
         self.layer_idx = original.layer_idx
@@ -144,9 +148,13 @@ class SVALlamaAttention(nn.Module):
         v = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         cos, sin = position_embeddings
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
-        if past_key_values is not None:
-            k, v = past_key_values.update(k, v, self.layer_idx)
-        out = self.sva_attention(q, k, v, attention_mask)
+        held = cache4.layer_of(past_key_values, self.layer_idx)
+        if held is not None:
+            out = self._attention_cache4(q, k, v, held, attention_mask)
+        else:
+            if past_key_values is not None:
+                k, v = past_key_values.update(k, v, self.layer_idx)
+            out = self.sva_attention(q, k, v, attention_mask)
         out = out.transpose(1, 2).contiguous().reshape(*input_shape, -1)
         return self.o_proj(out), None
 
@@ -191,6 +199,8 @@ class SVALlamaAttention(nn.Module):
         k_low, codes = self._key_catalog(keys, q_len)
         if profile:
             outer["static_key_catalog_ms"] = self._profile_elapsed_ms(query.device, t1)
+        if q_len > 1 and self.serving.prompt_attention == "dense":
+            return self._dense_prompt(query, keys, values, k_len, mask)
         shortlist = min(self.serving.coarse_shortlist, k_len)
         budget = min(self.serving.budget, shortlist)
         if static_decode:
@@ -270,8 +280,52 @@ class SVALlamaAttention(nn.Module):
             self._key_len = self._codes_len = n
         return out
 
+    def _dense_prompt(self, query, keys, values, k_len, mask, seq_offsets=None, seq_lens=None):
+        """Prompt tokens by dense attention over every key (prompt_attention
+        "dense"): the catalog is kept as usual, the lookup starts with the
+        first single token.  The statistics count lookups, so no prompt token.
+        A float mask allows where it is > -1e4, a bool mask where it is true."""
+
+        with torch.no_grad():
+            return kernels.prompt_attention(query, keys, values, k_len, self.scaling, mask=mask,
+                                            seq_offsets=seq_offsets, seq_lens=seq_lens)
+
+    def _attention_cache4(self, query, key, value, held, attention_mask):
+        """sva_attention over a cache held in 4 bits (cache4.FourBitCache):
+        the new rows key / value [1, G, T, D] are written to it, the catalog
+        is appended from them as they are, and the lookup's rows are verified
+        where they lie.  A chunk of a prompt by dense attention reads the rows
+        before it back."""
+
+        if self.serving.summon_mode != "scan" or query.shape[0] != 1:
+            raise ValueError("A 4-bit cache takes one sequence in summon_mode='scan'.")
+        kernels.require_device(query, key, value)
+        q_len, start = query.shape[2], held.length
+        held.append(key, value)
+        k_len = held.length
+        sig = ("cache4", key.device, key.dtype, self._heads, key.shape[3], self.serving.rank_dim)
+        self._ensure_capacity(k_len, key.device)
+        if start == 0 or (self._signature == sig and self._key_len == self._codes_len == start):
+            rows, row0 = key[0], start
+        else:  # the catalog of another cache, or of rows since dropped
+            rows, row0 = held.read()[0][0], 0
+        kernels.write_encode(rows if rows.stride(-1) == 1 else rows.contiguous(), self.sva_k_proj,
+                             self.sva_coarse_codebooks, self._k_low[:, row0:k_len], self._codes[:, row0:k_len], 0,
+                             k_len - row0)
+        self._key_len = self._codes_len = k_len
+        self._postings = self._fast = None
+        self._signature = sig
+        mask = None if attention_mask is None else attention_mask[..., :q_len, :k_len]
+        if q_len > 1 and self.serving.prompt_attention == "dense":
+            keys, values = (key, value) if start == 0 else held.read(query.dtype)
+            return self._dense_prompt(query, keys[0], values[0], k_len, mask)
+        shortlist = min(self.serving.coarse_shortlist, k_len)
+        budget = min(self.serving.budget, shortlist)
+        return self._scan_attention(query, held, None, self._k_low, self._codes, k_len, mask, shortlist, budget)
+
     def _scan_attention(self, query, keys, values, k_low, codes, k_len, mask, shortlist, budget):
-        """sva/llama.py:226-328 on the HIP path, chunked over query tokens."""
+        """sva/llama.py:226-328 on the HIP path, chunked over query tokens.
+        keys / values [G, N, D], or a 4-bit layer and None."""
 
         outs = []
         for qs, qe, m, n in self._query_chunks(query, k_len, mask, shortlist, budget, codes):
@@ -280,8 +334,12 @@ class SVALlamaAttention(nn.Module):
                                                 codes, n, shortlist)
             _, _, sl_count, fin_idx, fin_count = kernels.summon_select(lut, rng, q_low, codes, k_low, n, shortlist,
                                                                        budget, mask=m, keep_shortlist=False)
-            outs.append(kernels.verify(qc, keys, values, fin_idx, fin_count, n, self.scaling,
-                                       out_dtype=query.dtype))
+            if values is None:
+                with torch.no_grad():
+                    outs.append(kernels.cache4_verify(qc, keys.data, keys.scales, fin_idx, fin_count, n, self.scaling))
+            else:
+                outs.append(kernels.verify(qc, keys, values, fin_idx, fin_count, n, self.scaling,
+                                           out_dtype=query.dtype))
             if self.stats is not None:
                 self.stats.add_device(int(self.layer_idx or 0), {
                     "summoned": sl_count, "exact_scored": fin_count, "verified": fin_count,
@@ -339,7 +397,10 @@ class SVALlamaAttention(nn.Module):
         shortlist = min(self.serving.coarse_shortlist, k_len)
         budget = min(self.serving.budget, shortlist)
         mask = None
-        if attention_mask is not None:
+        dense = q_len > 1 and self.serving.prompt_attention == "dense"
+        if attention_mask is not None and dense:
+            mask = attention_mask[..., :q_len, :k_len]  # (sequences may differ: padded prompts)
+        elif attention_mask is not None:
             m = attention_mask[..., :q_len, :k_len]
             # decode steps included: a left-padded batch gives each sequence
             # its own mask row, which the packed launch cannot take
@@ -356,6 +417,8 @@ class SVALlamaAttention(nn.Module):
                                   value.storage_offset())
         seq = torch.arange(batch, device=device, dtype=torch.int64)
         cat_off, kv_off = seq * cap, seq * rows_per_seq
+        if dense:
+            return self._dense_prompt(query, keys, values, k_len, mask, kv_off, torch.full_like(seq, k_len))
         outs = []
         for qs, qe, m, n in self._query_chunks(query, k_len, mask, shortlist, budget, codes):
             lens = torch.full((batch,), n, device=device, dtype=torch.int64)
@@ -498,9 +561,11 @@ class SVALlamaPatcher:
                  adaptive_min_budget: int | None = None, adaptive_mid_budget: int | None = None,
                  adaptive_low_margin: float = 0.35, adaptive_high_margin: float = 0.70,
                  profile_components: bool = False, static_tail_rebuild_interval: int = 64,
-                 layers: list[int] | None = None) -> None:
+                 layers: list[int] | None = None, prompt_attention: str = "summon") -> None:
         if summon_mode not in SUMMON_MODES:
             raise ValueError(f"Unknown SVA summon_mode: {summon_mode!r}")
+        if prompt_attention not in PROMPT_MODES:
+            raise ValueError(f"Unknown SVA prompt_attention: {prompt_attention!r}")
         self.model = model
         self.bundle = bundle
         self.stats = SVAStats()
@@ -520,6 +585,7 @@ class SVALlamaPatcher:
             adaptive_high_margin=adaptive_high_margin,
             profile_components=profile_components,
             static_tail_rebuild_interval=static_tail_rebuild_interval,
+            prompt_attention=prompt_attention,
         )
 
     def patch(self) -> "SVALlamaPatcher":
@@ -595,9 +661,15 @@ def patch_llama_attention(model: nn.Module, artifact_dir_or_bundle: str | Path |
                           inverted_cells_per_subspace: int = 8, adaptive_min_budget: int | None = None,
                           adaptive_mid_budget: int | None = None, adaptive_low_margin: float = 0.35,
                           adaptive_high_margin: float = 0.70, profile_components: bool = False,
-                          static_tail_rebuild_interval: int = 64, layers: list[int] | None = None) -> SVALlamaPatcher:
+                          static_tail_rebuild_interval: int = 64, layers: list[int] | None = None,
+                          prompt_attention: str = "summon") -> SVALlamaPatcher:
     """Patch a Llama-family model with SVA attention; returns the (already
-    applied) reversible handle (sva/llama.py:808-848)."""
+    applied) reversible handle (sva/llama.py:808-848).
+
+    prompt_attention: how a call of several tokens attends.  "summon" as the
+    reference does, every token by its own lookup; "dense" by exact attention
+    over every key (kernels.prompt_attention), the lookup then serving single
+    tokens alone."""
 
     bundle = (artifact_dir_or_bundle if isinstance(artifact_dir_or_bundle, SVAArtifactBundle)
               else load_sva_artifact_bundle(artifact_dir_or_bundle))
@@ -607,5 +679,6 @@ def patch_llama_attention(model: nn.Module, artifact_dir_or_bundle: str | Path |
                            adaptive_min_budget=adaptive_min_budget, adaptive_mid_budget=adaptive_mid_budget,
                            adaptive_low_margin=adaptive_low_margin, adaptive_high_margin=adaptive_high_margin,
                            profile_components=profile_components,
-                           static_tail_rebuild_interval=static_tail_rebuild_interval, layers=layers).patch()
+                           static_tail_rebuild_interval=static_tail_rebuild_interval, layers=layers,
+                           prompt_attention=prompt_attention).patch()
 
