@@ -542,12 +542,13 @@ int sva_stream_read(const void *src, int64_t bytes, uint32_t *sink, int64_t sink
  *                  t*kv_row_stride + d
  *   first_rows     [n_seq] int64 on the device: token t of sequence b goes to
  *                  cache row first_rows[b] + t; rows outside [0, rows) are
- *                  skipped.  Two sequences must not name one row.
+ *                  skipped.  Two sequences must not name one row.  NULL: one
+ *                  sequence, from row first_row (not read otherwise).
  */
 int sva_cache4_write(const void *keys, const void *values, int kv_dtype, int64_t kv_seq_stride,
                      int64_t kv_head_stride, int64_t kv_row_stride, int64_t n_seq, int64_t n_rows, int64_t G,
-                     int64_t D, const int64_t *first_rows, uint8_t *data, uint8_t *scales, int64_t rows,
-                     void *stream);
+                     int64_t D, const int64_t *first_rows, int64_t first_row, uint8_t *data, uint8_t *scales,
+                     int64_t rows, void *stream);
 
 /*
  * The values of rows first_rows[b] + t, laid out as sva_cache4_write takes
@@ -555,8 +556,8 @@ int sva_cache4_write(const void *keys, const void *values, int kv_dtype, int64_t
  * whose cache row lies outside [0, rows) are left as they were.
  */
 int sva_cache4_read(const uint8_t *data, const uint8_t *scales, int64_t rows, const int64_t *first_rows,
-                    int64_t n_seq, int64_t n_rows, int64_t G, int64_t D, void *keys, void *values, int kv_dtype,
-                    int64_t kv_seq_stride, int64_t kv_head_stride, int64_t kv_row_stride, void *stream);
+                    int64_t first_row, int64_t n_seq, int64_t n_rows, int64_t G, int64_t D, void *keys, void *values,
+                    int kv_dtype, int64_t kv_seq_stride, int64_t kv_head_stride, int64_t kv_row_stride, void *stream);
 
 /*
  * sva_verify over a 4-bit cache: softmax attention of each query item over

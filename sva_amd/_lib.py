@@ -85,8 +85,8 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
     "sva_prompt_attention": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64,
                                   _I64, _I64, _I64, _I64, _F, _P, _I, _I64, _I64, _P, _I, _I64, _I64, _I64, _P, _SZ,
                                   _P]),
-    "sva_cache4_write": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P]),
-    "sva_cache4_read": (_I, [_P, _P, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I, _I64, _I64, _I64, _P]),
+    "sva_cache4_write": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P]),
+    "sva_cache4_read": (_I, [_P, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I, _I64, _I64, _I64, _P]),
     "sva_cache4_verify": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64,
                                _I64, _I64, _F, _P, _I, _I64, _I64, _I64, _P]),
     "sva_cache4_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),

@@ -21,7 +21,8 @@ struct Cache4Rows {
   const void* keys;  // written to by the read
   const void* values;
   int64_t seq_stride, head_stride, row_stride;  // elements
-  const int64_t* first_rows;                    // [n_seq] cache row of each sequence's row 0
+  const int64_t* first_rows;                    // [n_seq] cache row of each sequence's row 0, or NULL:
+  int64_t first_row;                            // that of the one sequence
   uint8_t* data;
   uint8_t* scales;
   int64_t rows;     // of the cache
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(WB) cache4_write_kernel(Cache4Rows p) {
   const int64_t t = c / per_row >> 1;
   const int kv = (int)(c / per_row & 1);
   const int g = (int)blockIdx.y % p.G, b = (int)blockIdx.y / p.G;
-  const int64_t row = p.first_rows[b] + t;
+  const int64_t row = (p.first_rows ? p.first_rows[b] : p.first_row) + t;
   if (row < 0 || row >= p.rows) return;  // outside the cache: nothing is written (the same for a whole quad)
   float x[8];
   load8<DT>(kv ? p.values : p.keys, b * p.seq_stride + g * p.head_stride + t * p.row_stride + 8 * chunk, p.vec, x);
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(WB) cache4_read_kernel(Cache4Rows p) {
   const int64_t t = c / per_row >> 1;
   const int kv = (int)(c / per_row & 1);
   const int g = (int)blockIdx.y % p.G, b = (int)blockIdx.y / p.G;
-  const int64_t row = p.first_rows[b] + t;
+  const int64_t row = (p.first_rows ? p.first_rows[b] : p.first_row) + t;
   if (row < 0 || row >= p.rows) return;
   const int64_t half = (g * p.rows + row) * 2 + kv;
   const uint32_t w = *(const uint32_t*)(p.data + half * (p.D / 2) + 4 * chunk);
@@ -272,7 +273,8 @@ int launch_verify(const Verify4Params& p, int64_t items, hipStream_t stream) {
 int check_rows(const char* name, const void* keys, const void* values, int dtype, int64_t n_seq, int64_t n_rows,
                int64_t G, int64_t D, const int64_t* first_rows, const uint8_t* data, const uint8_t* scales,
                int64_t rows) {
-  SVA_REQUIRE(keys && values && first_rows && data && scales, "%s: null pointer", name);
+  SVA_REQUIRE(keys && values && data && scales, "%s: null pointer", name);
+  SVA_REQUIRE(first_rows || n_seq == 1, "%s: several sequences need their first rows", name);
   SVA_REQUIRE(n_seq > 0 && n_rows > 0 && G > 0 && rows > 0, "%s: bad sizes", name);
   SVA_REQUIRE(dtype >= 0 && dtype <= 2, "%s: bad dtype", name);
   SVA_REQUIRE(D > 0 && D <= 256 && D % kCache4Block == 0, "%s: head_dim %lld is not a multiple of 32 up to 256", name,
@@ -284,7 +286,7 @@ int check_rows(const char* name, const void* keys, const void* values, int dtype
 
 Cache4Rows rows_params(const void* keys, const void* values, int dtype, int64_t seq_stride, int64_t head_stride,
                        int64_t row_stride, int64_t n_rows, int64_t G, int64_t D, const int64_t* first_rows,
-                       uint8_t* data, uint8_t* scales, int64_t rows) {
+                       int64_t first_row, uint8_t* data, uint8_t* scales, int64_t rows) {
   const int64_t word = dtype == F32 ? 4 : 8;  // elements of 16 bytes
   Cache4Rows p;
   p.keys = keys;
@@ -293,6 +295,7 @@ Cache4Rows rows_params(const void* keys, const void* values, int dtype, int64_t 
   p.head_stride = head_stride;
   p.row_stride = row_stride;
   p.first_rows = first_rows;
+  p.first_row = first_row;
   p.data = data;
   p.scales = scales;
   p.rows = rows;
@@ -308,14 +311,14 @@ Cache4Rows rows_params(const void* keys, const void* values, int dtype, int64_t 
 
 extern "C" int sva_cache4_write(const void* keys, const void* values, int kv_dtype, int64_t kv_seq_stride,
                                 int64_t kv_head_stride, int64_t kv_row_stride, int64_t n_seq, int64_t n_rows,
-                                int64_t G, int64_t D, const int64_t* first_rows, uint8_t* data, uint8_t* scales,
-                                int64_t rows, void* stream) {
+                                int64_t G, int64_t D, const int64_t* first_rows, int64_t first_row,
+                                uint8_t* data, uint8_t* scales, int64_t rows, void* stream) {
   sva::clear_error();
   if (const int rc = check_rows("sva_cache4_write", keys, values, kv_dtype, n_seq, n_rows, G, D, first_rows, data,
                                 scales, rows))
     return rc;
   const Cache4Rows p = rows_params(keys, values, kv_dtype, kv_seq_stride, kv_head_stride, kv_row_stride, n_rows, G, D,
-                                   first_rows, data, scales, rows);
+                                   first_rows, first_row, data, scales, rows);
   const dim3 grid((unsigned)((n_rows * 2 * (D / 8) + WB - 1) / WB), (unsigned)(n_seq * G));
   auto* fn = kv_dtype == F32 ? cache4_write_kernel<F32>
                              : (kv_dtype == BF16 ? cache4_write_kernel<BF16> : cache4_write_kernel<F16>);
@@ -325,7 +328,7 @@ extern "C" int sva_cache4_write(const void* keys, const void* values, int kv_dty
 }
 
 extern "C" int sva_cache4_read(const uint8_t* data, const uint8_t* scales, int64_t rows, const int64_t* first_rows,
-                               int64_t n_seq, int64_t n_rows, int64_t G, int64_t D, void* keys, void* values,
+                               int64_t first_row, int64_t n_seq, int64_t n_rows, int64_t G, int64_t D, void* keys, void* values,
                                int kv_dtype, int64_t kv_seq_stride, int64_t kv_head_stride, int64_t kv_row_stride,
                                void* stream) {
   sva::clear_error();
@@ -333,7 +336,7 @@ extern "C" int sva_cache4_read(const uint8_t* data, const uint8_t* scales, int64
                                 scales, rows))
     return rc;
   const Cache4Rows p = rows_params(keys, values, kv_dtype, kv_seq_stride, kv_head_stride, kv_row_stride, n_rows, G, D,
-                                   first_rows, const_cast<uint8_t*>(data), const_cast<uint8_t*>(scales), rows);
+                                   first_rows, first_row, const_cast<uint8_t*>(data), const_cast<uint8_t*>(scales), rows);
   const dim3 grid((unsigned)((n_rows * 2 * (D / 8) + WB - 1) / WB), (unsigned)(n_seq * G));
   auto* fn = kv_dtype == F32 ? cache4_read_kernel<F32>
                              : (kv_dtype == BF16 ? cache4_read_kernel<BF16> : cache4_read_kernel<F16>);

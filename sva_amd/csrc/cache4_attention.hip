@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
   const int len = (int)seq_keys(p.lens, p.offs, p.N, p.rows, b, off);
   const int ranges = tile_ranges(len, p.chunk);
   if (split >= ranges) return;
-  const int k0 = split * p.chunk, k1 = min(len, k0 + p.chunk);
+  const int k0 = split * p.chunk, k1 = k0 + min(p.chunk, len - k0);
   const int blocks = PAD ? p.D / kCache4Block : NB;
   const int dim = PAD ? p.D : D;
 

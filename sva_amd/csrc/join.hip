@@ -88,21 +88,39 @@ __global__ void __launch_bounds__(JB) join_kernel(JoinParams p) {
   }
 }
 
-// Many items of few ranges (prompts): a wave an item, 64 elements at a time.
+// Many items of few ranges (prompts): a wave an item, 64 elements and eight
+// ranges at a time, with a running maximum: a range's stats and sums are
+// loaded together, so an item is two round trips to memory.
 __global__ void __launch_bounds__(RB) join_rows_kernel(JoinParams p, int items) {
   const int item = (int)blockIdx.x * (RB / WAVE) + (int)threadIdx.x / WAVE;
   if (item >= items) return;
   const JoinItem x = join_item(p, item);
   if (x.ranges == 1) return;
-  float M = -INFINITY, Z = 0.0f;
-  for (int s = 0; s < x.ranges; ++s) M = fmaxf(M, x.stats[2 * s]);
-  for (int s = 0; s < x.ranges; ++s) Z += x.stats[2 * s + 1] * join_share(x.stats[2 * s], M);
+  constexpr int U = 8;
   for (int d = lane_id(); d < p.D; d += WAVE) {
-    float a = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < x.ranges; ++s) {
-      const float c = join_share(x.stats[2 * s], M);
-      a += c == 0.0f ? 0.0f : x.sums[(int64_t)s * p.D + d] * c;
+    float M = -INFINITY, Z = 0.0f, a = 0.0f;
+    for (int s0 = 0; s0 < x.ranges; s0 += U) {
+      float2 st[U];
+      float sm[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = min(s0 + u, x.ranges - 1);
+        st[u] = *(const float2*)(x.stats + 2 * s);
+        sm[u] = x.sums[(int64_t)s * p.D + d];
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, st[u].x);  // (the last range again behind the end)
+      const float c = join_share(M, top);
+      Z *= c, a *= c, M = top;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float f = s0 + u < x.ranges ? join_share(st[u].x, M) : 0.0f;
+        if (f != 0.0f) {
+          Z += st[u].y * f;
+          a += sm[u] * f;
+        }
+      }
     }
     store_elem(p.out, x.at + d, p.out_dtype, Z == 0.0f ? 0.0f : a / Z);
   }

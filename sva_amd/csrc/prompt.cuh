@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   if (split >= ranges) return;
   const bool partial = ranges > 1;  // joined by a second kernel
   const int kbeg = split * p.chunk;
-  const int kend = min(keys, kbeg + p.chunk);
+  const int kend = kbeg + min(p.chunk, max(keys - kbeg, 0));
 
   // this wave's rows, one per lane and half
   const int wrow = rt * BM + w * 32;
@@ -393,6 +393,13 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
         scores(kbuf + ((t + 1) & 1) * TB, sn);  // (behind the last tile: not used)
         if (!first) sums(vbuf + ((t + 1) & 1) * TB, pp);
         const float zs = weigh(sc, pc);
+        if constexpr (DP == 128 && ES == 2) {  // a matrix instruction, then the vector instructions of its time
+#pragma unroll
+          for (int i = 0; i < 4 * NF; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+          }
+        }
         settle(zs, sc, pc);
       }
       arrive();

@@ -20,16 +20,17 @@ int64_t row_tiles(int64_t H, int64_t G, int64_t Q) { return (H / G * Q + BM - 1)
 // of whole prompts are of every length, and dispatch evens them out: they are
 // split only where they do not fill the card once.  Tokens over a cache that
 // is much longer make row tiles of one length: about five workgroups for each
-// of the two places of a CU, so that a last round of them is a small part.
-// Ranges cost a second launch and their sums' way through memory.  (9 x 64
-// bf16: 8192 whole tokens 120 us in one range, 145 with a second behind key
-// 4736; 512 tokens each over 8 x 32768 keys 530 us in two ranges, 450 in
-// seven, 520 in 16; a token each of 32 sequences of up to 131072 keys 376 us
-// in eight, 289 in 28, 318 in 64; 12 x 64 fp32, 1001 tokens 77 us in one, 54 in
-// two.)
+// of the two places of a CU, so that a last round of them is a small part;
+// fewer where there are many rows, whose sums go through memory once for each
+// range.  (9 x 64 bf16: 8192 whole tokens 120 us in one range, 145 with a
+// second behind key 4736; 512 tokens each over 8 x 32768 keys 530 us in two
+// ranges, 437 in six, 462 in nine, 520 in 16; a token each of 32 sequences of
+// up to 131072 keys 376 us in eight, 289 in 28, 318 in 64; 12 x 64 fp32, 1001
+// tokens 77 us in one, 46 in three, 51 in four.)
 int64_t chunk_keys(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t n_keys) {
   const int64_t tiles = n_seq * G * row_tiles(H, G, Q), cus = sva::device_cu_count();
-  const int64_t want = 2 * Q > n_keys ? (cus + tiles - 1) / tiles : (10 * cus + tiles / 2) / tiles;
+  const int64_t places = n_seq * H * Q > 8192 ? 7 * cus : 10 * cus;
+  const int64_t want = 2 * Q > n_keys ? (cus + tiles - 1) / tiles : (places + tiles / 2) / tiles;
   const int64_t ranges = std::max<int64_t>(1, std::min<int64_t>(64, want));
   return std::max<int64_t>(256, ((n_keys + ranges - 1) / ranges + 63) / 64 * 64);
 }

@@ -799,13 +799,15 @@ def _check_cache4(data: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, i
         raise ValueError(f"4-bit data must be contiguous uint8 [G, rows, 2, D / 2], got {data.dtype} "
                          f"{tuple(data.shape)}")
     kv_heads, rows, _, half = data.shape
-    if scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (kv_heads, rows, 2,
-                                                                                            half // 16):
+    if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.shape != (kv_heads, rows, 2, half // 16):
         raise ValueError(f"4-bit scales must be contiguous uint8 {(kv_heads, rows, 2, half // 16)}, got "
                          f"{scales.dtype} {tuple(scales.shape)}")
     if half % 16 != 0 or half > 128 or half < 16:
         raise ValueError(f"a 4-bit cache takes head_dim a multiple of 32 up to 256, got {2 * half}")
     return kv_heads, rows, 2 * half
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (a microsecond less)
 
 
 def _inference_only(name: str, *tensors: torch.Tensor) -> None:
@@ -817,26 +819,38 @@ def _call(device: torch.device, name: str, *args) -> None:
     """An entry point on `device`'s current stream, with `device` current."""
 
     fn = getattr(lib(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(fn(*args, stream_handle(device)), name)
-        return
-    with torch.cuda.device(device):
-        check(fn(*args, stream_handle(device)), name)
+    if device.index is None or device.index == _current_device():
+        status = fn(*args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream_handle(device))
+    if status:
+        check(status, name)
 
 
-def _seq_tensor(name: str, t, n_seq: int, device: torch.device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor):
-        t = torch.tensor([t] if isinstance(t, int) else list(t), device=device, dtype=torch.int64)
-    if t.dtype != torch.int64 or tuple(t.shape) != (n_seq,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be int64 [{n_seq}], got {t.dtype} {tuple(t.shape)}")
+def _seq_tensor(name: str, t: torch.Tensor, n_seq: int) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.shape != (n_seq,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be an int64 tensor [{n_seq}], got {t}")
     return t
+
+
+def _first_rows(first_rows, n_seq: int, device: torch.device):
+    """(device tensor or None, row of a single sequence) of an int, ints, or an int64 tensor [n_seq]."""
+
+    if not isinstance(first_rows, torch.Tensor):
+        rows = [first_rows] if isinstance(first_rows, int) else list(first_rows)
+        if len(rows) == n_seq == 1:
+            return None, int(rows[0])
+        first_rows = torch.tensor(rows, device=device, dtype=torch.int64)
+    return _seq_tensor("first_rows", first_rows, n_seq), 0
 
 
 def cache4_write(keys: torch.Tensor, values: torch.Tensor, data: torch.Tensor, scales: torch.Tensor,
                  first_rows) -> None:
     """Writes keys / values [n_seq, G, T, D] (or [G, T, D]) into a 4-bit cache
     (cache4_alloc): token t of sequence b into row first_rows[b] + t.
-    first_rows: int64 [n_seq] on the device, or an int or ints (copied there).
+    first_rows: int64 [n_seq] on the device; the int of a single sequence; or
+    ints, which are copied there first.
     Rows outside the cache are skipped; two sequences must not name one row."""
 
     kv_heads, rows, dim = _check_cache4(data, scales)
@@ -846,17 +860,17 @@ def cache4_write(keys: torch.Tensor, values: torch.Tensor, data: torch.Tensor, s
             keys.shape[3] != dim:
         raise ValueError(f"keys / values must be [n_seq, {kv_heads}, T, {dim}] of one dtype, got {keys.dtype} "
                          f"{tuple(keys.shape)} and {values.dtype} {tuple(values.shape)}")
-    device = require_device(keys, values, data, scales, first_rows if isinstance(first_rows, torch.Tensor) else None)
-    _inference_only("cache4_write", keys, values)
     n_seq, _, n_rows, _ = keys.shape
-    first = _seq_tensor("first_rows", first_rows, n_seq, device)
+    first_rows, first_row = _first_rows(first_rows, n_seq, keys.device)
+    device = require_device(keys, values, data, scales, first_rows)
+    _inference_only("cache4_write", keys, values)
     dtype = dtype_code(keys)
     if n_seq == 0 or n_rows == 0:
         return
     if keys.stride(-1) != 1 or values.stride() != keys.stride():
         keys, values = keys.contiguous(), values.contiguous()
     _call(device, "sva_cache4_write", ptr(keys), ptr(values), dtype, keys.stride(0), keys.stride(1), keys.stride(2),
-          n_seq, n_rows, kv_heads, dim, ptr(first), ptr(data), ptr(scales), rows)
+          n_seq, n_rows, kv_heads, dim, ptr(first_rows), first_row, ptr(data), ptr(scales), rows)
 
 
 def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: int,
@@ -866,10 +880,9 @@ def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: in
     lie inside the cache: the outputs of others are undefined."""
 
     kv_heads, rows, dim = _check_cache4(data, scales)
-    device = require_device(data, scales, first_rows if isinstance(first_rows, torch.Tensor) else None)
-    n_seq = first_rows.shape[0] if isinstance(first_rows, torch.Tensor) and first_rows.dim() else (
-        1 if isinstance(first_rows, (int, torch.Tensor)) else len(first_rows))
-    first = _seq_tensor("first_rows", first_rows, n_seq, device)
+    n_seq = 1 if isinstance(first_rows, int) else len(first_rows)
+    first_rows, first_row = _first_rows(first_rows, n_seq, data.device)
+    device = require_device(data, scales, first_rows)
     if dtype not in DTYPE_CODES:
         raise TypeError(f"unsupported dtype {dtype}; expected float32, bfloat16 or float16")
     if n_rows < 0 or n_rows > rows:
@@ -877,8 +890,8 @@ def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: in
     keys = torch.empty(n_seq, kv_heads, n_rows, dim, device=device, dtype=dtype)
     values = torch.empty_like(keys)
     if n_seq and n_rows:
-        _call(device, "sva_cache4_read", ptr(data), ptr(scales), rows, ptr(first), n_seq, n_rows, kv_heads, dim,
-              ptr(keys), ptr(values), dtype_code(keys), keys.stride(0), keys.stride(1), keys.stride(2))
+        _call(device, "sva_cache4_read", ptr(data), ptr(scales), rows, ptr(first_rows), first_row, n_seq, n_rows,
+              kv_heads, dim, ptr(keys), ptr(values), dtype_code(keys), keys.stride(0), keys.stride(1), keys.stride(2))
     return keys, values
 
 
@@ -896,8 +909,8 @@ def _cache4_query(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, n_k
         if n_keys > rows:
             raise ValueError(f"{n_keys} keys of a cache of {rows} rows")
     else:
-        seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq, q.device)
-        seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq, q.device)
+        seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq)
+        seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq)
     device = require_device(q, data, scales, seq_offsets, seq_lens)
     return q, device, kv_heads, rows, seq_offsets, seq_lens
 
@@ -939,7 +952,7 @@ def cache4_verify(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, fin
     n_seq, heads, q_len, dim = q.shape
     items = n_seq * heads * q_len
     if fin_idx.dim() != 2 or fin_idx.dtype != torch.int32 or not fin_idx.is_contiguous() or fin_idx.shape[0] != items \
-            or fin_count.dtype != torch.int32 or tuple(fin_count.shape) != (items,) or not fin_count.is_contiguous():
+            or fin_count.dtype != torch.int32 or fin_count.shape != (items,) or not fin_count.is_contiguous():
         raise ValueError(f"fin_idx must be contiguous int32 [{items}, B] and fin_count int32 [{items}]")
     require_device(q, fin_idx, fin_count)
     budget = fin_idx.shape[1]
@@ -1038,11 +1051,11 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     _inference_only("prompt_attention", q, keys, values)
     dtype = dtype_code(q)
     if seq_offsets is not None:
-        seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq, device)
-        seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq, device)
+        seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq)
+        seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq)
     if packed:
-        q_offsets = _seq_tensor("q_offsets", q_offsets, n_seq, device)
-        q_lens = _seq_tensor("q_lens", q_lens, n_seq, device)
+        q_offsets = _seq_tensor("q_offsets", q_offsets, n_seq)
+        q_lens = _seq_tensor("q_lens", q_lens, n_seq)
     if q4.stride(-1) != 1:
         q4 = q4.contiguous()
     if keys.stride(-1) != 1 or values.stride() != keys.stride():

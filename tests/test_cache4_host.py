@@ -82,16 +82,16 @@ def test_c_entry_points_refuse():
         return lib.sva_cache4_verify(p, dt, 0, 0, 0, p, p, 100, None, None, 100, idx, p, n_seq, 4, 2, 1, D, B, one, p,
                                      1, 0, 0, 0, None)
 
-    def write(D=64, n=3, dt=1, data=p):
-        return lib.sva_cache4_write(p, p, dt, 0, 0, 0, 1, n, 2, D, p, data, p, 100, None)
+    def write(D=64, n=3, dt=1, data=p, first=p, n_seq=1):
+        return lib.sva_cache4_write(p, p, dt, 0, 0, 0, n_seq, n, 2, D, first, 0, data, p, 100, None)
 
-    def read(D=64, n=3, dt=1, first=p):
-        return lib.sva_cache4_read(p, p, 100, first, 1, n, 2, D, p, p, dt, 0, 0, 0, None)
+    def read(D=64, n=3, dt=1, first=p, n_seq=1):
+        return lib.sva_cache4_read(p, p, 100, first, 0, n_seq, n, 2, D, p, p, dt, 0, 0, 0, None)
 
     calls = [attention(q=None), attention(D=48), attention(D=288), attention(H=3), attention(off=p), attention(n_seq=2),
              attention(ws=None), attention(dt=3), attention(data=ctypes.c_void_p(264)), verify(D=40),
              verify(B=0), verify(idx=None), verify(n_seq=2), verify(dt=-1), write(D=33), write(n=0), write(dt=7),
-             write(data=None), read(D=0), read(n=-1), read(dt=3), read(first=None)]
+             write(data=None), write(first=None, n_seq=2), read(D=0), read(n=-1), read(dt=3), read(first=None, n_seq=2)]
     assert calls == [1] * len(calls), calls
     assert attention(Q=1 << 20) == 3  # SVA_ERR_UNSUPPORTED
     big = lib.sva_cache4_attention_workspace_bytes(1, 9, 3, 1, 64, 1 << 20)
