@@ -807,19 +807,32 @@ def _check_cache4(data: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, i
     return kv_heads, rows, 2 * half
 
 
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # (a microsecond less)
+# (raw accessors: a microsecond less than the checked ones, on calls of a few)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _inference_only(name: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} runs inference only: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{name} runs inference only: call it under torch.no_grad()")
+
+
+def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device:
+    """require_device by device indexes; it gives the error where they differ."""
+
+    index = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            return require_device(first, *rest)
+    return first.device if index >= 0 else require_device(first)
 
 
 def _call(device: torch.device, name: str, *args) -> None:
     """An entry point on `device`'s current stream, with `device` current."""
 
     fn = getattr(lib(), name)
-    if device.index is None or device.index == _current_device():
+    if device.index == _current_device():
         status = fn(*args, stream_handle(device))
     else:
         with torch.cuda.device(device):
@@ -862,15 +875,15 @@ def cache4_write(keys: torch.Tensor, values: torch.Tensor, data: torch.Tensor, s
                          f"{tuple(keys.shape)} and {values.dtype} {tuple(values.shape)}")
     n_seq, _, n_rows, _ = keys.shape
     first_rows, first_row = _first_rows(first_rows, n_seq, keys.device)
-    device = require_device(keys, values, data, scales, first_rows)
+    device = _same_device(keys, values, data, scales, first_rows)
     _inference_only("cache4_write", keys, values)
     dtype = dtype_code(keys)
     if n_seq == 0 or n_rows == 0:
         return
     if keys.stride(-1) != 1 or values.stride() != keys.stride():
         keys, values = keys.contiguous(), values.contiguous()
-    _call(device, "sva_cache4_write", ptr(keys), ptr(values), dtype, keys.stride(0), keys.stride(1), keys.stride(2),
-          n_seq, n_rows, kv_heads, dim, ptr(first_rows), first_row, ptr(data), ptr(scales), rows)
+    _call(device, "sva_cache4_write", keys.data_ptr(), values.data_ptr(), dtype, *keys.stride()[:3], n_seq, n_rows,
+          kv_heads, dim, ptr(first_rows), first_row, data.data_ptr(), scales.data_ptr(), rows)
 
 
 def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: int,
@@ -882,7 +895,7 @@ def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: in
     kv_heads, rows, dim = _check_cache4(data, scales)
     n_seq = 1 if isinstance(first_rows, int) else len(first_rows)
     first_rows, first_row = _first_rows(first_rows, n_seq, data.device)
-    device = require_device(data, scales, first_rows)
+    device = _same_device(data, scales, first_rows)
     if dtype not in DTYPE_CODES:
         raise TypeError(f"unsupported dtype {dtype}; expected float32, bfloat16 or float16")
     if n_rows < 0 or n_rows > rows:
@@ -890,8 +903,8 @@ def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: in
     keys = torch.empty(n_seq, kv_heads, n_rows, dim, device=device, dtype=dtype)
     values = torch.empty_like(keys)
     if n_seq and n_rows:
-        _call(device, "sva_cache4_read", ptr(data), ptr(scales), rows, ptr(first_rows), first_row, n_seq, n_rows,
-              kv_heads, dim, ptr(keys), ptr(values), dtype_code(keys), keys.stride(0), keys.stride(1), keys.stride(2))
+        _call(device, "sva_cache4_read", data.data_ptr(), scales.data_ptr(), rows, ptr(first_rows), first_row, n_seq,
+              n_rows, kv_heads, dim, keys.data_ptr(), values.data_ptr(), DTYPE_CODES[dtype], *keys.stride()[:3])
     return keys, values
 
 
@@ -911,7 +924,7 @@ def _cache4_query(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, n_k
     else:
         seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq)
         seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq)
-    device = require_device(q, data, scales, seq_offsets, seq_lens)
+    device = _same_device(q, data, scales, seq_offsets, seq_lens)
     return q, device, kv_heads, rows, seq_offsets, seq_lens
 
 
@@ -934,9 +947,9 @@ def cache4_attention(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, 
     # a buffer of the call's own: calls on other streams and captured graphs never share one
     ws = torch.empty(int(lib().sva_cache4_attention_workspace_bytes(n_seq, heads, kv_heads, q_len, dim, n_keys)),
                      device=device, dtype=torch.uint8)
-    _call(device, "sva_cache4_attention", ptr(q), dtype_code(q), q.stride(0), q.stride(1), q.stride(2), ptr(data),
-          ptr(scales), rows, ptr(seq_offsets), ptr(seq_lens), n_keys, n_seq, heads, kv_heads, q_len, dim,
-          float(scaling), ptr(out), dtype_code(out), out.stride(0), out.stride(1), out.stride(2), ptr(ws), ws.numel())
+    _call(device, "sva_cache4_attention", q.data_ptr(), dtype_code(q), *q.stride()[:3], data.data_ptr(),
+          scales.data_ptr(), rows, ptr(seq_offsets), ptr(seq_lens), n_keys, n_seq, heads, kv_heads, q_len, dim,
+          float(scaling), out.data_ptr(), dtype_code(out), *out.stride()[:3], ws.data_ptr(), ws.numel())
     return out
 
 
@@ -954,17 +967,17 @@ def cache4_verify(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, fin
     if fin_idx.dim() != 2 or fin_idx.dtype != torch.int32 or not fin_idx.is_contiguous() or fin_idx.shape[0] != items \
             or fin_count.dtype != torch.int32 or fin_count.shape != (items,) or not fin_count.is_contiguous():
         raise ValueError(f"fin_idx must be contiguous int32 [{items}, B] and fin_count int32 [{items}]")
-    require_device(q, fin_idx, fin_count)
+    _same_device(q, fin_idx, fin_count)
     budget = fin_idx.shape[1]
     out = torch.empty(n_seq, heads, q_len, dim, device=device, dtype=out_dtype or q.dtype)
     if out.numel() == 0:
         return out
     if n_keys <= 0 or budget == 0:
         return out.zero_()
-    _call(device, "sva_cache4_verify", ptr(q), dtype_code(q), q.stride(0), q.stride(1), q.stride(2), ptr(data),
-          ptr(scales), rows, ptr(seq_offsets), ptr(seq_lens), n_keys, ptr(fin_idx), ptr(fin_count), n_seq, heads,
-          kv_heads, q_len, dim, budget, float(scaling), ptr(out), dtype_code(out), out.stride(0), out.stride(1),
-          out.stride(2))
+    _call(device, "sva_cache4_verify", q.data_ptr(), dtype_code(q), *q.stride()[:3], data.data_ptr(),
+          scales.data_ptr(), rows, ptr(seq_offsets), ptr(seq_lens), n_keys, fin_idx.data_ptr(), fin_count.data_ptr(),
+          n_seq, heads, kv_heads, q_len, dim, budget, float(scaling), out.data_ptr(), dtype_code(out),
+          *out.stride()[:3])
     return out
 
 
@@ -1047,7 +1060,7 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
         raise ValueError(f"{n_seq} sequences of up to {n_keys} keys need seq_offsets and seq_lens, or rows for them")
     if out is not None and (out.shape != shape or out.stride(-1) != 1 or (out_dtype or out.dtype) != out.dtype):
         raise ValueError(f"out must be {tuple(shape)} with contiguous rows, got {out.dtype} {tuple(out.shape)}")
-    device = require_device(q, keys, values, mask, seq_offsets, seq_lens, q_offsets, q_lens, out)
+    device = _same_device(q, keys, values, mask, seq_offsets, seq_lens, q_offsets, q_lens, out)
     _inference_only("prompt_attention", q, keys, values)
     dtype = dtype_code(q)
     if seq_offsets is not None:
@@ -1079,8 +1092,8 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     # a buffer of the call's own: calls on other streams and captured graphs never share one
     ws = torch.empty(int(lib().sva_prompt_attention_workspace_bytes(n_seq, heads, kv_heads, q_len, dim, n_keys)),
                      device=device, dtype=torch.uint8)
-    _call(device, "sva_prompt_attention", ptr(q4), dtype, q4.stride(0), q4.stride(1), q4.stride(2), ptr(q_offsets),
-          ptr(q_lens), n_rows, ptr(keys), ptr(values), keys.stride(0), keys.stride(1), rows, ptr(seq_offsets),
-          ptr(seq_lens), n_keys, n_seq, heads, kv_heads, q_len, dim, float(scaling), ptr(m), mtype, mseq, mtok, ptr(out),
-          dtype_code(out), o4.stride(0), o4.stride(1), o4.stride(2), ptr(ws), ws.numel())
+    _call(device, "sva_prompt_attention", q4.data_ptr(), dtype, *q4.stride()[:3], ptr(q_offsets), ptr(q_lens), n_rows,
+          keys.data_ptr(), values.data_ptr(), *keys.stride()[:2], rows, ptr(seq_offsets), ptr(seq_lens), n_keys, n_seq,
+          heads, kv_heads, q_len, dim, float(scaling), ptr(m), mtype, mseq, mtok, out.data_ptr(), dtype_code(out),
+          *o4.stride()[:3], ws.data_ptr(), ws.numel())
     return out
