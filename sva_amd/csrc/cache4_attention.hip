@@ -315,10 +315,10 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
 
 // Keys per workgroup: enough workgroups to fill the card, four times as many
 // where sequences may differ in length (the last to end is then a small part
-// of the call); ranges of at least 256 keys and at most 256 of them (each
+// of the call); ranges of at least 256 keys and at most 384 of them (each
 // costs a row of partial sums).
 int64_t chunk_keys(int64_t n_seq, int64_t groups, int64_t n_keys) {
-  const int64_t want = std::min<int64_t>(256, std::max<int64_t>(1, (n_seq > 1 ? 4096 : 1024) / groups));
+  const int64_t want = std::min<int64_t>(384, std::max<int64_t>(1, (n_seq > 1 ? 4096 : 1024) / groups));
   const int64_t unit = AW * TK;
   return std::max<int64_t>(2 * unit, ((n_keys + want - 1) / want + unit - 1) / unit * unit);
 }

@@ -61,9 +61,13 @@ __global__ void __launch_bounds__(JB) join_kernel(JoinParams p) {
     float sm[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int s = min(s0 + u * PARTS, x.ranges - 1);
-      st[u] = *(const float2*)(x.stats + 2 * s);
-      sm[u] = x.sums[(int64_t)s * p.D + min(d, p.D - 1)];
+      const int s = s0 + u * PARTS;
+      st[u] = make_float2(0.0f, 0.0f);
+      sm[u] = 0.0f;
+      if (s < x.ranges) {
+        st[u] = *(const float2*)(x.stats + 2 * s);
+        sm[u] = x.sums[(int64_t)s * p.D + min(d, p.D - 1)];
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -104,13 +108,16 @@ __global__ void __launch_bounds__(RB) join_rows_kernel(JoinParams p, int items) 
       float sm[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int s = min(s0 + u, x.ranges - 1);
-        st[u] = *(const float2*)(x.stats + 2 * s);
-        sm[u] = x.sums[(int64_t)s * p.D + d];
+        st[u] = make_float2(-INFINITY, 0.0f);
+        sm[u] = 0.0f;
+        if (s0 + u < x.ranges) {
+          st[u] = *(const float2*)(x.stats + 2 * (s0 + u));
+          sm[u] = x.sums[(int64_t)(s0 + u) * p.D + d];
+        }
       }
       float top = M;
 #pragma unroll
-      for (int u = 0; u < U; ++u) top = fmaxf(top, st[u].x);  // (the last range again behind the end)
+      for (int u = 0; u < U; ++u) top = fmaxf(top, st[u].x);
       const float c = join_share(M, top);
       Z *= c, a *= c, M = top;
 #pragma unroll
