@@ -55,7 +55,9 @@ SVA_DEV void load8(const void* base, int64_t e, bool vec, float (&x)[8]) {
 
 // One thread per 8 elements; the 4 threads of a block share its largest
 // magnitude by quad permutes.  Reads 16 (fp32: 32) and writes 4 consecutive
-// bytes per thread, and a scale byte per block: bound by memory.
+// bytes per thread, and a scale byte per block: bound by memory (131072 rows
+// of 8 x 128 bf16: written and read back 306 us, 4.4 TB/s, where a large copy
+// moves 4.9; a decode step's rows are 2.5 us, a launch).
 template <int DT>
 __global__ void __launch_bounds__(WB) cache4_write_kernel(Cache4Rows p) {
   const uint32_t per_row = (uint32_t)p.D / 8;  // threads of a K or V row
@@ -134,7 +136,9 @@ __global__ void __launch_bounds__(WB) cache4_read_kernel(Cache4Rows p) {
 // Each row slot keeps an online softmax of its own (32-bit); slots merge by
 // cross-lane sums, waves through LDS.  A chosen row is two lines of the
 // cache wherever it is, so what bounds a decode step's few hundred rows is
-// the latency of list, row and merge, not bandwidth.
+// the latency of list, row and merge, not bandwidth (9 heads x 512 rows of 1M:
+// 8.4 us; 72 items x 2048 rows 18.6 us with 16 waves an item, 23.5 with 8; two,
+// four or eight rounds in flight are alike).
 struct Verify4Params {
   const void* q;
   int q_dtype;
