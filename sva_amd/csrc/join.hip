@@ -1,4 +1,6 @@
-// The second kernel of split attention (join.h).
+// The second kernel of split attention (join.h).  Bound by the way of the sums
+// through memory, which other XCDs wrote: 9 items of 328 ranges 6 us, 768 of
+// at most 21 14 us, 36864 of six 30 us.
 #include "join.h"
 
 #include "capi_internal.h"
