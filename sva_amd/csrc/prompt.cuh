@@ -96,6 +96,29 @@ struct PromptType {
   static constexpr int waves(int dp) { return dp > 128 || (DT == F32 && dp > 64) ? 1 : 2; }
 };
 
+// Which of the four keys at mask element i (of its row) a mask allows, bit by
+// bit, in one load of any alignment.
+SVA_DEV uint32_t prompt_mask_allows4(const void* row, int64_t i, int mtype) {
+  if (mtype == MASK_BOOL) {
+    uint32_t u;
+    __builtin_memcpy(&u, (const uint8_t*)row + i, 4);
+    return (u & 0xFFu ? 1u : 0u) | (u & 0xFF00u ? 2u : 0u) | (u & 0xFF0000u ? 4u : 0u) | (u >> 24 ? 8u : 0u);
+  }
+  uint32_t bits = 0u;
+  if (mtype == MASK_F32) {
+    float x[4];
+    __builtin_memcpy(x, (const float*)row + i, 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) bits |= x[k] > -1e4f ? 1u << k : 0u;
+  } else {
+    uint16_t x[4];
+    __builtin_memcpy(x, (const uint16_t*)row + i, 8);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) bits |= elem_from_bits(x[k], mtype == MASK_BF16 ? BF16 : F16) > -1e4f ? 1u << k : 0u;
+  }
+  return bits;
+}
+
 SVA_DEV bool prompt_mask_allows(const void* mask, int64_t i, int mtype) {
   return mtype == MASK_BOOL ? ((const uint8_t*)mask)[i] != 0 : mask_allows(mask, i, mtype);
 }
@@ -295,13 +318,20 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const int key = n0 + 32 * kt + 8 * (k / 4) + 4 * hf + k % 4;
-        bool ok = key <= lim;
+      for (int k = 0; k < 16; k += 4) {
+        const int key = n0 + 32 * kt + 2 * k + 4 * hf;
+        uint32_t seen = 15u;
         if (MASK) {
-          if (ok) ok = prompt_mask_allows(mrow, key, p.mask_type);
+          seen = 0u;
+          if (key + 3 <= lim) {
+            seen = prompt_mask_allows4(mrow, key, p.mask_type);
+          } else {
+            for (int j = 0; j < 4; ++j)
+              if (key + j <= lim && prompt_mask_allows(mrow, key + j, p.mask_type)) seen |= 1u << j;
+          }
         }
-        s[kt][k] = ok ? s[kt][k] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[kt][k + j] = key + j <= lim && (seen >> j & 1u) ? s[kt][k + j] : -INFINITY;
       }
   };
   auto weigh = [&](const f32x16 (&s)[KT], weights (&pw)[KT]) {

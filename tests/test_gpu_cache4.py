@@ -299,3 +299,26 @@ def test_offsets_past_32_bits(device):
                        kernels.cache4_verify(q, small, small_s, idx, cnt, 300, 0.1))
     assert all(torch.equal(a, b) for a, b in zip(kernels.cache4_read(data, scales, first, 300),
                                                  kernels.cache4_read(small, small_s, 0, 300)))
+
+
+@pytest.mark.parametrize("scaling", [0.0, -0.3, 2.0])
+def test_attention_scales_and_rising_scores(device, scaling):
+    """Scales of 0 and below; keys that grow, so that the reference moves often, or shrink."""
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(21)
+    for size in (np.linspace(0.05, 20, 1500), np.linspace(20, 0.05, 1500)):
+        k = torch.from_numpy((rng.standard_normal((1, 1500, 64)) * size[:, None]).astype(np.float32)).to(device)
+        v = torch.from_numpy(rng.standard_normal((1, 1500, 64)).astype(np.float32)).to(device)
+        data, scales = kernels.cache4_alloc(1, 1500, 64, device)
+        kernels.cache4_write(k, v, data, scales, 0)
+        K, V = decoded(data, scales)
+        q = torch.from_numpy(rng.standard_normal((1, 3, 2, 64)).astype(np.float32)).to(device)
+        got = kernels.cache4_attention(q, data, scales, 1500, scaling)
+        allowed = np.arange(1500) <= 1498 + np.arange(2)[:, None]
+        sign = -1.0 if scaling < 0 else 1.0
+        for h in range(3):
+            x = sign * q[0, h].double().cpu().numpy()
+            ref, bound = attend(x, K[0], V[0], allowed, sign * scaling)
+            size_, _ = attend(x, K[0], np.abs(V[0]), allowed, sign * scaling)
+            close(got[0, h], ref, bound, scale=size_)

@@ -262,3 +262,68 @@ def test_offsets_past_32_bits(device):
     got = kernels.prompt_attention(q, k, v, 300, 0.1, seq_offsets=off, seq_lens=ln)
     want = kernels.prompt_attention(q, k[:, -300:].contiguous(), v[:, -300:].contiguous(), 300, 0.1)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rising", [True, False])
+def test_scores_far_apart_in_16_bits(device, dtype, rising):
+    """The reference moves often, or stays far above later scores; over several ranges of keys too."""
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(12)
+    for n, Q in ((500, 500), (3000, 5)):
+        q, k, v = (normal(rng, s, torch.float32, device) for s in ((1, 3, Q, 64), (1, n, 64), (1, n, 64)))
+        size = torch.linspace(0.1, 12, n, device=device)[:, None]
+        k = k * (size if rising else size.flip(0))
+        q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+        got = kernels.prompt_attention(q, k, v, n, 1.0)
+        for h in range(3):
+            check(got[0, h], q[0, h], k[0], v[0], causal(Q, n), 1.0)
+
+
+def test_a_mask_of_the_causal_rule_equals_it(device):
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(13)
+    for n, Q in ((333, 333), (1200, 70)):
+        q, k, v = (normal(rng, s, torch.bfloat16, device) for s in ((1, 6, Q, 64), (2, n, 64), (2, n, 64)))
+        mask = torch.ones(Q, n + 3, dtype=torch.bool, device=device).tril(n - Q)[:, :n]  # rows at odd addresses
+        want = kernels.prompt_attention(q, k, v, n, 0.125).float()
+        got = kernels.prompt_attention(q, k, v, n, 0.125, mask=mask).float()
+        # other ranges of keys: weights within half a step each, of values up to 4.5, and half a step of the outputs
+        assert (got - want).abs().max() <= 4.5 * 4 * HALF_STEP[torch.bfloat16]
+
+
+def test_packed_prompts_in_a_graph(device):
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(14)
+    lens = [100, 1, 60]
+    q, k, v = (normal(rng, s, torch.float16, device) for s in ((9, 161, 64), (3, 161, 64), (3, 161, 64)))
+    off, ln = torch.tensor([0, 100, 101], device=device), torch.tensor(lens, device=device)
+    out = torch.zeros(9, 161, 64, device=device, dtype=torch.float16)
+
+    def call():
+        return kernels.prompt_attention(q, k, v, 100, 0.125, seq_offsets=off, seq_lens=ln, q_offsets=off, q_lens=ln,
+                                        max_q=100, out=out)
+
+    want = call().clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for lens in ([100, 1, 60], [50, 1, 10], [100, 1, 60]):  # lengths are read when it runs
+        ln.copy_(torch.tensor(lens, device=device))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, call())
+        if lens[0] == 100:
+            assert torch.equal(got, want)
+        else:
+            assert (got[:, 50:100] == 0).all() and got[:, :50].abs().max() > 0
