@@ -15,9 +15,19 @@
 //    maximum is then taken, the sums rescaled and the weights done again.  The
 //    sum is needed anyway, so an ordinary tile looks for no maximum.  (fp16
 //    weights are 2^8 at a new reference, to keep small ones normal.)
-//  * Weights are rounded to the type of V for the product (2^-9 of each, of
-//    random sign, as V's own rounding); m, the sum of weights and the sums are
-//    fp32.  fp32 inputs use the fp32 matrix instructions throughout.
+//  * Weights are rounded to the type of V for the product (bf16: at most 2^-8
+//    of each, of random sign, as V's own rounding); m, the sum of weights and
+//    the sums are fp32.  (A second term for the rest would cost 8192 tokens of
+//    9 x 64 161 us against 120, 8 x 512 over 32768 keys 591 against 431, and
+//    prompts of 32 x 128, out of registers, four times.)  fp32 inputs use the
+//    fp32 matrix instructions throughout.
+//  * At most 16 query rows a KV head (decode tokens): memory sets the time, and
+//    half of the product's 32 columns are free.  They take each weight's second
+//    term, its rest after rounding: the outputs keep about 16 bits of the
+//    weights (bf16 difference from fp32 attention 2.5e-3 -> 6e-5).  Two waves
+//    take a tile's 32-key halves, joined in LDS.  32 sequences of up to 131072
+//    keys, 9 x 64: 293 us (one wave, one term 289); 24 of up to 42K, 32 x 128:
+//    384 (417).
 //  * Three tiles are in work at once: while tile t is weighed on the vector
 //    units, tile t + 1's scores and tile t - 1's sums are on the matrix units.
 // What bounds it: at 9 x 64, 32768 bf16 tokens (1.33 ms, 930 TFLOP/s; a
@@ -124,15 +134,18 @@ SVA_DEV bool prompt_mask_allows(const void* mask, int64_t i, int mtype) {
 }
 
 // How a call's rows are read and masked: whole aligned rows of DP elements
-// under the causal rule, the same under a mask, anything else.
-enum PromptMode : int { PROMPT_CAUSAL = 0, PROMPT_MASK = 1, PROMPT_ANY = 2 };
+// under the causal rule, the same under a mask, anything else.  PROMPT_FEW
+// added: 16-bit calls of at most 16 query rows a KV head, two-term weights.
+enum PromptMode : int { PROMPT_CAUSAL = 0, PROMPT_MASK = 1, PROMPT_ANY = 2, PROMPT_FEW = 4 };
+constexpr int kFewRows = 16;
 
 template <int DT, int DP, int MODE>
 __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(PromptParams p) {
-  constexpr bool VEC = MODE != PROMPT_ANY;
-  const bool MASK = MODE == PROMPT_MASK || (MODE == PROMPT_ANY && p.mask != nullptr);
+  constexpr int FORM = MODE % PROMPT_FEW;
+  constexpr bool VEC = FORM != PROMPT_ANY, FEW = MODE >= PROMPT_FEW;
+  const bool MASK = FORM == PROMPT_MASK || (FORM == PROMPT_ANY && p.mask != nullptr);
   constexpr int ES = PromptType<DT>::ES, BN = PromptType<DT>::BN;
-  constexpr int KT = BN / 32;            // 32-key blocks of a tile
+  constexpr int KT = FEW ? 1 : BN / 32;  // 32-key blocks of a tile that a wave takes
   constexpr int CPR = DP * ES / 16;      // 16-byte chunks of a row
   constexpr int CH = BN * CPR / 256;     // chunks per thread
   constexpr int EC = 16 / ES;            // elements of a chunk
@@ -172,9 +185,10 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   const int kend = kbeg + min(p.chunk, max(keys - kbeg, 0));
 
   // this wave's rows, one per lane and half
-  const int wrow = rt * BM + w * 32;
+  const int wrow = FEW ? 0 : rt * BM + w * 32;
   const int wend = min(rows, wrow + 32);
-  const bool busy = wrow < rows;
+  const bool busy = FEW ? w < BN / 32 : wrow < rows;
+  const int kt0 = FEW ? w : 0;  // this wave's first block of a tile
   const int wfull = min(len, wrow / grp + shift + 1);  // keys below are seen by every row of the wave
   const int64_t kvb = (int64_t)g * p.kv_hs + off * p.kv_rs;  // element offset of key 0
   auto q_at = [&](int r, int64_t bs, int64_t hs, int64_t ts) {
@@ -190,7 +204,8 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   using weights = typename std::conditional<DT == F32, f32x16, frag_pair>::type;  // of 32 keys
   constexpr int NF = DT == F32 ? DP / 8 : DP / 16;  // fragments of a row per lane
   constexpr int FE = DT == F32 ? 4 : 8;             // elements of one: d = 2 FE f + FE hf + i
-  const int row = wrow + l32;
+  const bool second = FEW && l32 >= kFewRows;  // this lane's weights are the second terms of its row's
+  const int row = wrow + (FEW ? l32 % kFewRows : l32);
   const bool live = row < rows;
   const int lim = live ? (MASK ? kend - 1 : min(kend - 1, row / grp + shift)) : -1;  // the last key of the row
   const unsigned char* mrow = nullptr;                                                 // its mask row
@@ -301,7 +316,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
       for (int k = 0; k < 16; ++k) s[kt][k] = 0.0f;
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const frag a = *(const frag*)(kb + ((32 * kt + l32) * CPR + ((2 * f + hf) ^ k_chunk<CPR>(l32))) * 16);
+        const frag a = *(const frag*)(kb + ((32 * (kt0 + kt) + l32) * CPR + ((2 * f + hf) ^ k_chunk<CPR>(l32))) * 16);
         if constexpr (DT == BF16) {
           s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, bq[f], s[kt], 0, 0, 0);
         } else if constexpr (DT == F16) {
@@ -313,13 +328,13 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
       }
     }
   };
-  // a lane's score k of block kt is key n0 + 32 kt + 8 (k / 4) + 4 hf + k % 4
+  // a lane's score k of block kt0 + kt is its key 8 (k / 4) + 4 hf + k % 4
   auto hide = [&](int n0, f32x16 (&s)[KT]) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int k = 0; k < 16; k += 4) {
-        const int key = n0 + 32 * kt + 2 * k + 4 * hf;
+        const int key = n0 + 32 * (kt0 + kt) + 2 * k + 4 * hf;
         uint32_t seen = 15u;
         if (MASK) {
           seen = 0u;
@@ -351,6 +366,11 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
           const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][k + 1], sl, -mref));
           pair e;
           e[0] = (typename Elem::type)e0, e[1] = (typename Elem::type)e1;
+          if constexpr (FEW) {
+            pair r;
+            r[0] = (typename Elem::type)(e0 - (float)e[0]), r[1] = (typename Elem::type)(e1 - (float)e[1]);
+            e = second ? r : e;
+          }
           pw[kt][k / 8][k % 8] = e[0], pw[kt][k / 8][k % 8 + 1] = e[1];
           zs = Elem::sum2(e, zs);
         }
@@ -386,7 +406,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
       if constexpr (DT == F32) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float* vrow = (const float*)(vb + (32 * kt + 8 * (k / 4) + 4 * hf + k % 4) * CPR * 16);
+          const float* vrow = (const float*)(vb + (32 * (kt0 + kt) + 8 * (k / 4) + 4 * hf + k % 4) * CPR * 16);
 #pragma unroll
           for (int i = 0; i < NO; ++i)
             o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(vrow[32 * i + l32], pw[kt][k], o[i], 0, 0, 0);
@@ -400,7 +420,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
               s16x4 half[2];
               frag v;
             } a;
-            const int row = 32 * kt + 16 * st + 4 * hf + m16 / 4;
+            const int row = 32 * (kt0 + kt) + 16 * st + 4 * hf + m16 / 4;
             const int ch = (4 * i + 2 * (lane >> 4 & 1) + (m16 & 3) / 2) ^ v_chunk<CPR>(m16 / 4);
             const unsigned char* at = vb + (row * CPR + ch) * 16 + (m16 & 1) * 8;
             a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
@@ -435,7 +455,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
         const float zs = weigh(sc, pc);
         if constexpr (DP == 128 && ES == 2) {  // a matrix instruction, then the vector instructions of its time
 #pragma unroll
-          for (int i = 0; i < 4 * NF; ++i) {
+          for (int i = 0; i < 2 * KT * NF; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
           }
@@ -462,12 +482,38 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
       sums(vbuf + ((t - 1) & 1) * TB, pw);
     }
   }
-  if (!busy) return;
+  if (!FEW && !busy) return;
 
   // the two halves of the wave hold a row's keys
   {
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(z), __float_as_uint(z), false, false);
     z = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  if constexpr (FEW) {  // both terms, then both waves: wave 0 goes on with all of it
+    z += __shfl_xor(z, kFewRows, WAVE);
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o[i][k] += __shfl_xor(o[i][k], kFewRows, WAVE);
+    float* part = (float*)lds + lane;  // [m, z, sums][lane], in the tiles' place
+    __syncthreads();
+    if (w == 1) {
+      part[0] = mref, part[WAVE] = z;
+#pragma unroll
+      for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) part[(2 + 16 * i + k) * WAVE] = o[i][k];
+    }
+    __syncthreads();
+    if (w != 0) return;
+    const float m1 = part[0], mn = fmaxf(mref, m1);
+    const float f0 = __builtin_amdgcn_exp2f(mref - mn), f1 = __builtin_amdgcn_exp2f(m1 - mn);
+    mref = mn;
+    z = z * f0 + part[WAVE] * f1;
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o[i][k] = o[i][k] * f0 + part[(2 + 16 * i + k) * WAVE] * f1;
   }
   bool odd = false;
 #pragma unroll
@@ -532,7 +578,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
     }
     return;
   }
-  if (!live) return;
+  if (!live || second) return;
   // four consecutive elements at a time
   void* dst = partial ? (void*)p.sums : p.out;
   const int type = partial ? (int)F32 : p.out_dtype;

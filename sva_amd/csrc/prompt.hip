@@ -1,12 +1,8 @@
 // Dense attention of whole prompts (sva_prompt_attention): argument checks,
 // the choice of tile and of key ranges, launches.  The kernel: prompt.cuh.
 #include <algorithm>
-#include <type_traits>
 
-#include "prompt.cuh"
-
-#include "capi_internal.h"
-#include "summon.h"
+#include "prompt_launch.h"
 
 using namespace sva;
 
@@ -35,28 +31,14 @@ int64_t chunk_keys(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t n_key
   return std::max<int64_t>(256, ((n_keys + ranges - 1) / ranges + 63) / 64 * 64);
 }
 
-template <int DT, int DP, int MODE>
-int launch(const PromptParams& p, hipStream_t stream) {
-  constexpr int lds = 4 * PromptType<DT>::BN * DP * PromptType<DT>::ES;
-  constexpr auto fn = prompt_kernel<DT, DP, MODE>;
-  SVA_SET_MAX_LDS_ONCE(fn, sva::kMaxLds, "hipFuncSetAttribute(prompt_kernel)");
-  const int64_t blocks = (int64_t)p.G * p.row_tiles * p.splits * p.n_seq;
-  hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), lds, stream, p);
-  SVA_CHECK_LAUNCH("prompt_kernel");
-  return SVA_OK;
-}
-
-template <int DT, int MODE>
-int launch_dim(const PromptParams& p, hipStream_t stream) {
-  if (p.D <= 64) return launch<DT, 64, MODE>(p, stream);
-  if (p.D <= 128) return launch<DT, 128, MODE>(p, stream);
-  return launch<DT, 256, MODE>(p, stream);
-}
-
+// (few rows: their second terms cost nothing there; from 17 rows on they would
+// need columns of their own, prompt.cuh)
 template <int DT>
-int launch_mode(const PromptParams& p, bool vec, hipStream_t stream) {
-  if (!vec) return launch_dim<DT, PROMPT_ANY>(p, stream);
-  return p.mask ? launch_dim<DT, PROMPT_MASK>(p, stream) : launch_dim<DT, PROMPT_CAUSAL>(p, stream);
+int launch_type(const PromptParams& p, bool vec, hipStream_t stream) {
+  if constexpr (DT != F32) {
+    if ((int64_t)p.H / p.G * p.Q <= kFewRows) return launch_prompt_few(p, DT, vec, stream);
+  }
+  return launch_prompt<DT, 0>(p, vec, stream);
 }
 
 }  // namespace
@@ -142,9 +124,9 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   p.o_ts = out_tok_stride;
   SVA_REQUIRE((int64_t)p.G * p.row_tiles * p.splits * n_seq < (1ll << 31), "sva_prompt_attention: too many items");
   int rc;
-  if (dtype == F32) rc = launch_mode<F32>(p, vec, (hipStream_t)stream);
-  else if (dtype == BF16) rc = launch_mode<BF16>(p, vec, (hipStream_t)stream);
-  else rc = launch_mode<F16>(p, vec, (hipStream_t)stream);
+  if (dtype == F32) rc = launch_type<F32>(p, vec, (hipStream_t)stream);
+  else if (dtype == BF16) rc = launch_type<BF16>(p, vec, (hipStream_t)stream);
+  else rc = launch_type<F16>(p, vec, (hipStream_t)stream);
   if (rc != SVA_OK || p.splits == 1) return rc;
   JoinParams j;
   j.sums = p.sums;
