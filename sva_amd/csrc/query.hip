@@ -78,14 +78,19 @@ __global__ void __launch_bounds__(PREP_BLOCK) query_lut_kernel(LutParams p) {
   {
     const float4* w4 = reinterpret_cast<const float4*>(p.q_proj + (int64_t)h * D * R);
     for (int i = t; i < D * R / 4; i += PREP_BLOCK) reinterpret_cast<float4*>(W)[i] = w4[i];
-    const float4* c4 = reinterpret_cast<const float4*>(p.codebooks + (int64_t)h * S * C * sub);
-    for (int i = t; i < S * C * sub / 4; i += PREP_BLOCK) {
-      const float4 v = c4[i];
-      float* row = cb + (4 * i / sub) * cbs + (4 * i) % sub;  // sub % 4 == 0: a float4 stays in its row
-      row[0] = v.x;
-      row[1] = v.y;
-      row[2] = v.z;
-      row[3] = v.w;
+    const float* books = p.codebooks + (int64_t)h * S * C * sub;
+    if (sub % 4 == 0) {  // a float4 stays in its row
+      const float4* c4 = reinterpret_cast<const float4*>(books);
+      for (int i = t; i < S * C * sub / 4; i += PREP_BLOCK) {
+        const float4 v = c4[i];
+        float* row = cb + (4 * i / sub) * cbs + (4 * i) % sub;
+        row[0] = v.x;
+        row[1] = v.y;
+        row[2] = v.z;
+        row[3] = v.w;
+      }
+    } else {
+      for (int i = t; i < S * C * sub; i += PREP_BLOCK) cb[i / sub * cbs + i % sub] = books[i];
     }
   }
   const int64_t qbase = (int64_t)b * p.q_bs + (int64_t)h * p.q_hs + (int64_t)tq * p.q_ts;
