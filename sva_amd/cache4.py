@@ -5,17 +5,31 @@ about a quarter of a bf16 cache's memory.
 patched with scan-mode SVA attention read it in place: new rows are written
 once, a decode token's lookup is verified on the 4-bit rows it chose
 (``kernels.cache4_verify``), and the key catalog comes from the keys as the
-model made them.  Other layers get the rows back in the model's type, so a
+model made them.  The catalog is kept with the cache, so caches may be decoded
+in turn, cut and copied.  Other layers get the rows back in the model's type, so a
 partly patched model runs too (the read costs what a 16-bit cache would).
 One sequence per cache, head_dim a multiple of 32 up to 256.
 """
 
 from __future__ import annotations
 
+from dataclasses import dataclass
+
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
 from . import kernels
+
+
+@dataclass
+class Catalog:
+    """The key catalog of one patched layer over a FourBitLayer: k_low [H, capacity, R] and codes [H, capacity, S], of
+    which the first `rows` rows are those of the cache."""
+
+    owner: str
+    k_low: torch.Tensor
+    codes: torch.Tensor
+    rows: int = 0
 
 
 class FourBitLayer(CacheLayerMixin):
@@ -28,6 +42,7 @@ class FourBitLayer(CacheLayerMixin):
         self.data: torch.Tensor | None = None
         self.scales: torch.Tensor | None = None
         self.length = 0
+        self.catalog: Catalog | None = None
 
     def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
         self.dtype, self.device = key_states.dtype, key_states.device
@@ -54,10 +69,32 @@ class FourBitLayer(CacheLayerMixin):
             kernels.cache4_write(key_states, value_states, self.data, self.scales, self.length)
         self.length = end
 
-    def read(self, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        """Keys and values [1, G, length, D] of the rows in use."""
+    def read(self, dtype: torch.dtype | None = None, begin: int = 0,
+             end: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values [1, G, rows, D] of the rows in use, or of [begin, end) of them."""
 
-        return kernels.cache4_read(self.data, self.scales, 0, self.length, dtype or self.dtype)
+        end = self.length if end is None else end
+        return kernels.cache4_read(self.data, self.scales, begin, end - begin, dtype or self.dtype)
+
+    def catalog_of(self, owner: str, heads: int, rank: int, subspaces: int, code_dtype: torch.dtype) -> Catalog:
+        """The catalog of the patched layer `owner`, with room for every row of the cache: the one kept here, or an
+        empty one in its place where that is another layer's."""
+
+        kept, capacity = self.catalog, self.data.shape[1]
+        if kept is not None and kept.owner == owner and kept.k_low.shape[1] >= capacity:
+            return kept
+        self.catalog = Catalog(owner, torch.empty(heads, capacity, rank, device=self.device),
+                               torch.empty(heads, capacity, subspaces, device=self.device, dtype=code_dtype))
+        if kept is not None and kept.owner == owner:
+            self.catalog.rows = n = kept.rows
+            self.catalog.k_low[:, :n].copy_(kept.k_low[:, :n])
+            self.catalog.codes[:, :n].copy_(kept.codes[:, :n])
+        return self.catalog
+
+    def _cut(self, length: int) -> None:
+        self.length = length
+        if self.catalog is not None:
+            self.catalog.rows = min(self.catalog.rows, length)
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args, **kwargs):
         """For layers that attend by themselves: the rows so far, as they are held (a first prompt: as given)."""
@@ -76,13 +113,13 @@ class FourBitLayer(CacheLayerMixin):
         return -1
 
     def reset(self) -> None:
-        self.length = 0
+        self._cut(0)
 
     def crop(self, tokens_to_remove: int) -> None:
         """Drops the last -tokens_to_remove rows (a positive number: rows behind it)."""
 
         keep = tokens_to_remove if tokens_to_remove > 0 else self.length + tokens_to_remove
-        self.length = max(0, min(self.length, keep))
+        self._cut(max(0, min(self.length, keep)))
 
     def offload(self) -> None:
         raise NotImplementedError("a 4-bit cache stays on the GPU")

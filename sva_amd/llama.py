@@ -20,6 +20,7 @@ repeat_kv).
 from __future__ import annotations
 
 import time
+import uuid
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Any
@@ -121,6 +122,7 @@ class SVALlamaAttention(nn.Module):
         return (time.perf_counter() - start) * 1000.0
 
     def reset_catalog(self) -> None:
+        self._catalog_owner = uuid.uuid4().hex       # names this layer's catalogs in 4-bit caches (never one of another)
         self._k_low: torch.Tensor | None = None      # [H, capacity, R] fp32
         self._codes: torch.Tensor | None = None      # [H, capacity, S]
         self._key_len = 0                            # rows with k_low (and, unless lazy, codes)
@@ -293,9 +295,9 @@ class SVALlamaAttention(nn.Module):
     def _attention_cache4(self, query, key, value, held, attention_mask):
         """sva_attention over a cache held in 4 bits (cache4.FourBitCache):
         the new rows key / value [1, G, T, D] are written to it, the catalog
-        is appended from them as they are, and the lookup's rows are verified
-        where they lie.  A chunk of a prompt by dense attention reads the rows
-        before it back."""
+        that it keeps is appended from them as they are, and the lookup's rows
+        are verified where they lie.  A chunk of a prompt by dense attention
+        reads the rows before it back."""
 
         if self.serving.summon_mode != "scan" or query.shape[0] != 1:
             raise ValueError("A 4-bit cache takes one sequence in summon_mode='scan'.")
@@ -303,25 +305,26 @@ class SVALlamaAttention(nn.Module):
         q_len, start = query.shape[2], held.length
         held.append(key, value)
         k_len = held.length
-        sig = ("cache4", key.device, key.dtype, self._heads, key.shape[3], self.serving.rank_dim)
-        self._ensure_capacity(k_len, key.device)
-        if start == 0 or (self._signature == sig and self._key_len == self._codes_len == start):
-            rows, row0 = key[0], start
-        else:  # the catalog of another cache, or of rows since dropped
-            rows, row0 = held.read()[0][0], 0
-        kernels.write_encode(rows if rows.stride(-1) == 1 else rows.contiguous(), self.sva_k_proj,
-                             self.sva_coarse_codebooks, self._k_low[:, row0:k_len], self._codes[:, row0:k_len], 0,
-                             k_len - row0)
-        self._key_len = self._codes_len = k_len
-        self._postings = self._fast = None
-        self._signature = sig
+        catalog = held.catalog_of(self._catalog_owner, self._heads, self._rank, self._subspaces,
+                                  _code_dtype(self._codewords))
+
+        def encode(rows, begin, end):
+            kernels.write_encode(rows if rows.stride(-1) == 1 else rows.contiguous(), self.sva_k_proj,
+                                 self.sva_coarse_codebooks, catalog.k_low[:, begin:end], catalog.codes[:, begin:end], 0,
+                                 end - begin)
+            catalog.rows = end
+
+        if catalog.rows < start:  # rows that came in without this layer: as they are held
+            begin = catalog.rows
+            encode(held.read(begin=begin, end=start)[0][0], begin, start)
+        encode(key[0], start, k_len)
         mask = None if attention_mask is None else attention_mask[..., :q_len, :k_len]
         if q_len > 1 and self.serving.prompt_attention == "dense":
             keys, values = (key, value) if start == 0 else held.read(query.dtype)
             return self._dense_prompt(query, keys[0], values[0], k_len, mask)
         shortlist = min(self.serving.coarse_shortlist, k_len)
         budget = min(self.serving.budget, shortlist)
-        return self._scan_attention(query, held, None, self._k_low, self._codes, k_len, mask, shortlist, budget)
+        return self._scan_attention(query, held, None, catalog.k_low, catalog.codes, k_len, mask, shortlist, budget)
 
     def _scan_attention(self, query, keys, values, k_low, codes, k_len, mask, shortlist, budget):
         """sva/llama.py:226-328 on the HIP path, chunked over query tokens.
