@@ -9,7 +9,7 @@ namespace sva {
 
 struct JoinParams {
   const float* sums;   // [n_seq * H * Q, splits, D]
-  const float* stats;  // [n_seq * H * Q, splits, 2]: m, z; z = 0: the range has no key, its sums are not read
+  const float* stats;  // [n_seq * H * Q, splits, 2]: m, z; a range in which the item sees no key: z and sums of 0
   int splits, H, G, Q, D;
   const int64_t* q_lens;     // packed tokens: sequence b's are rows q_offsets[b] + t, t < q_lens[b], of q_rows;
   const int64_t* q_offsets;  // NULL: Q tokens of every sequence

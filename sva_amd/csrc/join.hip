@@ -36,8 +36,10 @@ SVA_DEV JoinItem join_item(const JoinParams& p, int item) {
   return x;
 }
 
-// A range's share of the joined sums: 2^(m - M).  (A range without a key has
-// sums of 0; one done again whose scores are all NaN has m = -inf and z NaN.)
+// A range's share of the joined sums: 2^(m - M).  A share of 0 still counts:
+// sums that are not finite stay so, as in one range.  (A range without a key
+// has sums of 0; one done again whose scores are all NaN has m = -inf and z
+// NaN.)
 SVA_DEV float join_share(float m, float M) { return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M); }
 
 // Few items of many ranges (decode): a workgroup takes 32 elements of one
@@ -73,11 +75,10 @@ __global__ void __launch_bounds__(JB) join_kernel(JoinParams p) {
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float c = s0 + u * PARTS < x.ranges ? join_share(st[u].x, M) : 0.0f;
-      if (c != 0.0f) {
-        Z += st[u].y * c;
-        a += sm[u] * c;
-      }
+      if (s0 + u * PARTS >= x.ranges) continue;
+      const float c = join_share(st[u].x, M);
+      Z += st[u].y * c;
+      a += sm[u] * c;
     }
   }
   red[0][threadIdx.x] = a;
@@ -124,11 +125,10 @@ __global__ void __launch_bounds__(RB) join_rows_kernel(JoinParams p, int items) 
       Z *= c, a *= c, M = top;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float f = s0 + u < x.ranges ? join_share(st[u].x, M) : 0.0f;
-        if (f != 0.0f) {
-          Z += st[u].y * f;
-          a += sm[u] * f;
-        }
+        if (s0 + u >= x.ranges) continue;
+        const float f = join_share(st[u].x, M);
+        Z += st[u].y * f;
+        a += sm[u] * f;
       }
     }
     store_elem(p.out, x.at + d, p.out_dtype, Z == 0.0f ? 0.0f : a / Z);
