@@ -1080,13 +1080,14 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
     if out.numel() == 0 or n_seq == 0 or q_len == 0:
         return out
     if n_keys <= 0:
-        if packed:
-            n_keys = 1  # (every length is 0: the rows of sequences become 0)
-            if rows == 0:
-                keys = values = keys.new_zeros(kv_heads, 1, dim)
-                rows = 1
-        else:
+        if not packed:
             return out.zero_()
+        # rows of sequences become 0: one key, and lengths of 0
+        n_keys = 1
+        seq_offsets = seq_lens = torch.zeros(n_seq, device=device, dtype=torch.int64)
+        if rows == 0:
+            keys = values = keys.new_zeros(kv_heads, 1, dim)
+            rows = 1
     m, mtype, mseq, mtok = (None, 0, 0, 0) if mask is None else _prompt_mask(mask, n_seq, q_len, n_keys)
     o4 = out if out.dim() == 4 else out.unsqueeze(0)
     # a buffer of the call's own: calls on other streams and captured graphs never share one

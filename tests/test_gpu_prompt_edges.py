@@ -1,4 +1,4 @@
-"""Prompt attention: the accuracy of few rows."""
+"""Prompt attention: empty caches and the accuracy of few rows."""
 
 from __future__ import annotations
 
@@ -11,6 +11,24 @@ from .test_gpu_cache4 import close
 from .test_gpu_prompt_attention import normal
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("Q", [1, 4])
+def test_packed_tokens_over_no_key_are_zero(device, Q):
+    """n_keys 0: nothing is seen, whatever the cache's rows and the given lengths hold."""
+    from sva_amd import kernels
+
+    ones = lambda *s: torch.ones(*s, device=device)  # noqa: E731
+    zero = torch.zeros(1, dtype=torch.int64, device=device)
+    for where in ({}, {"seq_offsets": zero, "seq_lens": zero}, {"seq_offsets": zero, "seq_lens": zero + 5}):
+        got = kernels.prompt_attention(ones(2, Q + 2, 64), ones(1, 9, 64), ones(1, 9, 64), 0, 1.0, q_offsets=zero + 1,
+                                       q_lens=zero + Q, max_q=Q, out=ones(2, Q + 2, 64) * 5, **where)
+        assert (got[:, 1:Q + 1] == 0).all() and (got[:, 0] == 5).all() and (got[:, -1] == 5).all()
+    two = torch.zeros(2, dtype=torch.int64, device=device)
+    got = kernels.prompt_attention(ones(2, 4, 64), ones(1, 0, 64), ones(1, 0, 64), 0, 1.0, seq_offsets=two,
+                                   seq_lens=two, q_offsets=torch.tensor([0, 3], device=device), q_lens=two + 1,
+                                   max_q=1, out=ones(2, 4, 64) * 5)
+    assert (got[:, [0, 3]] == 0).all() and (got[:, [1, 2]] == 5).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
