@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
   const int full = min(k1, len - p.Q + rt * TR / grp + 1);      // keys below are seen by every row
   // (a scale of 0: the smallest normal one gives the same weights, and -inf times it stays -inf)
   const float sl = fmaxf(fabsf(p.scaling) * kLog2e, 1.17549435e-38f);
-  float mref = -3.0e38f, z = 0.0f;
+  float top = -3.40282347e38f, z = 0.0f;  // the largest score that the reference m = top * sl stands for
   uint32_t nan_blocks = 0u;
   f32x4 o[2 * NB];
 #pragma unroll
@@ -194,12 +194,14 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
         for (int i = 0; i < 4; ++i) s[t][i] = base + 16 * t + 4 * qd + i <= lim ? s[t][i] : -INFINITY;
     }
     bf16x8 pw[NP];
+    // (the reference comes off before the scale, exactly: rounded after it, as fma(s, sl, -m) would take it, it is off
+    // by more than the weights' range from scores of 2^30 on)
     auto weigh = [&]() {
       float zs = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], sl, -mref));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4 + 1], sl, -mref));
+        const float e0 = __builtin_amdgcn_exp2f((s[i / 4][i % 4] - top) * sl);
+        const float e1 = __builtin_amdgcn_exp2f((s[i / 4][i % 4 + 1] - top) * sl);
         bf16x2 h;
         h[0] = (__bf16)e0, h[1] = (__bf16)e1;
         pw[0][i] = h[0], pw[0][i + 1] = h[1];
@@ -217,14 +219,13 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
     // score): the sum is needed anyway, so an ordinary tile looks for no maximum
     float zs = weigh();
     if (__any(zs > kMost)) {
-      float top = s[0][0];
+      float most = top;
 #pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
-      top = fmaxf(top, __shfl_xor(top, 16, WAVE));
-      top = fmaxf(top, __shfl_xor(top, 32, WAVE));
-      const float mn = fmaxf(mref, top * sl);
-      const float corr = __builtin_amdgcn_exp2f(mref - mn);
-      mref = mn;
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, s[i / 4][i % 4]);
+      most = fmaxf(most, __shfl_xor(most, 16, WAVE));
+      most = fmaxf(most, __shfl_xor(most, 32, WAVE));
+      const float corr = __builtin_amdgcn_exp2f((top - most) * sl);
+      top = most;
       z *= corr;
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) o[i] *= corr;
@@ -276,6 +277,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
   nan_blocks |= (uint32_t)__shfl_xor((int)nan_blocks, 32, WAVE);
   __syncthreads();
   float* mine = (float*)lds + (w * TR + m16) * PS;
+  const float mref = fminf(fmaxf(top * sl, -3.40282347e38f), 3.40282347e38f);
   if (qd == 0) mine[0] = mref, mine[1] = z, mine[2] = __uint_as_float(nan_blocks);
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) {

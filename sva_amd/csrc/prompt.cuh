@@ -40,7 +40,9 @@
 // for their longest row tile (8192 tokens: 576 workgroups, 120 us).
 //  * A masked key's V meets a weight of 0, which a NaN or an infinity
 //    survives: a wave whose sums are not finite does its rows again, key by
-//    key, over the keys they may see alone (some hundred times the time).
+//    key, over the keys they may see alone (some hundred times the time).  So
+//    does one with a score past 2^26, where a reference in fp32 is no longer
+//    within a few units of it.
 #pragma once
 // (loads to LDS name m0 among what they change)
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -155,6 +157,8 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   constexpr float kLog2e = 1.44269504088896340736f;
   constexpr float kMost = DT == F16 ? 32768.0f : 65536.0f;  // a lane's weights of a tile may sum to
   constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;         // how far below the maximum a new reference lies
+  constexpr float kNoKey = -3.40282347e38f;                 // the reference of a row that has seen no key
+  constexpr float kFar = 67108864.0f;                       // references past 2^26: done again
   using Elem = PromptType<DT>;
   using pair = typename Elem::pair;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -242,7 +246,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   const float sl = fmaxf(fabsf(p.scaling) * kLog2e, 1.17549435e-38f);
 
   f32x16 o[NO];
-  float mref = -3.0e38f, z = 0.0f;
+  float mref = kNoKey, z = 0.0f;
 #pragma unroll
   for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -515,7 +519,8 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
 #pragma unroll
       for (int k = 0; k < 16; ++k) o[i][k] = o[i][k] * f0 + part[(2 + 16 * i + k) * WAVE] * f1;
   }
-  bool odd = false;
+  // (fma(s, sl, -m) is exact before its rounding, m is not: it is off by up to 2 at 2^26, by 128 at 2^31)
+  bool odd = mref != kNoKey && fabsf(mref) > kFar;
 #pragma unroll
   for (int i = 0; i < NO; ++i)
 #pragma unroll
