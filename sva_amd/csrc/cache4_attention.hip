@@ -16,6 +16,8 @@
 //  * S^T leaves a lane with 8 scores of one query row, which are its share of
 //    the P^T operand: weights never cross lanes.  V goes through LDS, each
 //    wave its own 32 rows, and comes back transposed (ds_read_b64_tr_b16).
+//  * V near the type's largest meets weights of 2^-60 (the reference lies 60
+//    above the maximum from the first such block on): its sums stay finite.
 //  * A block that reads as NaN is kept out of V (0 * NaN would reach rows that
 //    may not see it) and marks the query rows that may.
 // Workgroups split the keys (partials joined by a second kernel), a
@@ -69,6 +71,9 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
   constexpr int SB = NB > 4 ? NB / 4 : 1;  // scale blocks a lane's words lie in
   constexpr int LDS = AW * (TK * VS > TR * PS * 4 ? TK * VS : TR * PS * 4);
   constexpr float kMost = 65536.0f;  // a lane's weights of a tile may sum to
+  // scales of V from 2^64 on: sums of smaller V (weights of 2^18 a row and tile) and, with weights of 2^-60 of that,
+  // of any V stay below 2^110 over 2^24 tiles, and all waves and ranges together below fp32's largest number
+  constexpr uint32_t kLarge = (127u + 64u) << 23;
   __shared__ __align__(16) unsigned char lds[LDS];
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
   const int m16 = lane & 15, qd = lane >> 4;
@@ -111,7 +116,8 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
   const int full = min(k1, len - p.Q + rt * TR / grp + 1);      // keys below are seen by every row
   // (a scale of 0: the smallest normal one gives the same weights, and -inf times it stays -inf)
   const float sl = fmaxf(fabsf(p.scaling) * kLog2e, 1.17549435e-38f);
-  float top = -3.40282347e38f, z = 0.0f;  // the largest score that the reference m = top * sl stands for
+  float top = -3.40282347e38f, z = 0.0f;  // the largest score that the reference m = top * sl + above stands for
+  float above = 0.0f, most_sum = kMost;
   uint32_t nan_blocks = 0u;
   f32x4 o[2 * NB];
 #pragma unroll
@@ -180,7 +186,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
       for (int j = 0; j < NB; ++j) {
         const uint32_t sc = x.vs[t][NB > 4 ? j / 4 : 0];
         const bool nan = sc == 0x7F800000u;
-        bad = bad || nan;
+        bad = bad || sc >= kLarge;
         const bf16x8 v = cache4_unpack8_bf16(nan ? 0u : x.vc[t][j], __uint_as_float(nan ? 0x3F800000u : sc));
         *(bf16x8*)(vl + (16 * t + m16) * VS + (qd * NB + j) * 16) = v;
       }
@@ -193,6 +199,27 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[t][i] = base + 16 * t + 4 * qd + i <= lim ? s[t][i] : -INFINITY;
     }
+    if (__ballot(bad) != 0ull) {  // some V block of the tile is large, or reads as NaN
+      bool large = false;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int b = 0; b < SB; ++b) large = large || (x.vs[t][b] >= kLarge && x.vs[t][b] != 0x7F800000u);
+      if (above == 0.0f && __any(large)) {
+        above = 60.0f, most_sum = kMost * 0x1p-60f;
+        z *= 0x1p-60f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) o[i] *= 0x1p-60f;
+      }
+      // which NaN blocks may this query row see?
+      for (int i = 0; i < 8; ++i) {
+        const int key = base + 16 * (i / 4) + 4 * qd + i % 4;
+        if (key > lim) continue;
+        const uint8_t* sp = p.scales + ((row0 + key) * 2 + 1) * blocks;
+        for (int n = 0; n < blocks; ++n)
+          if (sp[n] == kCache4Nan) nan_blocks |= 1u << n;
+      }
+    }
     bf16x8 pw[NP];
     // (the reference comes off before the scale, exactly: rounded after it, as fma(s, sl, -m) would take it, it is off
     // by more than the weights' range from scores of 2^30 on)
@@ -200,8 +227,8 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
       float zs = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const float e0 = __builtin_amdgcn_exp2f((s[i / 4][i % 4] - top) * sl);
-        const float e1 = __builtin_amdgcn_exp2f((s[i / 4][i % 4 + 1] - top) * sl);
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4] - top, sl, -above));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4 + 1] - top, sl, -above));
         bf16x2 h;
         h[0] = (__bf16)e0, h[1] = (__bf16)e1;
         pw[0][i] = h[0], pw[0][i + 1] = h[1];
@@ -218,7 +245,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
     // the reference moves where the weights sum to more than kMost (the first tile always: it starts below every
     // score): the sum is needed anyway, so an ordinary tile looks for no maximum
     float zs = weigh();
-    if (__any(zs > kMost)) {
+    if (__any(zs > most_sum)) {
       float most = top;
 #pragma unroll
       for (int i = 0; i < 8; ++i) most = fmaxf(most, s[i / 4][i % 4]);
@@ -232,15 +259,6 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
       zs = weigh();
     }
     z += zs;
-    if (__ballot(bad) != 0ull) {  // some V block of the tile reads as NaN: which of them may this query row see?
-      for (int i = 0; i < 8; ++i) {
-        const int key = base + 16 * (i / 4) + 4 * qd + i % 4;
-        if (key > lim) continue;
-        const uint8_t* sp = p.scales + ((row0 + key) * 2 + 1) * blocks;
-        for (int n = 0; n < blocks; ++n)
-          if (sp[n] == kCache4Nan) nan_blocks |= 1u << n;
-      }
-    }
     // sums: rows = elements 16 i + .., columns = query rows
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) {
@@ -277,7 +295,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
   nan_blocks |= (uint32_t)__shfl_xor((int)nan_blocks, 32, WAVE);
   __syncthreads();
   float* mine = (float*)lds + (w * TR + m16) * PS;
-  const float mref = fminf(fmaxf(top * sl, -3.40282347e38f), 3.40282347e38f);
+  const float mref = fminf(fmaxf(top * sl, -3.40282347e38f), 3.40282347e38f) + above;
   if (qd == 0) mine[0] = mref, mine[1] = z, mine[2] = __uint_as_float(nan_blocks);
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) {
