@@ -134,10 +134,12 @@ __global__ void __launch_bounds__(WB) cache4_read_kernel(Cache4Rows p) {
 // query, of a row's K and V and of the sums, so a row is one 4-byte load per
 // lane and half, and a wave takes 64 / LPR rows a round, U rounds in flight.
 // Each row slot keeps an online softmax of its own (32-bit); slots merge by
-// cross-lane sums, waves through LDS.  A chosen row is two lines of the
+// cross-lane sums, waves through LDS.  (From the first V block with a scale of
+// 2^64 on a wave's weights and sums are 2^-60 of themselves: sums of any V stay
+// finite.)  A chosen row is two lines of the
 // cache wherever it is, so what bounds a decode step's few hundred rows is
 // the latency of list, row and merge, not bandwidth (9 heads x 512 rows of 1M:
-// 8.4 us; 72 items x 2048 rows 18.6 us with 16 waves an item, 23.5 with 8; two,
+// 8.4 us; 72 items x 2048 rows 19.1 us with 16 waves an item, 23.5 with 8; two,
 // four or eight rounds in flight are alike).
 struct Verify4Params {
   const void* q;
@@ -162,7 +164,8 @@ template <int LPR, int WPI>
 __global__ void __launch_bounds__(WPI * WAVE) cache4_verify_kernel(Verify4Params p) {
   constexpr int RPW = WAVE / LPR;  // rows a wave takes a round
   constexpr int U = 4;             // rounds in flight
-  __shared__ float part[WPI][LPR * 8 + 2];
+  constexpr uint32_t kLarge = 127 + 64;  // a scale byte
+  __shared__ float part[WPI][LPR * 8 + 3];  // a wave's m, z, scale of weights, sums
   const int64_t item = blockIdx.x;
   const int lane = lane_id(), w = (int)threadIdx.x / WAVE;
   const int slot = lane / LPR, c = lane % LPR;
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(WPI * WAVE) cache4_verify_kernel(Verify4Params
   }
   const int NB = p.D / kCache4Block;
   const int64_t row0 = (int64_t)g * p.rows + off;
-  float m = -INFINITY, z = 0.0f, acc[8];
+  float m = -INFINITY, z = 0.0f, down = 1.0f, acc[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
   for (int r0 = w * RPW * U; r0 < count; r0 += WPI * RPW * U) {
@@ -217,6 +220,15 @@ __global__ void __launch_bounds__(WPI * WAVE) cache4_verify_kernel(Verify4Params
       sc[u] = ok[u] ? d * p.scaling : -INFINITY;
       mn = fmaxf(mn, sc[u]);
     }
+    bool large = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) large = large || (vs[u] >= kLarge && vs[u] != (uint32_t)kCache4Nan);
+    if (down == 1.0f && __any(large)) {
+      down = 0x1p-60f;
+      z *= down;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] *= down;
+    }
     // no row yet: the sums stay 0.  A NaN score leaves the maximum alone and makes its own weight NaN.
     const float corr = mn == -INFINITY ? 1.0f : __expf(m - mn);
     z *= corr;
@@ -224,7 +236,7 @@ __global__ void __launch_bounds__(WPI * WAVE) cache4_verify_kernel(Verify4Params
     for (int i = 0; i < 8; ++i) acc[i] *= corr;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float wt = ok[u] ? __expf(sc[u] - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
+      const float wt = ok[u] ? __expf(sc[u] - (mn == -INFINITY ? 0.0f : mn)) * down : 0.0f;
       float v[8];
       cache4_unpack8(vc[u], cache4_scale(vs[u]), v);
       z += wt;
@@ -246,21 +258,22 @@ __global__ void __launch_bounds__(WPI * WAVE) cache4_verify_kernel(Verify4Params
     float a = acc[i] * f;
 #pragma unroll
     for (int s = LPR; s < WAVE; s <<= 1) a += __shfl_xor(a, s, WAVE);
-    if (slot == 0) part[w][2 + 8 * c + i] = a;
+    if (slot == 0) part[w][3 + 8 * c + i] = a;
   }
-  if (lane == 0) part[w][0] = M, part[w][1] = Z;
+  if (lane == 0) part[w][0] = M, part[w][1] = Z, part[w][2] = down;
   __syncthreads();
   for (int d = (int)threadIdx.x; d < p.D; d += WPI * WAVE) {
-    float Mi = -INFINITY;
+    float Mi = -INFINITY, least = 1.0f;
 #pragma unroll
-    for (int v = 0; v < WPI; ++v) Mi = fmaxf(Mi, part[v][0]);
+    for (int v = 0; v < WPI; ++v) Mi = fmaxf(Mi, part[v][0]), least = fminf(least, part[v][2]);
     float Zi = 0.0f, a = 0.0f;
 #pragma unroll
     for (int v = 0; v < WPI; ++v) {
       const float mv = part[v][0];
-      const float fv = mv == -INFINITY ? 1.0f : __expf(mv - Mi);  // (no rows: its sums are 0, or NaN)
+      const float even = part[v][2] == least ? 1.0f : least;
+      const float fv = mv == -INFINITY ? 1.0f : __expf(mv - Mi) * even;  // (no rows: its sums are 0, or NaN)
       Zi += part[v][1] * fv;
-      a += part[v][2 + d] * fv;
+      a += part[v][3 + d] * fv;
     }
     const int64_t o = (int64_t)b * p.o_bs + (int64_t)h * p.o_hs + (int64_t)t * p.o_ts + d;
     store_elem(p.out, o, p.out_dtype, Zi == 0.0f ? 0.0f : a / Zi);

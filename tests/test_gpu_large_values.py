@@ -49,3 +49,18 @@ def test_cache4_attention(device, kind, size, dtype, n):
         scale, _ = attend(x, K[0], np.abs(V[0]), allowed, 1.0)
         # (1e-36: products below the smallest normal number, each off by at most that)
         close(got[0, h], ref, bound + n * 2.0 ** -126, scale=scale)
+
+
+@pytest.mark.parametrize("kind,size", [("rising", 3e38), ("alike", 3e38), ("late", 3e38), ("alike", 1e36)])
+def test_cache4_verify(device, kind, size):
+    from sva_amd import kernels
+
+    q, k, v = inputs(device, kind, size, Q=1)
+    data, scales = kernels.cache4_alloc(1, N, D, device)
+    kernels.cache4_write(k, v, data, scales, 0)
+    K, V = decoded(data, scales)
+    idx = torch.arange(N, device=device, dtype=torch.int32).expand(3, N).contiguous()
+    got = kernels.cache4_verify(q, data, scales, idx, torch.full((3,), N, device=device, dtype=torch.int32), N, 1.0)
+    for h in range(3):
+        ref, bound = attend(q[0, h].double().cpu().numpy(), K[0], V[0], np.ones((1, N), bool), 1.0)
+        close(got[0, h], ref, 2 * bound)
