@@ -42,7 +42,8 @@
 //    survives: a wave whose sums are not finite does its rows again, key by
 //    key, over the keys they may see alone (some hundred times the time).  So
 //    does one with a score past 2^26, where a reference in fp32 is no longer
-//    within a few units of it.
+//    within a few units of it, and one with larger sums than the ranges'
+//    together can hold.
 #pragma once
 // (loads to LDS name m0 among what they change)
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   constexpr float kMost = DT == F16 ? 32768.0f : 65536.0f;  // a lane's weights of a tile may sum to
   constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;         // how far below the maximum a new reference lies
   constexpr float kNoKey = -3.40282347e38f;                 // the reference of a row that has seen no key
+  constexpr float kLarge = 0x1p110f;                        // 64 ranges' sums of less stay finite together
   constexpr float kFar = 67108864.0f;                       // references past 2^26: done again
   using Elem = PromptType<DT>;
   using pair = typename Elem::pair;
@@ -519,12 +521,13 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
 #pragma unroll
       for (int k = 0; k < 16; ++k) o[i][k] = o[i][k] * f0 + part[(2 + 16 * i + k) * WAVE] * f1;
   }
+  const float most = partial ? kLarge : 3.40282347e38f;
   // (fma(s, sl, -m) is exact before its rounding, m is not: it is off by up to 2 at 2^26, by 128 at 2^31)
   bool odd = mref != kNoKey && fabsf(mref) > kFar;
 #pragma unroll
   for (int i = 0; i < NO; ++i)
 #pragma unroll
-    for (int k = 0; k < 16; ++k) odd = odd || !(fabsf(o[i][k]) <= 3.40282347e38f);
+    for (int k = 0; k < 16; ++k) odd = odd || !(fabsf(o[i][k]) <= most);
   auto part_at = [&](int r) {
     const int tok = r / grp, head = g * grp + r % grp;
     return (((int64_t)b * p.H + head) * p.Q + tok) * p.splits + split;
@@ -534,41 +537,55 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
     for (int r = wrow; r < wend; ++r) {
       const int end = MASK ? kend : min(kend, r / grp + shift + 1);
       const int64_t qa = q_at(r, p.q_bs, p.q_hs, p.q_ts);
-      float m = -INFINITY, zz = 0.0f, acc[DP / 64];
+      // (finite V with larger sums: once more, weights and sums 2^-60 of themselves)
+      float m, zz, down = 1.0f, acc[DP / 64];
+      for (;;) {
+        m = -INFINITY, zz = 0.0f;
+        bool finite[DP / 64];
 #pragma unroll
-      for (int k = 0; k < DP / 64; ++k) acc[k] = 0.0f;
-      for (int n0 = kbeg; n0 < end; n0 += WAVE) {
-        const int key = n0 + lane;
-        bool ok = key < end;
-        if (MASK)
-          ok = ok && prompt_mask_allows(p.mask, (int64_t)b * p.mask_bs + (int64_t)(r / grp) * p.mask_ts + key,
-                                        p.mask_type);
-        float sc = -INFINITY;
-        if (ok) {
-          sc = 0.0f;
-          const int64_t ka = kvb + (int64_t)key * p.kv_rs;
-          for (int d = 0; d < p.D; ++d)
-            sc = __builtin_fmaf(load_elem(p.q, qa + d, DT), load_elem(p.keys, ka + d, DT), sc);
-          sc *= p.scaling * kLog2e;
-        }
-        const float mn = fmaxf(m, wave_max(sc));
-        const float corr = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float e = ok ? __builtin_amdgcn_exp2f(sc - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
-        m = mn;
-        zz = zz * corr + wave_sum(e);
+        for (int k = 0; k < DP / 64; ++k) acc[k] = 0.0f, finite[k] = true;
+        for (int n0 = kbeg; n0 < end; n0 += WAVE) {
+          const int key = n0 + lane;
+          bool ok = key < end;
+          if (MASK)
+            ok = ok && prompt_mask_allows(p.mask, (int64_t)b * p.mask_bs + (int64_t)(r / grp) * p.mask_ts + key,
+                                          p.mask_type);
+          float sc = -INFINITY;
+          if (ok) {
+            sc = 0.0f;
+            const int64_t ka = kvb + (int64_t)key * p.kv_rs;
+            for (int d = 0; d < p.D; ++d)
+              sc = __builtin_fmaf(load_elem(p.q, qa + d, DT), load_elem(p.keys, ka + d, DT), sc);
+            sc *= p.scaling * kLog2e;
+          }
+          const float mn = fmaxf(m, wave_max(sc));
+          const float corr = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          const float e = ok ? __builtin_amdgcn_exp2f(sc - (mn == -INFINITY ? 0.0f : mn)) * down : 0.0f;
+          m = mn;
+          zz = zz * corr + wave_sum(e);
 #pragma unroll
-        for (int k = 0; k < DP / 64; ++k) acc[k] *= corr;
-        const uint64_t seen = __ballot(ok);
-        for (int j = 0; j < min(WAVE, end - n0); ++j) {
-          if (!(seen >> j & 1ull)) continue;
-          const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e), j));
-          const int64_t va = kvb + (int64_t)(n0 + j) * p.kv_rs;
+          for (int k = 0; k < DP / 64; ++k) acc[k] *= corr;
+          const uint64_t seen = __ballot(ok);
+          for (int j = 0; j < min(WAVE, end - n0); ++j) {
+            if (!(seen >> j & 1ull)) continue;
+            const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(e), j));
+            const int64_t va = kvb + (int64_t)(n0 + j) * p.kv_rs;
 #pragma unroll
-          for (int k = 0; k < DP / 64; ++k) {
-            const int d = lane + 64 * k;
-            if (d < p.D) acc[k] = __builtin_fmaf(pj, load_elem(p.values, va + d, DT), acc[k]);
+            for (int k = 0; k < DP / 64; ++k) {
+              const int d = lane + 64 * k;
+              if (d < p.D) {
+                const float v = load_elem(p.values, va + d, DT);
+                finite[k] = finite[k] && fabsf(v) <= 3.40282347e38f;
+                acc[k] = __builtin_fmaf(pj, v, acc[k]);
+              }
+            }
           }
         }
+        bool large = false;
+#pragma unroll
+        for (int k = 0; k < DP / 64; ++k) large = large || (finite[k] && zz == zz && !(fabsf(acc[k]) <= kLarge));
+        if (down != 1.0f || !__any(large)) break;
+        down = 0x1p-60f;
       }
 #pragma unroll
       for (int k = 0; k < DP / 64; ++k) {
@@ -579,7 +596,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
         else
           store_elem(p.out, q_at(r, p.o_bs, p.o_hs, p.o_ts) + d, p.out_dtype, zz == 0.0f ? 0.0f : acc[k] / zz);
       }
-      if (partial && lane == 0) p.stats[2 * part_at(r)] = m, p.stats[2 * part_at(r) + 1] = zz;
+      if (partial && lane == 0) p.stats[2 * part_at(r)] = down == 1.0f ? m : m + 60.0f, p.stats[2 * part_at(r) + 1] = zz;
     }
     return;
   }

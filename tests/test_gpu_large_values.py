@@ -64,3 +64,20 @@ def test_cache4_verify(device, kind, size):
     for h in range(3):
         ref, bound = attend(q[0, h].double().cpu().numpy(), K[0], V[0], np.ones((1, N), bool), 1.0)
         close(got[0, h], ref, 2 * bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Q,n", [(2, N), (2, 200), (150, 150)])
+@pytest.mark.parametrize("kind,size", [("rising", 1e36), ("rising", 3e38), ("alike", 3e38), ("late", 3e38)])
+def test_prompt_attention(device, kind, size, Q, n, dtype):
+    from sva_amd import kernels
+
+    q, k, v = (x.to(dtype) for x in inputs(device, kind, size, Q=Q, n=n))
+    got = kernels.prompt_attention(q, k, v, n, 1.0, out_dtype=torch.float32)
+    allowed = np.arange(n) <= n - Q + np.arange(Q)[:, None]
+    for h in range(3):
+        x, K, V = (t.double().cpu().numpy() for t in (q[0, h], k[0], v[0]))
+        ref, bound = attend(x, K, V, allowed, 1.0)
+        scale, _ = attend(x, K, np.abs(V), allowed, 1.0)
+        weights = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -22
+        close(got[0, h], ref, bound, weights=weights, scale=scale)
