@@ -8,7 +8,9 @@ once, a decode token's lookup is verified on the 4-bit rows it chose
 model made them.  The catalog is kept with the cache, so caches may be decoded
 in turn, cut and copied.  Other layers get the rows back in the model's type, so a
 partly patched model runs too (the read costs what a 16-bit cache would).
-One sequence per cache, head_dim a multiple of 32 up to 256.
+One sequence per cache, head_dim a multiple of 32 up to 256.  Inference only:
+rows that require a gradient are refused (run the model under
+``torch.no_grad()``).
 """
 
 from __future__ import annotations
@@ -65,8 +67,7 @@ class FourBitLayer(CacheLayerMixin):
             data[:, :self.length].copy_(self.data[:, :self.length])
             scales[:, :self.length].copy_(self.scales[:, :self.length])
             self.data, self.scales = data, scales
-        with torch.no_grad():
-            kernels.cache4_write(key_states, value_states, self.data, self.scales, self.length)
+        kernels.cache4_write(key_states, value_states, self.data, self.scales, self.length)
         self.length = end
 
     def read(self, dtype: torch.dtype | None = None, begin: int = 0,

@@ -812,6 +812,8 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 
 def _inference_only(name: str, *tensors: torch.Tensor) -> None:
+    """Refuses tensors that require a gradient where one would be recorded."""
+
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
@@ -874,9 +876,9 @@ def cache4_write(keys: torch.Tensor, values: torch.Tensor, data: torch.Tensor, s
         raise ValueError(f"keys / values must be [n_seq, {kv_heads}, T, {dim}] of one dtype, got {keys.dtype} "
                          f"{tuple(keys.shape)} and {values.dtype} {tuple(values.shape)}")
     n_seq, _, n_rows, _ = keys.shape
+    _inference_only("cache4_write", keys, values)
     first_rows, first_row = _first_rows(first_rows, n_seq, keys.device)
     device = _same_device(keys, values, data, scales, first_rows)
-    _inference_only("cache4_write", keys, values)
     dtype = dtype_code(keys)
     if n_seq == 0 or n_rows == 0:
         return
@@ -908,7 +910,8 @@ def cache4_read(data: torch.Tensor, scales: torch.Tensor, first_rows, n_rows: in
     return keys, values
 
 
-def _cache4_query(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, n_keys: int, seq_offsets, seq_lens):
+def _cache4_query(name: str, q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, n_keys: int, seq_offsets,
+                  seq_lens):
     kv_heads, rows, dim = _check_cache4(data, scales)
     q = _as_query(q)
     n_seq, heads, q_len, head_dim = q.shape
@@ -924,6 +927,7 @@ def _cache4_query(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, n_k
     else:
         seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq)
         seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq)
+    _inference_only(name, q)
     device = _same_device(q, data, scales, seq_offsets, seq_lens)
     return q, device, kv_heads, rows, seq_offsets, seq_lens
 
@@ -936,8 +940,8 @@ def cache4_attention(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, 
     where it sees none).  One sequence of n_keys rows at row 0, or seq_offsets
     / seq_lens with n_keys at least the longest."""
 
-    q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query(q, data, scales, n_keys, seq_offsets, seq_lens)
-    _inference_only("cache4_attention", q)
+    q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query("cache4_attention", q, data, scales, n_keys,
+                                                                     seq_offsets, seq_lens)
     n_seq, heads, q_len, dim = q.shape
     out = torch.empty(n_seq, heads, q_len, dim, device=device, dtype=out_dtype or q.dtype)
     if out.numel() == 0:
@@ -960,8 +964,8 @@ def cache4_verify(q: torch.Tensor, data: torch.Tensor, scales: torch.Tensor, fin
     item over the rows its budget list names (fin_idx [items, B], fin_count
     [items], as budget_select gives them)."""
 
-    q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query(q, data, scales, n_keys, seq_offsets, seq_lens)
-    _inference_only("cache4_verify", q)
+    q, device, kv_heads, rows, seq_offsets, seq_lens = _cache4_query("cache4_verify", q, data, scales, n_keys,
+                                                                     seq_offsets, seq_lens)
     n_seq, heads, q_len, dim = q.shape
     items = n_seq * heads * q_len
     if fin_idx.dim() != 2 or fin_idx.dtype != torch.int32 or not fin_idx.is_contiguous() or fin_idx.shape[0] != items \
@@ -1060,8 +1064,8 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
         raise ValueError(f"{n_seq} sequences of up to {n_keys} keys need seq_offsets and seq_lens, or rows for them")
     if out is not None and (out.shape != shape or out.stride(-1) != 1 or (out_dtype or out.dtype) != out.dtype):
         raise ValueError(f"out must be {tuple(shape)} with contiguous rows, got {out.dtype} {tuple(out.shape)}")
-    device = _same_device(q, keys, values, mask, seq_offsets, seq_lens, q_offsets, q_lens, out)
     _inference_only("prompt_attention", q, keys, values)
+    device = _same_device(q, keys, values, mask, seq_offsets, seq_lens, q_offsets, q_lens, out)
     dtype = dtype_code(q)
     if seq_offsets is not None:
         seq_offsets = _seq_tensor("seq_offsets", seq_offsets, n_seq)

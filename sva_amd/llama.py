@@ -151,6 +151,8 @@ class SVALlamaAttention(nn.Module):
         cos, sin = position_embeddings
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
         held = cache4.layer_of(past_key_values, self.layer_idx)
+        if held is not None or (q.shape[2] > 1 and self.serving.prompt_attention == "dense"):
+            kernels._inference_only("attention over a 4-bit cache" if held is not None else "prompt_attention", q, k, v)
         if held is not None:
             out = self._attention_cache4(q, k, v, held, attention_mask)
         else:
@@ -286,11 +288,11 @@ class SVALlamaAttention(nn.Module):
         """Prompt tokens by dense attention over every key (prompt_attention
         "dense"): the catalog is kept as usual, the lookup starts with the
         first single token.  The statistics count lookups, so no prompt token.
-        A float mask allows where it is > -1e4, a bool mask where it is true."""
+        A float mask allows where it is > -1e4, a bool mask where it is true.
+        Inputs that require a gradient are refused."""
 
-        with torch.no_grad():
-            return kernels.prompt_attention(query, keys, values, k_len, self.scaling, mask=mask,
-                                            seq_offsets=seq_offsets, seq_lens=seq_lens)
+        return kernels.prompt_attention(query, keys, values, k_len, self.scaling, mask=mask, seq_offsets=seq_offsets,
+                                        seq_lens=seq_lens)
 
     def _attention_cache4(self, query, key, value, held, attention_mask):
         """sva_attention over a cache held in 4 bits (cache4.FourBitCache):
@@ -338,8 +340,7 @@ class SVALlamaAttention(nn.Module):
             _, _, sl_count, fin_idx, fin_count = kernels.summon_select(lut, rng, q_low, codes, k_low, n, shortlist,
                                                                        budget, mask=m, keep_shortlist=False)
             if values is None:
-                with torch.no_grad():
-                    outs.append(kernels.cache4_verify(qc, keys.data, keys.scales, fin_idx, fin_count, n, self.scaling))
+                outs.append(kernels.cache4_verify(qc, keys.data, keys.scales, fin_idx, fin_count, n, self.scaling))
             else:
                 outs.append(kernels.verify(qc, keys, values, fin_idx, fin_count, n, self.scaling,
                                            out_dtype=query.dtype))
