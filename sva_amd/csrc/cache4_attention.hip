@@ -62,8 +62,8 @@ struct Attend4Params {
 
 // NB: 32-element blocks of a row that the tiles are laid out for, a lane
 // holding words qd * NB .. of 8 codes each; PAD: only p.D / 32 of them are
-// there.  NT, NP: bf16 terms of the query and of the weights.
-template <int NB, bool PAD, int NT, int NP>
+// there.  NT: bf16 terms of the query.
+template <int NB, bool PAD, int NT>
 __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) cache4_attention_kernel(Attend4Params p) {
   constexpr int D = 32 * NB;
   constexpr int VS = 2 * D + 32;  // V row pitch in LDS: 4 rows x 32 bytes of a transposed read meet no bank twice
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
           if (sp[n] == kCache4Nan) nan_blocks |= 1u << n;
       }
     }
-    bf16x8 pw[NP];
+    bf16x8 pw[2];
     // (the reference comes off before the scale, exactly: rounded after it, as fma(s, sl, -m) would take it, it is off
     // by more than the weights' range from scores of 2^30 on)
     auto weigh = [&]() {
@@ -232,13 +232,8 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
         bf16x2 h;
         h[0] = (__bf16)e0, h[1] = (__bf16)e1;
         pw[0][i] = h[0], pw[0][i + 1] = h[1];
-        if constexpr (NP == 2) {
-          pw[1][i] = (__bf16)(e0 - (float)h[0]), pw[1][i + 1] = (__bf16)(e1 - (float)h[1]);
-          zs += e0 + e1;
-        } else {
-          const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
-          zs = __builtin_amdgcn_fdot2_f32_bf16(h, one, zs, false);
-        }
+        pw[1][i] = (__bf16)(e0 - (float)h[0]), pw[1][i + 1] = (__bf16)(e1 - (float)h[1]);
+        zs += e0 + e1;
       }
       return zs;
     };
@@ -270,7 +265,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
       a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
       a.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 16 * VS));
 #pragma unroll
-      for (int n = 0; n < NP; ++n) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, pw[n], o[i], 0, 0, 0);
+      for (int n = 0; n < 2; ++n) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, pw[n], o[i], 0, 0, 0);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
@@ -349,12 +344,12 @@ int64_t row_tiles(int64_t H, int64_t G, int64_t Q) { return (H / G * Q + TR - 1)
 
 template <int NB, bool PAD>
 int launch(const Attend4Params& p, dim3 grid, hipStream_t stream) {
-  if (p.q_dtype == BF16 && p.out_dtype == BF16)
-    hipLaunchKernelGGL((cache4_attention_kernel<NB, PAD, 1, 2>), grid, dim3(AW * WAVE), 0, stream, p);
-  else if (p.q_dtype != F32)
-    hipLaunchKernelGGL((cache4_attention_kernel<NB, PAD, 2, 2>), grid, dim3(AW * WAVE), 0, stream, p);
+  if (p.q_dtype == BF16)
+    hipLaunchKernelGGL((cache4_attention_kernel<NB, PAD, 1>), grid, dim3(AW * WAVE), 0, stream, p);
+  else if (p.q_dtype == F16)
+    hipLaunchKernelGGL((cache4_attention_kernel<NB, PAD, 2>), grid, dim3(AW * WAVE), 0, stream, p);
   else
-    hipLaunchKernelGGL((cache4_attention_kernel<NB, PAD, 3, 2>), grid, dim3(AW * WAVE), 0, stream, p);
+    hipLaunchKernelGGL((cache4_attention_kernel<NB, PAD, 3>), grid, dim3(AW * WAVE), 0, stream, p);
   SVA_CHECK_LAUNCH("cache4_attention_kernel");
   return SVA_OK;
 }
