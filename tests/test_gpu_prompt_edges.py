@@ -1,4 +1,4 @@
-"""Prompt attention: empty caches and the accuracy of few rows."""
+"""Prompt attention: empty caches, masks at every width and alignment, and the accuracy of few rows."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import torch
 
 from .cache4_reference import attend
 from .test_gpu_cache4 import close
-from .test_gpu_prompt_attention import normal
+from .test_gpu_prompt_attention import check, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -29,6 +29,35 @@ def test_packed_tokens_over_no_key_are_zero(device, Q):
                                    seq_lens=two, q_offsets=torch.tensor([0, 3], device=device), q_lens=two + 1,
                                    max_q=1, out=ones(2, 4, 64) * 5)
     assert (got[:, [0, 3]] == 0).all() and (got[:, [1, 2]] == 5).all()
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 128), (torch.float32, 128),
+                                     (torch.bfloat16, 256), (torch.float16, 256), (torch.float32, 256),
+                                     (torch.bfloat16, 80), (torch.float16, 17), (torch.float32, 200),
+                                     (torch.bfloat16, 64)])
+@pytest.mark.parametrize("odd", [False, True])  # rows at odd addresses
+@pytest.mark.parametrize("Q,N", [(1, 300), (67, 130), (9, 1200)])
+def test_masks_at_every_width(device, dtype, D, odd, Q, N):
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(D + Q)
+    H, G = 4, 2
+    q, k, v = (normal(rng, s, dtype, device) for s in ((1, H, Q, D), (G, N, D), (G, N, D)))
+    if odd:
+        q, k, v = (torch.empty(1 + x.numel(), device=device, dtype=dtype)[1:].view(x.shape).copy_(x)
+                   for x in (q, k, v))
+    allowed = rng.random((Q, N)) < 0.4
+    if Q > 5:
+        allowed[5] = False
+        allowed[4] = True
+    mask = torch.from_numpy(allowed).to(device)
+    low = torch.zeros(Q, N, device=device).masked_fill(~mask, torch.finfo(torch.float32).min)
+    for m in (mask, low, low.to(dtype if dtype != torch.float32 else torch.bfloat16)):
+        got = kernels.prompt_attention(q, k, v, N, D ** -0.5, mask=m)
+        for h in range(H):
+            check(got[0, h], q[0, h], k[h // 2], v[h // 2], allowed, D ** -0.5)
+        if Q > 5:
+            assert (got[0, :, 5] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
