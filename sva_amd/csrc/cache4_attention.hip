@@ -22,9 +22,9 @@
 //    may not see it) and marks the query rows that may.
 // Workgroups split the keys (partials joined by a second kernel), a
 // workgroup's four waves take its 32-key tiles in turn, two tiles ahead in
-// registers.  What bounds it: one token over 1M keys, 9 x 64, 46.5 us of this
-// kernel, 4.6 TB/s (a large copy moves 4.9), the vector units half busy; 24
-// sequences, 32 x 128, 147 us, 3.8 TB/s, sequences of different lengths.
+// registers.  What bounds it: one token over 1M keys, 9 x 64, 48 us of this
+// kernel, 4.4 TB/s (a large copy moves 4.9), the vector units half busy; 24
+// sequences, 32 x 128, 150 us, 3.7 TB/s, sequences of different lengths.
 #include <algorithm>
 
 #include "cache4.h"

@@ -4,8 +4,8 @@
 // the keys row r may see, in one pass over the keys with a running reference
 // m.  The query rows of a KV head are (token, head of its group) pairs,
 // token-major, so one K / V tile serves every head of the group.  Four waves
-// of 32 query rows each share tiles of BN keys in LDS (two buffers: the
-// next tile is loaded into registers while this one is used).
+// of 32 query rows each share tiles of BN keys in LDS (two buffers of K and
+// of V: the next tiles arrive, straight from memory, while these are used).
 //  * S^T = K Q^T (rows: keys) leaves each lane with half of the tile's scores
 //    of one query row, and exactly the elements of P^T that the second
 //    product O^T = V^T P^T wants from it: weights stay in registers, a row's
@@ -26,7 +26,7 @@
 //    term, its rest after rounding: the outputs keep about 16 bits of the
 //    weights (bf16 difference from fp32 attention 2.5e-3 -> 6e-5).  Two waves
 //    take a tile's 32-key halves, joined in LDS.  32 sequences of up to 131072
-//    keys, 9 x 64: 293 us (one wave, one term 289); 24 of up to 42K, 32 x 128:
+//    keys, 9 x 64: 302 us, as one wave with one term; 24 of up to 42K, 32 x 128:
 //    384 (417).
 //  * Three tiles are in work at once: while tile t is weighed on the vector
 //    units, tile t + 1's scores and tile t - 1's sums are on the matrix units.

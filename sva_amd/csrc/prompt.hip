@@ -16,7 +16,8 @@ int64_t row_tiles(int64_t H, int64_t G, int64_t Q) { return (H / G * Q + BM - 1)
 // of whole prompts are of every length, and dispatch evens them out: they are
 // split only where they do not fill the card once.  Tokens over a cache that
 // is much longer make row tiles of one length: about five workgroups for each
-// of the two places of a CU, so that a last round of them is a small part;
+// of the two places of a CU (head_dim above 128, and fp32 above 64, have one
+// place, and so ten workgroups for it), so that a last round of them is a small part;
 // fewer where there are many rows, whose sums go through memory once for each
 // range.  (9 x 64 bf16: 8192 whole tokens 120 us in one range, 145 with a
 // second behind key 4736; 512 tokens each over 8 x 32768 keys 530 us in two

@@ -782,8 +782,8 @@ def stream_read(buf: torch.Tensor, sink: torch.Tensor | None = None) -> torch.Te
 
 def cache4_alloc(kv_heads: int, rows: int, head_dim: int, device) -> tuple[torch.Tensor, torch.Tensor]:
     """An empty 4-bit KV cache of one layer: data uint8 [G, rows, 2, D / 2] and
-    scales uint8 [G, rows, 2, D / 32], a row's K before its V (17 bits for 32
-    elements' 512 in bf16: K and V of a row take D + D / 16 bytes)."""
+    scales uint8 [G, rows, 2, D / 32], a row's K before its V (136 bits for 32
+    elements, 512 in bf16: K and V of a row take D + D / 16 bytes)."""
 
     if kv_heads < 1 or rows < 1 or head_dim < 1 or head_dim > 256 or head_dim % 32 != 0:
         raise ValueError(f"a 4-bit cache takes head_dim a multiple of 32 up to 256, got {kv_heads} x {rows} rows of "
