@@ -38,7 +38,6 @@ namespace {
 constexpr int AW = 4;       // waves per workgroup
 constexpr int TK = 32;      // keys per tile
 constexpr int TR = 16;      // query rows per workgroup
-constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Attend4Params {
   const void* q;
@@ -114,9 +113,8 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
   }
   const int lim = live ? min(k1 - 1, len - p.Q + tok) : -1;     // the last key this query row may see here
   const int full = min(k1, len - p.Q + rt * TR / grp + 1);      // keys below are seen by every row
-  // (a scale of 0: the smallest normal one gives the same weights, and -inf times it stays -inf)
-  const float sl = fmaxf(fabsf(p.scaling) * kLog2e, 1.17549435e-38f);
-  float top = -3.40282347e38f, z = 0.0f;  // the largest score that the reference m = top * sl + above stands for
+  const float sl = score_scale(p.scaling);
+  float top = -3.40282347e38f, z = 0.0f;  // weights are 2^((score - top) sl - above)
   float above = 0.0f, most_sum = kMost;
   uint32_t nan_blocks = 0u;
   f32x4 o[2 * NB];
@@ -204,12 +202,12 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int b = 0; b < SB; ++b) large = large || (x.vs[t][b] >= kLarge && x.vs[t][b] != 0x7F800000u);
+        for (int n = 0; n < SB; ++n) large = large || (x.vs[t][n] >= kLarge && x.vs[t][n] != 0x7F800000u);
       if (above == 0.0f && __any(large)) {
-        above = 60.0f, most_sum = kMost * 0x1p-60f;
-        z *= 0x1p-60f;
+        above = 60.0f, most_sum = kMost * kShifted;
+        z *= kShifted;
 #pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) o[i] *= 0x1p-60f;
+        for (int i = 0; i < 2 * NB; ++i) o[i] *= kShifted;
       }
       // which NaN blocks may this query row see?
       for (int i = 0; i < 8; ++i) {
@@ -283,15 +281,14 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
       if (base + 3 * STEP < k1) fetch(base + 3 * STEP, c);
     }
   }
-  // the waves' parts: [wave][query row][m, z, NaN blocks, sums]
+  // the waves' parts: [wave][query row][m, z (join.h), NaN blocks, sums]
   z += __shfl_xor(z, 16, WAVE);
   z += __shfl_xor(z, 32, WAVE);
   nan_blocks |= (uint32_t)__shfl_xor((int)nan_blocks, 16, WAVE);
   nan_blocks |= (uint32_t)__shfl_xor((int)nan_blocks, 32, WAVE);
   __syncthreads();
   float* mine = (float*)lds + (w * TR + m16) * PS;
-  const float mref = fminf(fmaxf(top * sl, -3.40282347e38f), 3.40282347e38f) + above;
-  if (qd == 0) mine[0] = mref, mine[1] = z, mine[2] = __uint_as_float(nan_blocks);
+  if (qd == 0) mine[0] = top, mine[1] = above == 0.0f ? z : -z, mine[2] = __uint_as_float(nan_blocks);
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) {
 #pragma unroll
@@ -306,15 +303,19 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
     const float* f = (const float*)lds + row * PS;
     float M = f[0], Z = 0.0f, a = 0.0f;
     uint32_t nb = 0u;
+    bool shifted = false;
 #pragma unroll
     for (int v = 0; v < AW; ++v) {
       M = fmaxf(M, f[v * TR * PS]);
+      shifted = shifted || f[v * TR * PS + 1] < 0.0f;
       nb |= __float_as_uint(f[v * TR * PS + 2]);
     }
 #pragma unroll
     for (int v = 0; v < AW; ++v) {
-      const float c = __builtin_amdgcn_exp2f(f[v * TR * PS] - M);
-      Z += f[v * TR * PS + 1] * c;
+      const float zv = f[v * TR * PS + 1];
+      float c = __builtin_amdgcn_exp2f((f[v * TR * PS] - M) * sl);
+      if (shifted && !(zv < 0.0f)) c *= kShifted;
+      Z += fabsf(zv) * c;
       a += f[v * TR * PS + 3 + d] * c;
     }
     if (nb >> (d / kCache4Block) & 1u) a = NAN;
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(AW * WAVE, NB <= 2 ? 4 : (NB == 4 ? 3 : 1)) ca
     } else {
       const int64_t at = (((int64_t)b * p.H + h) * p.Q + t) * p.splits + split;
       p.sums[at * p.D + d] = a;
-      if (d == 0) p.stats[2 * at] = M, p.stats[2 * at + 1] = Z;
+      if (d == 0) p.stats[2 * at] = M, p.stats[2 * at + 1] = shifted ? -Z : Z;
     }
   }
 }
@@ -429,6 +430,7 @@ extern "C" int sva_cache4_attention(const void* q, int q_dtype, int64_t q_seq_st
   JoinParams j;
   j.sums = p.sums;
   j.stats = p.stats;
+  j.sl = score_scale(scaling);
   j.splits = p.splits;
   j.H = p.H;
   j.G = p.G;

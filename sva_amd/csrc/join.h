@@ -1,6 +1,9 @@
 // Joining the key ranges of split attention: each workgroup of a split call
-// leaves, per query item and range, the maximum m of its scores (in base 2),
-// the sum z of 2^(score - m) and the weighted sums of V, in fp32.
+// leaves, per query item and range, a reference m that its scores q . K do not
+// pass by much, the sum z of the weights 2^((score - m) sl) and the weighted
+// sums of V, in fp32.  References are kept before the scale: differences of
+// close scores are then exact, whatever their size.  A z below 0 says that its
+// weights and sums were taken 2^-60 times (V near the largest number).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -10,6 +13,7 @@ namespace sva {
 struct JoinParams {
   const float* sums;   // [n_seq * H * Q, splits, D]
   const float* stats;  // [n_seq * H * Q, splits, 2]: m, z; a range in which the item sees no key: z and sums of 0
+  float sl;            // score_scale(scaling)
   int splits, H, G, Q, D;
   const int64_t* q_lens;     // packed tokens: sequence b's are rows q_offsets[b] + t, t < q_lens[b], of q_rows;
   const int64_t* q_offsets;  // NULL: Q tokens of every sequence
@@ -32,6 +36,16 @@ inline size_t join_bytes(int64_t items, int64_t splits, int64_t D) {
 inline int64_t join_stats_floats(int64_t items, int64_t splits) { return (items * splits * 2 + 3) / 4 * 4; }
 
 int launch_join(const JoinParams& p, int64_t n_seq, hipStream_t stream);
+
+constexpr float kShifted = 0x1p-60f;
+
+// What turns a score q . K (of -q, where the scale is below 0) into a base-2
+// exponent.  (A scale of 0: the smallest normal number gives the same weights,
+// and -inf times it stays -inf.)
+__host__ __device__ inline float score_scale(float scaling) {
+  const float sl = (scaling < 0.0f ? -scaling : scaling) * 1.44269504088896340736f;
+  return sl > 1.17549435e-38f ? sl : (sl <= 1.17549435e-38f ? 1.17549435e-38f : sl);
+}
 
 // Tokens of packed sequence b and the row of its first, inside [0, q_rows).
 __device__ inline int seq_tokens(const int64_t* q_lens, const int64_t* q_offsets, int64_t q_rows, int Q, int b,

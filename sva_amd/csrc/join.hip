@@ -36,29 +36,37 @@ SVA_DEV JoinItem join_item(const JoinParams& p, int item) {
   return x;
 }
 
-// A range's share of the joined sums: 2^(m - M).  A share of 0 still counts:
-// sums that are not finite stay so, as in one range.  (A range without a key
-// has sums of 0; one done again whose scores are all NaN has m = -inf and z
-// NaN.)
-SVA_DEV float join_share(float m, float M) { return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M); }
+// A range's share of the joined sums: 2^((m - M) sl).  A share of 0 still
+// counts: sums that are not finite stay so, as in one range.  (A range without
+// a key has sums of 0; one done again whose scores are all NaN has m = -inf
+// and z NaN.)
+SVA_DEV float join_share(float m, float M, float sl) {
+  return m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * sl);
+}
 
 // Few items of many ranges (decode): a workgroup takes 32 elements of one
 // item, 16 ranges at a time, eight rounds of loads in flight: 256 ranges are
 // two round trips.
 __global__ void __launch_bounds__(JB) join_kernel(JoinParams p) {
   __shared__ float red[2][JB];
-  __shared__ float top[JB / WAVE];
+  __shared__ float2 top[JB / WAVE];
   const JoinItem x = join_item(p, (int)blockIdx.x);
   const int d = (int)blockIdx.y * 32 + (int)threadIdx.x % 32, part = (int)threadIdx.x / 32;
   if (x.ranges == 1) return;
   constexpr int U = 8, PARTS = JB / 32;
   float M = -INFINITY;
-  for (int s = (int)threadIdx.x; s < x.ranges; s += JB) M = fmaxf(M, x.stats[2 * s]);
+  bool shifted = false;
+  for (int s = (int)threadIdx.x; s < x.ranges; s += JB) {
+    const float2 st = *(const float2*)(x.stats + 2 * s);
+    M = fmaxf(M, st.x);
+    shifted = shifted || st.y < 0.0f;
+  }
   M = wave_max(M);
-  if (lane_id() == 0) top[threadIdx.x / WAVE] = M;
+  float down = __any(shifted) ? kShifted : 1.0f;  // of ranges that are not
+  if (lane_id() == 0) top[threadIdx.x / WAVE] = make_float2(M, down);
   __syncthreads();
 #pragma unroll
-  for (int v = 0; v < JB / WAVE; ++v) M = fmaxf(M, top[v]);
+  for (int v = 0; v < JB / WAVE; ++v) M = fmaxf(M, top[v].x), down = fminf(down, top[v].y);
   float Z = 0.0f, a = 0.0f;
   for (int s0 = part; s0 < x.ranges; s0 += U * PARTS) {
     float2 st[U];
@@ -76,8 +84,8 @@ __global__ void __launch_bounds__(JB) join_kernel(JoinParams p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (s0 + u * PARTS >= x.ranges) continue;
-      const float c = join_share(st[u].x, M);
-      Z += st[u].y * c;
+      const float c = join_share(st[u].x, M, p.sl) * (st[u].y < 0.0f ? 1.0f : down);
+      Z += fabsf(st[u].y) * c;
       a += sm[u] * c;
     }
   }
@@ -106,6 +114,7 @@ __global__ void __launch_bounds__(RB) join_rows_kernel(JoinParams p, int items) 
   constexpr int U = 8;
   for (int d = lane_id(); d < p.D; d += WAVE) {
     float M = -INFINITY, Z = 0.0f, a = 0.0f;
+    bool shifted = false;
     for (int s0 = 0; s0 < x.ranges; s0 += U) {
       float2 st[U];
       float sm[U];
@@ -119,15 +128,18 @@ __global__ void __launch_bounds__(RB) join_rows_kernel(JoinParams p, int items) 
         }
       }
       float top = M;
+      bool now = shifted;
 #pragma unroll
-      for (int u = 0; u < U; ++u) top = fmaxf(top, st[u].x);
-      const float c = join_share(M, top);
+      for (int u = 0; u < U; ++u) top = fmaxf(top, st[u].x), now = now || st[u].y < 0.0f;
+      float c = join_share(M, top, p.sl);
+      if (now && !shifted) c *= kShifted, shifted = true;
       Z *= c, a *= c, M = top;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (s0 + u >= x.ranges) continue;
-        const float f = join_share(st[u].x, M);
-        Z += st[u].y * f;
+        float f = join_share(st[u].x, M, p.sl);
+        if (shifted && !(st[u].y < 0.0f)) f *= kShifted;
+        Z += fabsf(st[u].y) * f;
         a += sm[u] * f;
       }
     }

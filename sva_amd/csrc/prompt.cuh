@@ -155,7 +155,6 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   constexpr int BM = 4 * 32;             // query rows of a workgroup
   constexpr int TB = BN * DP * ES;       // bytes of a K or V tile
   constexpr int NO = DP / 32;            // 32-element blocks of the sums
-  constexpr float kLog2e = 1.44269504088896340736f;
   constexpr float kMost = DT == F16 ? 32768.0f : 65536.0f;  // a lane's weights of a tile may sum to
   constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;         // how far below the maximum a new reference lies
   constexpr float kNoKey = -3.40282347e38f;                 // the reference of a row that has seen no key
@@ -244,11 +243,10 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
       if (p.scaling < 0.0f) bq[f] = -bq[f];
     }
   }
-  // (a scale of 0: the smallest normal one gives the same weights, and -inf times it stays -inf)
-  const float sl = fmaxf(fabsf(p.scaling) * kLog2e, 1.17549435e-38f);
+  const float sl = score_scale(p.scaling);
 
   f32x16 o[NO];
-  float mref = kNoKey, z = 0.0f;
+  float top = kNoKey, mref = kNoKey, z = 0.0f;  // the reference before the scale and after it
 #pragma unroll
   for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -389,14 +387,13 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   // its maximum
   auto settle = [&](float zs, const f32x16 (&s)[KT], weights (&pw)[KT]) {
     if (__any(zs > kMost)) {
-      float top = s[0][0];
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int k = 0; k < 16; ++k) top = fmaxf(top, s[kt][k]);
       const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * sl;
-      const float mn = fmaxf(mref, top - kBelow);
+      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      const float mn = fmaxf(mref, top * sl - kBelow);
       const float corr = __builtin_amdgcn_exp2f(mref - mn);
       mref = mn;
       z *= corr;
@@ -495,6 +492,9 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(z), __float_as_uint(z), false, false);
     z = __uint_as_float(x[0]) + __uint_as_float(x[1]);
   }
+  const bool far = top != kNoKey && fabsf(mref) > kFar;
+  // what brings weights relative to m, rounded, to `top`, which is not
+  float even = top == kNoKey ? 1.0f : __builtin_amdgcn_exp2f(-__builtin_fmaf(top, sl, -mref));
   if constexpr (FEW) {  // both terms, then both waves: wave 0 goes on with all of it
     z += __shfl_xor(z, kFewRows, WAVE);
 #pragma unroll
@@ -504,17 +504,18 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
     float* part = (float*)lds + lane;  // [m, z, sums][lane], in the tiles' place
     __syncthreads();
     if (w == 1) {
-      part[0] = mref, part[WAVE] = z;
+      part[0] = top, part[WAVE] = far ? NAN : z * even;
 #pragma unroll
       for (int i = 0; i < NO; ++i)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) part[(2 + 16 * i + k) * WAVE] = o[i][k];
+        for (int k = 0; k < 16; ++k) part[(2 + 16 * i + k) * WAVE] = far ? NAN : o[i][k] * even;
     }
     __syncthreads();
     if (w != 0) return;
-    const float m1 = part[0], mn = fmaxf(mref, m1);
-    const float f0 = __builtin_amdgcn_exp2f(mref - mn), f1 = __builtin_amdgcn_exp2f(m1 - mn);
-    mref = mn;
+    const float m1 = part[0], mn = fmaxf(top, m1);
+    const float f0 = __builtin_amdgcn_exp2f((top - mn) * sl) * even, f1 = __builtin_amdgcn_exp2f((m1 - mn) * sl);
+    top = mn;
+    even = 1.0f;
     z = z * f0 + part[WAVE] * f1;
 #pragma unroll
     for (int i = 0; i < NO; ++i)
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   }
   const float most = partial ? kLarge : 3.40282347e38f;
   // (fma(s, sl, -m) is exact before its rounding, m is not: it is off by up to 2 at 2^26, by 128 at 2^31)
-  bool odd = mref != kNoKey && fabsf(mref) > kFar;
+  bool odd = far;
 #pragma unroll
   for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -556,11 +557,11 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
             const int64_t ka = kvb + (int64_t)key * p.kv_rs;
             for (int d = 0; d < p.D; ++d)
               sc = __builtin_fmaf(load_elem(p.q, qa + d, DT), load_elem(p.keys, ka + d, DT), sc);
-            sc *= p.scaling * kLog2e;
+            sc = p.scaling < 0.0f ? -sc : sc;
           }
           const float mn = fmaxf(m, wave_max(sc));
-          const float corr = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-          const float e = ok ? __builtin_amdgcn_exp2f(sc - (mn == -INFINITY ? 0.0f : mn)) * down : 0.0f;
+          const float corr = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sl);
+          const float e = ok ? __builtin_amdgcn_exp2f((sc - (mn == -INFINITY ? 0.0f : mn)) * sl) * down : 0.0f;
           m = mn;
           zz = zz * corr + wave_sum(e);
 #pragma unroll
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
 #pragma unroll
         for (int k = 0; k < DP / 64; ++k) large = large || (finite[k] && zz == zz && !(fabsf(acc[k]) <= kLarge));
         if (down != 1.0f || !__any(large)) break;
-        down = 0x1p-60f;
+        down = kShifted;
       }
 #pragma unroll
       for (int k = 0; k < DP / 64; ++k) {
@@ -596,7 +597,7 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
         else
           store_elem(p.out, q_at(r, p.o_bs, p.o_hs, p.o_ts) + d, p.out_dtype, zz == 0.0f ? 0.0f : acc[k] / zz);
       }
-      if (partial && lane == 0) p.stats[2 * part_at(r)] = down == 1.0f ? m : m + 60.0f, p.stats[2 * part_at(r) + 1] = zz;
+      if (partial && lane == 0) p.stats[2 * part_at(r)] = m, p.stats[2 * part_at(r) + 1] = down == 1.0f ? zz : -zz;
     }
     return;
   }
@@ -605,8 +606,8 @@ __global__ void __launch_bounds__(256, PromptType<DT>::waves(DP)) prompt_kernel(
   void* dst = partial ? (void*)p.sums : p.out;
   const int type = partial ? (int)F32 : p.out_dtype;
   const int64_t at = partial ? part_at(row) * p.D : q_at(row, p.o_bs, p.o_hs, p.o_ts);
-  const float f = partial ? 1.0f : (z == 0.0f ? 0.0f : 1.0f / z);
-  if (partial && hf == 0) p.stats[2 * part_at(row)] = mref, p.stats[2 * part_at(row) + 1] = z;
+  const float f = partial ? even : (z == 0.0f ? 0.0f : 1.0f / z);
+  if (partial && hf == 0) p.stats[2 * part_at(row)] = top, p.stats[2 * part_at(row) + 1] = z * even;
   const bool whole = partial ? p.D % 4 == 0 : p.out_vec;
 #pragma unroll
   for (int i = 0; i < NO; ++i)

@@ -132,6 +132,7 @@ extern "C" int sva_prompt_attention(const void* q, int dtype, int64_t q_seq_stri
   JoinParams j;
   j.sums = p.sums;
   j.stats = p.stats;
+  j.sl = score_scale(scaling);
   j.splits = p.splits;
   j.H = p.H;
   j.G = p.G;

@@ -41,3 +41,32 @@ def test_large_scores(device, Q, n, score, dtype):
         for t in range(Q):
             want = back[0, 0, :n - Q + 1 + t].double().mean(0)
             assert (got[0, :, t].double() - want).abs().max() <= 6.0 * ((n + 16) * 2.0 ** -23 + WEIGHTS), t
+
+
+@pytest.mark.parametrize("times,apart", [(0.0, 0.75), (1.25, 0.75), (1.375, 0.75), (-1.625, 0.75), (3.5, 0.75), (2048.0, 4.0), (-2048.0, 4.0)])
+@pytest.mark.parametrize("Q,n,far", [(2, 3000, 1024), (70, 3000, 1024), (2, 200, 100)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_close_scores_of_any_size_keep_their_distance(device, Q, n, far, times, apart, sign):
+    """Two kinds of keys whose scores of 24576 `times` lie `apart` (the last bit of 5e7 is 4), each kind in ranges of
+    its own, V 1 and 0: the output is the first kind's share of the weights, as of scores near 0.  Scores, their
+    difference and V are exact."""
+    from sva_amd import kernels
+
+    q = torch.zeros(1, 2, Q, D, device=device)
+    q[..., 0], q[..., 32] = sign * times, sign * apart / 4
+    k = torch.zeros(1, n, D, device=device)
+    k[..., 0] = 24576.0  # (values of the 4-bit format, in blocks of their own)
+    k[:, :far, 32] = 4.0
+    v = torch.zeros(1, n, D, device=device)
+    v[:, :far] = 1.0
+    data, scales = kernels.cache4_alloc(1, n, D, device)
+    kernels.cache4_write(k, v, data, scales, 0)
+    back = kernels.cache4_read(data, scales, 0, n, torch.float32)
+    assert torch.equal(back[0][0], k) and torch.equal(back[1][0], v)
+    got = [kernels.prompt_attention(q, k, v, n, sign), kernels.cache4_attention(q, data, scales, n, sign)]
+    seen = (n - Q + 1 + torch.arange(Q, device=device, dtype=torch.float64))[:, None]
+    weight = torch.tensor(apart, device=device, dtype=torch.float64).exp()
+    want = far * weight / (far * weight + seen - far)
+    for x in got:
+        # sums of n weights, two exponentials and a quotient, and (4 bits) weights of two terms
+        assert (x[0].double() - want).abs().max() <= (n + 16) * 2.0 ** -24 + WEIGHTS
