@@ -246,7 +246,7 @@ def _plain_reserve(tables, lens, refs, counts, P):
     shared = fits & (counts > 0) & (lens % P != 0) & (last >= 0) & (refs[last.clamp_min(0).long()] > 1)
     need = torch.where(fits, _pages_of(new_lens, P) - old + shared.long(), 0)
     upto = need.cumsum(0)
-    granted = fits & (upto <= (refs == 0).sum())
+    granted = fits & ((need == 0) | (upto <= (refs == 0).sum()))
     free = torch.argsort((refs != 0).int(), stable=True).int()
     begin = old - shared.long()
     taken = granted[:, None] & (at >= begin[:, None]) & (at < (begin + need)[:, None])
