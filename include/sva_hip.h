@@ -624,6 +624,136 @@ int sva_prompt_attention(const void *q, int dtype, int64_t q_seq_stride, int64_t
                          int64_t out_seq_stride, int64_t out_head_stride, int64_t out_tok_stride, void *workspace,
                          size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * A KV cache in pages, for sequences that grow, part and end.  No counterpart
+ * in the reference, whose caches are the model's.
+ *   pool     [n_pages, 2, G, P, D] of one layer, 16-byte aligned: a page holds
+ *            K, then V, of P rows of every KV head, contiguous; page_stride
+ *            elements (a multiple of 16 bytes) between pages.  P (page_rows)
+ *            is a power of two from 16 to 1024, D a multiple of 8 up to 256.
+ *   tables   [n_seq, max_pages] int32, table_stride entries between rows: row n
+ *            of sequence b lies in page tables[b][n / P], row n % P.  An entry
+ *            outside [0, n_pages) names no page: its rows are not there.
+ *   seq_lens [n_seq] int64: rows in use
+ *   refs     [n_pages] int32: the number of table entries within the lengths
+ *            that name a page; 0: it is free
+ * All of them live on the device.
+ */
+
+/*
+ * Writes rows of K and V: token t of sequence b goes to row first_rows[b] + t
+ * ([n_seq] int64 on the device); rows without a page, and below 0, are
+ * skipped.  No two of a call's tokens may name one row.
+ *   keys / values  (b, g, t, d) at b*kv_seq_stride + g*kv_head_stride +
+ *                  t*kv_row_stride + d, of the pool's dtype
+ */
+int sva_paged_write(const void *keys, const void *values, int kv_dtype, int64_t kv_seq_stride, int64_t kv_head_stride,
+                    int64_t kv_row_stride, int64_t n_seq, int64_t n_rows, int64_t G, int64_t D,
+                    const int64_t *first_rows, void *pool, int64_t n_pages, int64_t page_stride, int64_t page_rows,
+                    const int32_t *tables, int64_t table_stride, int64_t max_pages, void *stream);
+
+/*
+ * Rows first_rows[b] + t, laid out as sva_paged_write takes them (16-byte
+ * aligned rows); rows without a page read as 0.
+ */
+int sva_paged_read(const void *pool, int64_t n_pages, int64_t page_stride, int64_t page_rows, const int32_t *tables,
+                   int64_t table_stride, int64_t max_pages, const int64_t *first_rows, int64_t n_seq, int64_t n_rows,
+                   int64_t G, int64_t D, void *keys, void *values, int kv_dtype, int64_t kv_seq_stride,
+                   int64_t kv_head_stride, int64_t kv_row_stride, void *stream);
+
+/*
+ * Attention of the last Q tokens of every sequence over its rows: token t sees
+ * row n iff n <= seq_lens[b] - Q + t and the row has a page; a token that sees
+ * none gives 0.  n_keys is at least every length; the part of a sequence behind
+ * it, or behind max_pages pages, is not read.  What an unseen row holds, NaN
+ * and infinities included, reaches no output.
+ *   q        of the pool's dtype, (b, h, t, d) at b*q_seq_stride +
+ *            h*q_head_stride + t*q_tok_stride + d
+ *   out      (b, h, t, d) at b*out_seq_stride + h*out_head_stride +
+ *            t*out_tok_stride + d
+ * workspace: sva_paged_attention_workspace_bytes(...) bytes at n_keys, or at
+ * max_pages * page_rows where that is less (no state between calls).
+ */
+size_t sva_paged_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D, int64_t n_keys);
+int sva_paged_attention(const void *q, int dtype, int64_t q_seq_stride, int64_t q_head_stride, int64_t q_tok_stride,
+                        const void *pool, int64_t n_pages, int64_t page_stride, int64_t page_rows,
+                        const int32_t *tables, int64_t table_stride, int64_t max_pages, const int64_t *seq_lens,
+                        int64_t n_keys, int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D, float scaling,
+                        void *out, int out_dtype, int64_t out_seq_stride, int64_t out_head_stride,
+                        int64_t out_tok_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Room for counts[s] more rows behind every sequence (counts [n_seq] int64 on
+ * the device, or NULL: `count` each).  New pages are the lowest free ones, in
+ * the order of the sequences; seq_lens, tables and refs are brought up to
+ * date.  Where rows are to go into a last page that others hold too, the
+ * sequence leaves it to them for a new one, and (src[s], dst[s]) says which
+ * page is to be copied into which (-1: none): sva_pages_copy, before the next
+ * call that hands out pages.
+ *   first_rows [n_seq] int64: the first of the new rows (the length before);
+ *              -1: nothing was changed for this sequence, whose pages together
+ *              with those asked for by the ones before it are not there, whose
+ *              table is too short, or whose count is negative
+ */
+size_t sva_pages_reserve_workspace_bytes(int64_t n_seq, int64_t n_pages);
+int sva_pages_reserve(int32_t *tables, int64_t table_stride, int64_t max_pages, int64_t *seq_lens, int64_t n_seq,
+                      int32_t *refs, int64_t n_pages, int64_t page_rows, const int64_t *counts, int64_t count,
+                      int64_t *first_rows, int32_t *src, int32_t *dst, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+/*
+ * Row s of the tables becomes a fork of row sources[s] ([n_seq] int64 on the
+ * device), as that was before the call: the same pages and length.  sources[s]
+ * = -1 frees the sequence (length 0); s itself, or any other number, leaves it.
+ * Pages that no sequence names any more are free.
+ */
+size_t sva_pages_fork_workspace_bytes(int64_t n_seq, int64_t max_pages);
+int sva_pages_fork(int32_t *tables, int64_t table_stride, int64_t max_pages, int64_t *seq_lens, int64_t n_seq,
+                   int32_t *refs, int64_t n_pages, int64_t page_rows, const int64_t *sources, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/*
+ * The pages in use moved together: with `used` [1] of them, the k-th page in
+ * use from `used` on goes to the k-th free one below.  tables and refs are
+ * renumbered; (src[k], dst[k]) [n_pages / 2] are the pages to copy
+ * (sva_pages_copy; -1 behind the last).  Every holder of pages has to be in
+ * the tables.
+ */
+size_t sva_pages_compact_workspace_bytes(int64_t n_pages);
+int sva_pages_compact(int32_t *tables, int64_t table_stride, int64_t max_pages, int64_t n_seq, int32_t *refs,
+                      int64_t n_pages, int32_t *src, int32_t *dst, int32_t *used, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/*
+ * Page src[i] copied into page dst[i], in every layer.  Pairs with a number
+ * outside [0, n_pages) are skipped.  A page must be in one pair alone, unless
+ * as the source of several.
+ *   page i of layer l at l*layer_stride_bytes + i*page_stride_bytes, page_bytes
+ *   of it; all multiples of 16
+ */
+int sva_pages_copy(void *pool, int64_t n_pages, int64_t page_stride_bytes, int64_t layers, int64_t layer_stride_bytes,
+                   int64_t page_bytes, const int32_t *src, const int32_t *dst, int64_t n_pairs, void *stream);
+
+/*
+ * The next token of every row of logits from a given random number: weights
+ * exp((x - largest) / temperature); of the tokens in the order of falling
+ * logits (ties: the lower token first) the first top_k (0 or less: all), of
+ * these the ones with less than top_p of their sum before them (1 and more:
+ * all; at least one), of these the ones of at least min_p of the largest
+ * weight; then the first, by number, up to which the kept weights sum to more
+ * than uniforms[row] of their sum.  temperature <= 0: the largest logit.  A NaN
+ * counts as -inf; a row without any other number gives -1.  Weights are taken
+ * in 64 bits.  No counterpart in the reference (its models generate by
+ * themselves).
+ *   logits  row r at r*row_stride elements, `vocab` (at most 2^20) of them
+ *   temperature, top_k, top_p, min_p  [n_rows] on the device, or NULL: the
+ *   scalar behind it for every row
+ */
+int sva_sample_tokens(const void *logits, int dtype, int64_t row_stride, int64_t n_rows, int64_t vocab,
+                      const float *uniforms, const float *temperature, float temperature1, const int64_t *top_k,
+                      int64_t top_k1, const float *top_p, float top_p1, const float *min_p, float min_p1,
+                      int64_t *tokens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -92,6 +92,21 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
     "sva_cache4_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "sva_cache4_attention": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64,
                                   _F, _P, _I, _I64, _I64, _I64, _P, _SZ, _P]),
+    "sva_paged_write": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64,
+                             _I64, _P]),
+    "sva_paged_read": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I, _I64, _I64,
+                            _I64, _P]),
+    "sva_paged_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "sva_paged_attention": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64,
+                                 _I64, _I64, _I64, _F, _P, _I, _I64, _I64, _I64, _P, _SZ, _P]),
+    "sva_pages_reserve_workspace_bytes": (_SZ, [_I64, _I64]),
+    "sva_pages_reserve": (_I, [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "sva_pages_fork_workspace_bytes": (_SZ, [_I64, _I64]),
+    "sva_pages_fork": (_I, [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P, _SZ, _P]),
+    "sva_pages_compact_workspace_bytes": (_SZ, [_I64]),
+    "sva_pages_compact": (_I, [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "sva_pages_copy": (_I, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "sva_sample_tokens": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _F, _P, _I64, _P, _F, _P, _F, _P, _P]),
 }
 
 

@@ -1102,3 +1102,308 @@ def prompt_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, 
           heads, kv_heads, q_len, dim, float(scaling), ptr(m), mtype, mseq, mtok, out.data_ptr(), dtype_code(out),
           *o4.stride()[:3], ws.data_ptr(), ws.numel())
     return out
+
+
+# ---------------------------------------------------------------------------
+# a KV cache in pages
+
+
+def pages_alloc(n_pages: int, kv_heads: int, page_rows: int, head_dim: int, device,
+                dtype: torch.dtype = torch.bfloat16, layers: int | None = None) -> torch.Tensor:
+    """A pool of pages [n_pages, 2, G, P, D], or [layers, n_pages, 2, G, P, D]:
+    K, then V, of P rows of every KV head a page.  The rows are undefined."""
+
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {dtype}; expected float32, bfloat16 or float16")
+    shape = (n_pages, 2, kv_heads, page_rows, head_dim)
+    if min(shape) < 1 or (layers is not None and layers < 1):
+        raise ValueError(f"a pool of {n_pages} pages of {kv_heads} x {page_rows} rows of {head_dim}")
+    _check_page_shape(page_rows, head_dim)
+    return torch.empty(shape if layers is None else (layers, *shape), device=device, dtype=dtype)
+
+
+def _check_page_shape(page_rows: int, dim: int) -> None:
+    if page_rows < 16 or page_rows > 1024 or page_rows & (page_rows - 1) or dim < 1 or dim > 256 or dim % 8:
+        raise ValueError(f"pages take a power of two of 16 to 1024 rows and head_dim a multiple of 8 up to 256, got "
+                         f"{page_rows} rows of {dim}")
+
+
+def _check_pool(pool: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """(pages, G, P, D, elements between pages) of one layer's pool."""
+
+    if pool.dim() != 5 or pool.shape[1] != 2:
+        raise ValueError(f"a pool must be [pages, 2, G, P, D], got {tuple(pool.shape)}")
+    n, _, kv_heads, rows, dim = pool.shape
+    stride = pool.stride()
+    if stride[4] != 1 or stride[3] != dim or stride[2] != rows * dim or stride[1] != kv_heads * rows * dim or \
+            stride[0] < 2 * kv_heads * rows * dim:
+        raise ValueError(f"every page of a pool must be contiguous, got {tuple(pool.shape)} of strides {stride}")
+    _check_page_shape(rows, dim)
+    return n, kv_heads, rows, dim, stride[0]
+
+
+def _check_tables(tables: torch.Tensor, n_seq: int | None = None) -> tuple[int, int, int]:
+    """(sequences, entries, entries between rows) of page tables."""
+
+    if tables.dim() != 2 or tables.dtype != torch.int32 or (tables.shape[1] > 1 and tables.stride(1) != 1) or \
+            (n_seq is not None and tables.shape[0] != n_seq):
+        raise ValueError(f"tables must be int32 [{'n_seq' if n_seq is None else n_seq}, entries], got {tables.dtype} "
+                         f"{tuple(tables.shape)}")
+    return tables.shape[0], tables.shape[1], tables.stride(0)
+
+
+def paged_write(keys: torch.Tensor, values: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, first_rows) -> None:
+    """Writes keys / values [n_seq, G, T, D] (or [G, T, D]) of the pool's dtype
+    into their pages: token t of sequence b into row first_rows[b] + t (int64
+    [n_seq] on the device, as pages_reserve gives it, or ints).  Rows without a
+    page, and below 0, are skipped; no two tokens may name one row."""
+
+    n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(pool)
+    if keys.dim() == 3:
+        keys, values = keys.unsqueeze(0), values.unsqueeze(0)
+    if keys.dim() != 4 or keys.shape != values.shape or keys.dtype != pool.dtype or values.dtype != pool.dtype or \
+            keys.shape[1] != kv_heads or keys.shape[3] != dim:
+        raise ValueError(f"keys / values must be [n_seq, {kv_heads}, T, {dim}] of {pool.dtype}, got {keys.dtype} "
+                         f"{tuple(keys.shape)} and {values.dtype} {tuple(values.shape)}")
+    n_seq, _, n_rows, _ = keys.shape
+    _, entries, table_stride = _check_tables(tables, n_seq)
+    _inference_only("paged_write", keys, values, pool)
+    first_rows = _page_first_rows(first_rows, n_seq, pool.device)
+    device = _same_device(keys, values, pool, tables, first_rows)
+    dtype = dtype_code(keys)
+    if n_seq == 0 or n_rows == 0 or n_pages == 0 or entries == 0:
+        return
+    if keys.stride(-1) != 1 or values.stride() != keys.stride():
+        keys, values = keys.contiguous(), values.contiguous()
+    _call(device, "sva_paged_write", keys.data_ptr(), values.data_ptr(), dtype, *keys.stride()[:3], n_seq, n_rows,
+          kv_heads, dim, first_rows.data_ptr(), pool.data_ptr(), n_pages, page_stride, page_rows, tables.data_ptr(),
+          table_stride, entries)
+
+
+def _page_first_rows(first_rows, n_seq: int, device: torch.device) -> torch.Tensor:
+    if not isinstance(first_rows, torch.Tensor):
+        rows = [first_rows] if isinstance(first_rows, int) else list(first_rows)
+        first_rows = torch.tensor(rows, device=device, dtype=torch.int64)
+    return _seq_tensor("first_rows", first_rows, n_seq)
+
+
+def paged_read(pool: torch.Tensor, tables: torch.Tensor, first_rows, n_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows first_rows[b] + t, t < n_rows, of every sequence as keys and values
+    [n_seq, G, n_rows, D]; rows without a page read as 0."""
+
+    n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(pool)
+    n_seq, entries, table_stride = _check_tables(tables)
+    if n_rows < 0:
+        raise ValueError(f"{n_rows} rows")
+    first_rows = _page_first_rows(first_rows, n_seq, pool.device)
+    device = _same_device(pool, tables, first_rows)
+    dtype = dtype_code(pool)
+    keys = torch.empty(n_seq, kv_heads, n_rows, dim, device=device, dtype=pool.dtype)
+    values = torch.empty_like(keys)
+    if keys.numel() == 0:
+        return keys, values
+    if n_pages == 0 or entries == 0:
+        return keys.zero_(), values.zero_()
+    _call(device, "sva_paged_read", pool.data_ptr(), n_pages, page_stride, page_rows, tables.data_ptr(), table_stride,
+          entries, first_rows.data_ptr(), n_seq, n_rows, kv_heads, dim, keys.data_ptr(), values.data_ptr(), dtype,
+          *keys.stride()[:3])
+    return keys, values
+
+
+def paged_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, seq_lens: torch.Tensor, scaling: float,
+                    n_keys: int | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Attention [n_seq, H, Q, D] of the last Q tokens of every sequence over its
+    rows in pages: token t of q [n_seq, H, Q, D] (of the pool's dtype) sees row
+    n iff n <= seq_lens[b] - Q + t and the row has a page (0 where it sees
+    none).  seq_lens int64 [n_seq] on the device; n_keys: at least the longest
+    (rows behind it are not read; default: all that the tables can hold).
+    Inference only: no gradient."""
+
+    n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(pool)
+    q = _as_query(q)
+    n_seq, heads, q_len, head_dim = q.shape
+    _, entries, table_stride = _check_tables(tables, n_seq)
+    if head_dim != dim or q.dtype != pool.dtype or kv_heads == 0 or heads == 0 or heads % kv_heads != 0:
+        raise ValueError(f"query {q.dtype} {tuple(q.shape)} does not fit a pool of {kv_heads} KV heads of {dim} in "
+                         f"{pool.dtype}")
+    seq_lens = _seq_tensor("seq_lens", seq_lens, n_seq)
+    _inference_only("paged_attention", q, pool)
+    device = _same_device(q, pool, tables, seq_lens)
+    dtype = dtype_code(q)
+    # tokens before heads: the model's projection takes the result without a copy
+    out = torch.empty(n_seq, q_len, heads, dim, device=device, dtype=out_dtype or q.dtype).transpose(1, 2)
+    if out.numel() == 0:
+        return out
+    n_keys = entries * page_rows if n_keys is None else min(int(n_keys), entries * page_rows)
+    if n_keys <= 0 or n_pages == 0:
+        return out.zero_()
+    # a buffer of the call's own: calls on other streams and captured graphs never share one
+    ws = torch.empty(lib().sva_paged_attention_workspace_bytes(n_seq, heads, kv_heads, q_len, dim, n_keys),
+                     device=device, dtype=torch.uint8)
+    _call(device, "sva_paged_attention", q.data_ptr(), dtype, *q.stride()[:3], pool.data_ptr(), n_pages, page_stride,
+          page_rows, tables.data_ptr(), table_stride, entries, seq_lens.data_ptr(), n_keys, n_seq, heads, kv_heads,
+          q_len, dim, float(scaling), out.data_ptr(), dtype_code(out), *out.stride()[:3], ws.data_ptr(), ws.numel())
+    return out
+
+
+def _check_holders(tables, seq_lens, refs, page_rows: int):
+    """(sequences, entries, entries between rows, pages) of a pool's bookkeeping."""
+
+    n_seq, entries, table_stride = _check_tables(tables)
+    if n_seq > 1 and table_stride < entries:
+        raise ValueError("rows of the tables overlap")
+    if seq_lens is not None:
+        _seq_tensor("seq_lens", seq_lens, n_seq)
+    if refs.dim() != 1 or refs.dtype != torch.int32 or not refs.is_contiguous():
+        raise ValueError(f"refs must be int32 [pages], got {refs.dtype} {tuple(refs.shape)}")
+    if page_rows < 16 or page_rows > 1024 or page_rows & (page_rows - 1):
+        raise ValueError(f"pages take a power of two of 16 to 1024 rows, got {page_rows}")
+    return n_seq, entries, table_stride, refs.shape[0]
+
+
+def pages_reserve(tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, counts,
+                  page_rows: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Room for counts[b] more rows behind every sequence (int64 [n_seq] on the
+    device, or an int for all): tables, seq_lens and refs are brought up to date
+    in place.  New pages are the lowest free ones (refs 0), in the order of the
+    sequences; a shared last page that rows are to go into is left to the others
+    for a new one.  Returns (first_rows, src, dst): the first new row of every
+    sequence, -1 where nothing was granted (too few pages, too short a table, a
+    negative count) and nothing changed; and the pages to copy, -1 for none
+    (pages_copy(pool, src, dst), before the next call that hands out pages)."""
+
+    n_seq, entries, table_stride, n_pages = _check_holders(tables, seq_lens, refs, page_rows)
+    each = 0
+    if isinstance(counts, torch.Tensor):
+        counts = _seq_tensor("counts", counts, n_seq)
+    else:
+        each, counts = int(counts), None
+    device = _same_device(tables, seq_lens, refs, counts)
+    first_rows = torch.empty(n_seq, device=device, dtype=torch.int64)
+    src = torch.empty(n_seq, device=device, dtype=torch.int32)
+    dst = torch.empty_like(src)
+    if n_seq == 0:
+        return first_rows, src, dst
+    if n_pages == 0 or entries == 0:
+        return first_rows.fill_(-1), src.fill_(-1), dst.fill_(-1)
+    ws = torch.empty(lib().sva_pages_reserve_workspace_bytes(n_seq, n_pages), device=device, dtype=torch.uint8)
+    _call(device, "sva_pages_reserve", tables.data_ptr(), table_stride, entries, seq_lens.data_ptr(), n_seq,
+          refs.data_ptr(), n_pages, page_rows, ptr(counts), each, first_rows.data_ptr(), src.data_ptr(), dst.data_ptr(),
+          ws.data_ptr(), ws.numel())
+    return first_rows, src, dst
+
+
+def pages_fork(tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor, sources: torch.Tensor,
+               page_rows: int) -> None:
+    """Every sequence b becomes a fork of sequence sources[b] (int64 [n_seq] on
+    the device), as that was before the call: it names the same pages, none is
+    copied (pages_reserve parts them where rows are added).  -1 frees the
+    sequence; b itself, or any other number, leaves it as it is.  Pages that no
+    sequence names any more are free.  In place."""
+
+    n_seq, entries, table_stride, n_pages = _check_holders(tables, seq_lens, refs, page_rows)
+    device = _same_device(tables, seq_lens, refs, _seq_tensor("sources", sources, n_seq))
+    if n_seq == 0 or n_pages == 0 or entries == 0:
+        return
+    ws = torch.empty(lib().sva_pages_fork_workspace_bytes(n_seq, entries), device=device, dtype=torch.uint8)
+    _call(device, "sva_pages_fork", tables.data_ptr(), table_stride, entries, seq_lens.data_ptr(), n_seq,
+          refs.data_ptr(), n_pages, page_rows, sources.data_ptr(), ws.data_ptr(), ws.numel())
+
+
+def pages_compact(tables: torch.Tensor, refs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The pages in use moved together: tables and refs are renumbered in place
+    so that they are 0 .. used - 1.  Returns (src, dst, used): the pages to copy,
+    -1 behind the last (pages_copy(pool, src, dst)), and their number int32 [1].
+    Every holder of pages has to be in the tables."""
+
+    n_seq, entries, table_stride, n_pages = _check_holders(tables, None, refs, 16)
+    device = _same_device(tables, refs)
+    src = torch.empty(n_pages // 2, device=device, dtype=torch.int32)
+    dst = torch.empty_like(src)
+    used = torch.empty(1, device=device, dtype=torch.int32)
+    if n_pages == 0:
+        return src, dst, used.zero_()
+    if n_seq == 0 or entries == 0:  # (refs may still say that pages are in use)
+        tables, n_seq, entries, table_stride = torch.full((1, 1), -1, device=device, dtype=torch.int32), 1, 1, 1
+    ws = torch.empty(lib().sva_pages_compact_workspace_bytes(n_pages), device=device, dtype=torch.uint8)
+    _call(device, "sva_pages_compact", tables.data_ptr(), table_stride, entries, n_seq, refs.data_ptr(), n_pages,
+          src.data_ptr(), dst.data_ptr(), used.data_ptr(), ws.data_ptr(), ws.numel())
+    return src, dst, used
+
+
+def pages_copy(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copies page src[i] into page dst[i] (int32, on the device) of a pool
+    [(layers,) pages, 2, G, P, D], in every layer.  Pairs with a number outside
+    the pool are skipped.  A page must be in one pair alone, unless as the source
+    of several."""
+
+    layers = pool if pool.dim() == 6 else pool.unsqueeze(0)
+    if layers.dim() != 6 or layers.shape[0] == 0:
+        raise ValueError(f"a pool must be [pages, 2, G, P, D] or [layers, pages, 2, G, P, D], got {tuple(pool.shape)}")
+    n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(layers[0])
+    if src.dim() != 1 or src.dtype != torch.int32 or not src.is_contiguous() or dst.shape != src.shape or \
+            dst.dtype != torch.int32 or not dst.is_contiguous():
+        raise ValueError(f"src and dst must be int32 [pairs], got {src.dtype} {tuple(src.shape)} and {dst.dtype} "
+                         f"{tuple(dst.shape)}")
+    _inference_only("pages_copy", pool)
+    device = _same_device(pool, src, dst)
+    if src.numel() == 0 or n_pages == 0:
+        return
+    size = pool.element_size()
+    _call(device, "sva_pages_copy", pool.data_ptr(), n_pages, page_stride * size, layers.shape[0],
+          layers.stride(0) * size, 2 * kv_heads * page_rows * dim * size, src.data_ptr(), dst.data_ptr(), src.numel())
+
+
+# ---------------------------------------------------------------------------
+# the next token
+
+
+def _row_param(name: str, value, rows: int, dtype: torch.dtype):
+    """(tensor [rows] or None, scalar)."""
+
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous():
+        raise ValueError(f"{name} must be a number or a {dtype} tensor [{rows}], got {value.dtype} "
+                         f"{tuple(value.shape)}")
+    return value, 0
+
+
+def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0) -> torch.Tensor:
+    """The next token int64 [B] of every row of logits [B, V] from its random
+    number uniforms [B] (fp32, in [0, 1)).  Weights are exp((x - largest) /
+    temperature); kept are, of the tokens by falling logits (ties: the lower
+    first), the first top_k (0: all), of these the ones with less than top_p of
+    their sum before them (1: all), of these the ones of at least min_p of the
+    largest weight; the answer is the first token, by number, up to which the
+    kept weights sum to more than the random number times their sum.
+    temperature 0: the largest logit.  A NaN counts as -inf; a row of nothing
+    else gives -1.
+
+    temperature, top_k, top_p, min_p: a number, or a tensor [B] on the device
+    (fp32; top_k int64)."""
+
+    if logits.dim() != 2 or uniforms.dtype != torch.float32 or uniforms.shape != logits.shape[:1] or \
+            not uniforms.is_contiguous():
+        raise ValueError(f"logits [B, V] need fp32 uniforms [B], got {tuple(logits.shape)} and {uniforms.dtype} "
+                         f"{tuple(uniforms.shape)}")
+    rows, vocab = logits.shape
+    if vocab < 1 or vocab > 1 << 20:
+        raise ValueError(f"sample_tokens takes 1 to {1 << 20} tokens, got {vocab}")
+    t, t1 = _row_param("temperature", temperature, rows, torch.float32)
+    k, k1 = _row_param("top_k", top_k, rows, torch.int64)
+    p, p1 = _row_param("top_p", top_p, rows, torch.float32)
+    m, m1 = _row_param("min_p", min_p, rows, torch.float32)
+    if not (t1 >= 0 and k1 >= 0 and 0 <= p1 <= 1 and 0 <= m1 <= 1):
+        raise ValueError(f"temperature {t1} and top_k {k1} must not be negative, top_p {p1} and min_p {m1} lie in [0, 1]")
+    _inference_only("sample_tokens", logits)
+    dtype = dtype_code(logits)
+    device = _same_device(logits, uniforms, t, k, p, m)
+    if logits.stride(-1) != 1 or logits.stride(0) < 0:
+        logits = logits.contiguous()
+    tokens = torch.empty(rows, device=device, dtype=torch.int64)
+    if rows:
+        _call(device, "sva_sample_tokens", logits.data_ptr(), dtype, logits.stride(0), rows, vocab, uniforms.data_ptr(),
+              ptr(t), float(t1), ptr(k), int(k1), ptr(p), float(p1), ptr(m), float(m1), tokens.data_ptr())
+    return tokens

@@ -1,0 +1,183 @@
+"""The next token of a row of logits against the definition in 64 bits, at ties, cuts and values where it can go wrong."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from .paged_reference import sample
+
+pytestmark = pytest.mark.gpu
+
+# The kernel's shares of the sum are off by its weights' rounding: exp in 64 bits (a polynomial of degree 4 on 2^-7.5 of a
+# binade, 4e-14, and a table, 2^-53) and half of 2^-45 of the largest weight a token (2^-42 for 2^20 tokens), of at most
+# 2^20 tokens and a sum of at least 1 such weight.  A row whose border lies nearer than this to its random number or cut
+# has two answers; the rows below are none of these (asserted).
+def border(vocab):
+    point = min(46, 62 - max(0, (vocab - 1).bit_length()))
+    return 1e-13 + vocab * 2.0 ** -(point + 1)
+
+
+def compare(device, logits, u, dtype, near=None, **params):
+    """logits float32 [B, V]; params: numbers, or arrays [B]; near: the border's width."""
+    from sva_amd import kernels
+
+    x = torch.as_tensor(np.asarray(logits, np.float32)).to(device, dtype)
+    un = torch.as_tensor(np.asarray(u, np.float32)).to(device)
+    types = {"temperature": torch.float32, "top_k": torch.int64, "top_p": torch.float32, "min_p": torch.float32}
+    given = {k: torch.as_tensor(v).to(device, types[k]) if isinstance(v, np.ndarray) else v for k, v in params.items()}
+    got = kernels.sample_tokens(x, un, **given).tolist()
+    ref = x.double().cpu().numpy()
+    known = 0
+    for b in range(len(ref)):
+        p = {k: float(np.float32(v[b] if isinstance(v, np.ndarray) else v)) if k != "top_k" else
+             int(v[b] if isinstance(v, np.ndarray) else v) for k, v in params.items()}
+        want = sample(ref[b], float(un[b]), border=border(ref.shape[1]) if near is None else near, **p)
+        known += want is not None
+        assert want is None or got[b] == want, (b, got[b], want, p, float(un[b]))
+    assert known > len(ref) // 2
+    return got
+
+
+def normal(rng, B, V, spread=2.0):
+    return (rng.standard_normal((B, V)) * spread).astype(np.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [1, 2, 7, 64, 1000, 8191, 8192, 8193, 50001, 131072])
+def test_vocabularies(device, V, dtype):
+    rng = np.random.default_rng(V)
+    B = 12
+    compare(device, normal(rng, B, V), rng.random(B), dtype)
+    compare(device, normal(rng, B, V), rng.random(B), dtype, temperature=0.7, top_k=min(V, 50), top_p=0.9)
+    compare(device, normal(rng, B, V), rng.random(B), dtype, temperature=1.4, top_p=0.95, min_p=0.002)
+    compare(device, normal(rng, B, V), rng.random(B), dtype, temperature=0.0, top_k=7)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_every_row_its_own(device, dtype):
+    rng = np.random.default_rng(1)
+    B, V = 300, 3001
+    compare(device, normal(rng, B, V, 3.0), rng.random(B), dtype,
+            temperature=rng.choice([0.0, 0.2, 0.7, 1.0, 2.0], B).astype(np.float32),
+            top_k=rng.choice([0, 1, 2, 50, 2000, 3000, 3001, 10 ** 12, -4], B),
+            top_p=rng.choice([1.0, 0.9, 0.5, 0.01, 0.0, 0.9999], B).astype(np.float32),
+            min_p=rng.choice([0.0, 0.0, 0.1, 0.001, 1.0], B).astype(np.float32))
+
+
+@pytest.mark.parametrize("top_k,top_p", [(0, 1.0), (5000, 1.0), (0, 0.5), (7000, 0.3), (3, 0.5), (0, 0.00001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_ties(device, top_k, top_p, dtype):
+    """All logits equal, or of four values: cuts fall among more ties than are sorted; the lowest tokens stay."""
+    rng = np.random.default_rng(7)
+    V = 20000
+    for x in (np.full((6, V), -3.5, np.float32), rng.choice([0.0, -0.0, 1.0, -2.0], (6, V)).astype(np.float32)):
+        u = np.array([0.0, 0.25 + 1e-5, 0.5, 0.7, 0.9, 1 - 2.0 ** -24], np.float32)
+        # (equal logits weigh 1 each: their sums, and a sum of 15 bits times a number of 24, are exact, at a border too)
+        compare(device, x, u, dtype, near=0.0 if x.min() == x.max() else None, top_k=top_k, top_p=top_p)
+
+
+@pytest.mark.parametrize("top_k,top_p,T", [(5000, 1.0, 1.0), (0, 0.7, 1.0), (9000, 0.9, 1.0), (3000, 0.5, 0.01), (0, 0.999, 30.0)])
+def test_cuts_far_below_the_largest(device, top_k, top_p, T):
+    """One logit far above the others, so that a cut lies where the first bins say nothing; and logits far apart."""
+    rng = np.random.default_rng(3)
+    V = 30000
+    x = normal(rng, 8, V)
+    x[:4, 77] = 300.0
+    x[4:] *= 1e4
+    compare(device, x, rng.random(8), torch.float32, top_k=top_k, top_p=top_p, temperature=T)
+
+
+def test_values_that_are_not_finite(device):
+    rng = np.random.default_rng(5)
+    V = 9000
+    x = normal(rng, 8, V)
+    x[0] = -np.inf
+    x[1] = np.nan
+    x[2, ::2] = np.nan                 # as -inf
+    x[3, 5:] = -np.inf                 # five tokens
+    x[4, [17, 4000, 8999]] = np.inf    # share all of the weight
+    x[5, :8990] = np.finfo(np.float32).min
+    x[6] = -np.inf
+    x[6, 8999] = -3e38
+    u = np.array([0.5, 0.5, 0.3, 0.6, 0.5, 0.5, 0.99, 0.8])
+    for params in ({}, {"top_k": 40}, {"top_p": 0.9}, {"min_p": 0.1}, {"temperature": 0.0}, {"top_k": 8000, "top_p": 0.5}):
+        got = compare(device, x, u, torch.float32, **params)
+        assert got[0] == got[1] == -1 and got[6] == 8999 and got[4] in (17, 4000)
+
+
+def test_numbers_at_the_ends(device):
+    """0: the first kept token with any weight; just under 1, and 1 and above: the last; below 0 and NaN: as 0."""
+    from sva_amd import kernels
+
+    x = torch.tensor([[-200.0, 1.0, 3.0, 2.0, -200.0]], device=device).repeat(6, 1)
+    u = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, 7.0, -1.0, float("nan")], device=device)
+    assert kernels.sample_tokens(x, u).tolist() == [1, 3, 3, 3, 1, 1]
+    assert kernels.sample_tokens(x, u, top_k=2).tolist() == [2, 3, 3, 3, 2, 2]
+    odd = torch.tensor([float("nan")] * 6, device=device)
+    assert kernels.sample_tokens(x, u, top_p=odd).tolist() == [2] * 6        # one at least
+    assert kernels.sample_tokens(x, u, temperature=odd).tolist() == [2] * 6  # no weight at all: the largest
+    wide = torch.tensor([float("inf")] * 6, device=device)
+    assert kernels.sample_tokens(x, u, temperature=wide).tolist() == [0, 4, 4, 4, 0, 0]
+
+
+def test_strides_and_the_largest_vocabulary(device):
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(9)
+    V = 5003
+    x = torch.as_tensor(normal(rng, 6, V)).to(device)
+    u = torch.as_tensor(rng.random(6).astype(np.float32)).to(device)
+    want = kernels.sample_tokens(x, u, top_p=0.9)
+    padded = torch.full((6, 2, V + 5), 100.0, device=device)[:, 1]
+    padded[:, 1:V + 1] = x
+    assert torch.equal(kernels.sample_tokens(padded[:, 1:V + 1], u, top_p=0.9), want)
+    aligned = torch.full((6, 8192), 100.0, device=device)
+    aligned[:, :V] = x
+    assert torch.equal(kernels.sample_tokens(aligned[:, :V], u, top_p=0.9), want)
+    assert torch.equal(kernels.sample_tokens(x.T.contiguous().T, u, top_p=0.9), want)
+    assert torch.equal(kernels.sample_tokens(x[:1].expand(6, V), u, top_p=0.9)[:1], want[:1])
+    assert kernels.sample_tokens(x[:0], u[:0]).shape == (0,)
+    big = normal(rng, 3, 1 << 20)
+    compare(device, big, [0.1, 0.5, 0.9], torch.bfloat16)
+    compare(device, big, [0.1, 0.5, 0.9], torch.bfloat16, top_p=0.8, top_k=100000)
+
+
+def test_shares(device):
+    """Numbers spread evenly over [0, 1) give every token its share of them, within one."""
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(4)
+    n, V = 20000, 40
+    x = normal(rng, 1, V)
+    u = torch.as_tensor(((np.arange(n) + 0.5) / n).astype(np.float32)).to(device)
+    got = kernels.sample_tokens(torch.as_tensor(x).to(device).expand(n, V), u, temperature=0.9, top_k=20, top_p=0.95)
+    w = np.exp(x[0].astype(np.float64) / float(np.float32(0.9)))
+    order = np.argsort(-w)[:20]
+    share = np.cumsum(w[order]) / w[order].sum()
+    order = order[:int((share < float(np.float32(0.95))).sum()) + 1]
+    want = np.zeros(V)
+    want[order] = w[order] / w[order].sum() * n
+    assert (np.abs(np.bincount(got.cpu().numpy(), minlength=V) - want) <= 1.01 + n * 2.0 ** -23).all()
+
+
+def test_in_a_graph_and_on_another_stream(device):
+    from sva_amd import kernels
+
+    rng = np.random.default_rng(6)
+    x = torch.as_tensor(normal(rng, 5, 40000)).to(device)
+    u = torch.zeros(5, device=device)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        kernels.sample_tokens(x, u, top_p=0.9, top_k=10000)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kernels.sample_tokens(x, u, top_p=0.9, top_k=10000)
+    for i in range(10):
+        u.copy_(torch.as_tensor(rng.random(5).astype(np.float32)))
+        x.mul_(1.01)
+        graph.replay()
+        assert torch.equal(out, kernels.sample_tokens(x, u, top_p=0.9, top_k=10000)), i
