@@ -672,9 +672,11 @@ int sva_paged_read(const void *pool, int64_t n_pages, int64_t page_stride, int64
  *   out      (b, h, t, d) at b*out_seq_stride + h*out_head_stride +
  *            t*out_tok_stride + d
  * workspace: sva_paged_attention_workspace_bytes(...) bytes at n_keys, or at
- * max_pages * page_rows where that is less (no state between calls).
+ * max_pages * page_rows where that is less (no state between calls; 0: none
+ * is needed, and it may be NULL).
  */
-size_t sva_paged_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D, int64_t n_keys);
+size_t sva_paged_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D, int dtype,
+                                           int64_t n_keys);
 int sva_paged_attention(const void *q, int dtype, int64_t q_seq_stride, int64_t q_head_stride, int64_t q_tok_stride,
                         const void *pool, int64_t n_pages, int64_t page_stride, int64_t page_rows,
                         const int32_t *tables, int64_t table_stride, int64_t max_pages, const int64_t *seq_lens,

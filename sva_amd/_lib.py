@@ -96,7 +96,7 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
                              _I64, _P]),
     "sva_paged_read": (_I, [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _I, _I64, _I64,
                             _I64, _P]),
-    "sva_paged_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "sva_paged_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I, _I64]),
     "sva_paged_attention": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64,
                                  _I64, _I64, _I64, _F, _P, _I, _I64, _I64, _I64, _P, _SZ, _P]),
     "sva_pages_reserve_workspace_bytes": (_SZ, [_I64, _I64]),

@@ -62,8 +62,9 @@ struct PagedType {
   static constexpr int ES = DT == F32 ? 4 : 2;
   using elem = typename std::conditional<DT == BF16, __bf16, _Float16>::type;
   using frag = typename std::conditional<DT == BF16, bf16x8, f16x8>::type;
-  // waves per SIMD that the registers are kept to
-  static constexpr int waves(int dp, bool pad) { return dp * ES <= 128 ? (pad ? 3 : 4) : (dp * ES <= 256 ? 2 : 1); }
+  // waves per SIMD that the registers are kept to (four for the narrowest send 20 registers through scratch memory: 32
+  // sequences of up to 131072 keys, 9 x 64 bf16, 416 us against 297)
+  static constexpr int waves(int dp) { return dp * ES <= 128 ? 3 : (dp * ES <= 256 ? 2 : 1); }
 };
 
 template <int DT>
@@ -141,7 +142,7 @@ SVA_DEV void attend_again(const PagedParams& p, int64_t qa, int b, int g, int k0
 // DP: elements of a row that the tiles are laid out for; PAD: only p.D of them
 // are there.
 template <int DT, int DP, bool PAD>
-__global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP, PAD)) paged_attention_kernel(PagedParams p) {
+__global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP)) paged_attention_kernel(PagedParams p) {
   using Type = PagedType<DT>;
   constexpr bool WIDE = DT == F32;  // 32-bit elements
   constexpr int ES = Type::ES;
@@ -444,13 +445,20 @@ __global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP, PAD)) page
   }
 }
 
-// Keys per workgroup: enough workgroups to fill the card, four times as many
+// Keys per workgroup: enough workgroups to fill the card, eight times as many
 // where sequences may differ in length (the last to end is then a small part
-// of the call); ranges of at least 256 keys and at most 384 of them (each
-// costs a row of partial sums).
-int64_t chunk_keys(int64_t n_seq, int64_t groups, int64_t n_keys) {
-  const int64_t want = std::min<int64_t>(384, std::max<int64_t>(1, (n_seq > 1 ? 4096 : 1024) / groups));
-  return std::max<int64_t>(2 * STEP, ((n_keys + want - 1) / want + STEP - 1) / STEP * STEP);
+// of the call: 32 sequences of up to 131072 keys 383 us with a quarter as many,
+// 330 with half, 297); at most 384 ranges (each costs a row of partial sums),
+// of at least 256 keys, or of 1024 where those fill the card already (4 tokens
+// of 8 x 32768 keys, 12 x 64: 64 us, 71 with 256).  A range of 128 KB is one
+// workgroup's business, whatever follows: a CU takes 50 GB/s, and a second
+// launch 3 us (500 keys of 9 x 64: 7.4 us in one range, 9.2 in two; 1000 10.8
+// in one, 9.2 in four).
+int64_t chunk_keys(int64_t n_seq, int64_t groups, int64_t row_bytes, int64_t n_keys) {
+  if (n_keys * row_bytes <= 131072) return (n_keys + STEP - 1) / STEP * STEP;
+  const int64_t want = std::min<int64_t>(384, std::max<int64_t>(1, (n_seq > 1 ? 8192 : 1024) / groups));
+  const int64_t least = std::max<int64_t>(2 * STEP, std::min<int64_t>(8 * STEP, n_keys * groups / 768));
+  return (std::max<int64_t>(least, (n_keys + want - 1) / want) + STEP - 1) / STEP * STEP;
 }
 
 int64_t row_tiles(int64_t H, int64_t G, int64_t Q) { return (H / G * Q + TR - 1) / TR; }
@@ -471,11 +479,11 @@ int launch(const PagedParams& p, dim3 grid, hipStream_t stream) {
 }  // namespace
 
 extern "C" size_t sva_paged_attention_workspace_bytes(int64_t n_seq, int64_t H, int64_t G, int64_t Q, int64_t D,
-                                                      int64_t n_keys) {
+                                                      int dtype, int64_t n_keys) {
   if (n_seq <= 0 || H <= 0 || G <= 0 || Q <= 0 || D <= 0 || n_keys <= 0 || H % G != 0) return 0;
-  const int64_t chunk = chunk_keys(n_seq, n_seq * G * row_tiles(H, G, Q), n_keys);
+  const int64_t chunk = chunk_keys(n_seq, n_seq * G * row_tiles(H, G, Q), 2 * D * (dtype == F32 ? 4 : 2), n_keys);
   const int64_t splits = (n_keys + chunk - 1) / chunk;
-  return splits == 1 ? 256 : join_bytes(n_seq * H * Q, splits, D);
+  return splits == 1 ? 0 : join_bytes(n_seq * H * Q, splits, D);
 }
 
 extern "C" int sva_paged_attention(const void* q, int dtype, int64_t q_seq_stride, int64_t q_head_stride,
@@ -506,8 +514,8 @@ extern "C" int sva_paged_attention(const void* q, int dtype, int64_t q_seq_strid
   const int64_t tiles = row_tiles(H, G, Q);
   SVA_UNSUPPORTED(n_seq * G * tiles <= 65535, "sva_paged_attention: %lld tokens of %lld sequences in one call",
                   (long long)Q, (long long)n_seq);
-  const size_t need = sva_paged_attention_workspace_bytes(n_seq, H, G, Q, D, keys);
-  SVA_REQUIRE(workspace != nullptr && workspace_bytes >= need, "sva_paged_attention: workspace of %zu bytes required",
+  const size_t need = sva_paged_attention_workspace_bytes(n_seq, H, G, Q, D, dtype, keys);
+  SVA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "sva_paged_attention: workspace of %zu bytes required",
               need);
   PagedParams p;
   p.q = q;
@@ -530,7 +538,7 @@ extern "C" int sva_paged_attention(const void* q, int dtype, int64_t q_seq_strid
   p.Q = (int)Q;
   p.D = (int)D;
   p.row_tiles = (int)tiles;
-  p.chunk = (int)chunk_keys(n_seq, n_seq * G * tiles, keys);
+  p.chunk = (int)chunk_keys(n_seq, n_seq * G * tiles, 2 * D * es, keys);
   p.splits = (int)((keys + p.chunk - 1) / p.chunk);
   p.scaling = scaling;
   p.stats = (float*)workspace;

@@ -1238,11 +1238,11 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, s
     if n_keys <= 0 or n_pages == 0:
         return out.zero_()
     # a buffer of the call's own: calls on other streams and captured graphs never share one
-    ws = torch.empty(lib().sva_paged_attention_workspace_bytes(n_seq, heads, kv_heads, q_len, dim, n_keys),
-                     device=device, dtype=torch.uint8)
+    ws_bytes = lib().sva_paged_attention_workspace_bytes(n_seq, heads, kv_heads, q_len, dim, dtype, n_keys)
+    ws = torch.empty(ws_bytes, device=device, dtype=torch.uint8) if ws_bytes else None
     _call(device, "sva_paged_attention", q.data_ptr(), dtype, *q.stride()[:3], pool.data_ptr(), n_pages, page_stride,
           page_rows, tables.data_ptr(), table_stride, entries, seq_lens.data_ptr(), n_keys, n_seq, heads, kv_heads,
-          q_len, dim, float(scaling), out.data_ptr(), dtype_code(out), *out.stride()[:3], ws.data_ptr(), ws.numel())
+          q_len, dim, float(scaling), out.data_ptr(), dtype_code(out), *out.stride()[:3], ptr(ws), ws_bytes)
     return out
 
 

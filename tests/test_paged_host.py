@@ -142,7 +142,7 @@ def test_c_entries_refuse():
     refused("sva_paged_write", with_(write, {6: 40000}), "sequences", 3)
     read = [p, 4, 2 * 16 * 64, 16, p, 4, 4, p, 1, 1, 1, 64, p, p, 1, 64, 64, 64, None]
     refused("sva_paged_read", with_(read, {12: odd}), "16-byte")
-    attend = [p, 1, 64, 64, 64, p, 4, 2 * 16 * 64, 16, p, 4, 4, p, 64, 1, 1, 1, 1, 64, one, p, 1, 64, 64, 64, p, 1 << 20, None]
+    attend = [p, 1, 64, 64, 64, p, 4, 2 * 16 * 64, 16, p, 4, 4000, p, 64000, 1, 1, 1, 1, 64, one, p, 1, 64, 64, 64, p, 1 << 20, None]
     for changes, text in (({0: None}, "null"), ({12: None}, "null"), ({1: 5}, "dtype"), ({21: -1}, "dtype"), ({15: 3, 16: 2}, "sizes"),
                           ({18: 4}, "head_dim"), ({8: 17}, "rows a page"), ({5: odd}, "16-byte"), ({25: None}, "workspace"),
                           ({26: 10}, "workspace"), ({17: 0}, "sizes"), ({11: 1 << 30, 13: 1 << 40}, "too many")):
@@ -169,7 +169,7 @@ def test_c_entries_refuse():
 def test_workspaces():
     lib = _kernels().lib()
     size = lib.sva_paged_attention_workspace_bytes
-    assert size(0, 9, 3, 1, 64, 100) == size(1, 9, 2, 1, 64, 100) == 0
-    assert size(1, 9, 3, 1, 64, 256) == 256 < size(1, 9, 3, 1, 64, 100000) < 1 << 24
+    assert size(0, 9, 3, 1, 64, 1, 100000) == size(1, 9, 2, 1, 64, 1, 100000) == size(1, 9, 3, 1, 64, 1, 256) == 0
+    assert 256 < size(1, 9, 3, 1, 64, 0, 100000) < 1 << 24
     assert lib.sva_pages_reserve_workspace_bytes(3, 10) >= 3 * 16 + 40
     assert lib.sva_pages_fork_workspace_bytes(3, 10) >= 3 * 8 + 120 and lib.sva_pages_compact_workspace_bytes(7) >= 28
