@@ -5,19 +5,30 @@
 // are among the first top_k, have less than top_p of the sum of these before
 // them, and weigh at least min_p; the answer is the first token, by number, up
 // to which the kept weights sum to more than u of their sum.  T <= 0: the
-// largest logit.  A NaN counts as -inf; logits of +inf share all of the weight.
+// largest logit.  A NaN counts as -inf; infinity counts as the largest number.
 //
 // A token is a whole number, so weights are taken in 64 bits: exp2 from a table
-// of 64 and a polynomial, rounded to fixed point (up to 46 bits behind the
+// of 256 and a cubic (2e-13), rounded to fixed point (up to 46 bits behind the
 // point; 2^-47 of the largest is lost at most).  Sums of fixed-point weights are
 // exact, whatever their order: LDS atomics change no result.
 //
-// A row is one workgroup's, which reads it a few times (from the caches, after
-// the first): for M; for a histogram of counts or weights over 2048 bins of
-// x, linear below M; for the elements of the bin in which a cut falls, which
-// are sorted in LDS (a bin of too many is narrowed by the bits of x); for the
-// weights of the kept tokens by wave, then again by the one wave in whose share
-// the answer lies.
+// A row is one workgroup's, which reads it twice, the first time from memory:
+//  * for M and each thread's largest; where a cut is asked for, for a histogram
+//    over 2048 bins of x too, of counts and fp32 weights in one 64-bit word: it
+//    names the bin in which the cut falls.  (top_k of a few: the bin that top_k
+//    of the threads' largest reach bounds the cut, no histogram is needed);
+//  * for the exact weights above that bin (and of the whole row, for top_p),
+//    summed by shares of 2048 elements, and the bin's elements, which are sorted
+//    in LDS: exact weights decide the cut.
+// The share in which the answer lies is gone over again.  What the histogram
+// cannot decide (a bin of more elements than are sorted, logits or a temperature
+// at the ends of their range) is done over again with exact weights throughout,
+// bins narrowed by the bits of x.
+// What bounds it (256 rows of 131072 bf16 logits; 67 MB): the read for greedy
+// rows, 17 us; the 64-bit operations of the weights, 28 us a pass, in rows
+// without a cut (44); for top_p the histogram's exponentials and LDS atomics
+// too, 25 (84 to 95).  One row of 49152 fp32 logits, top_k 50, top_p 0.95: 14.6,
+// two passes of one CU over 192 KB and a dozen short steps between barriers.
 #include <algorithm>
 
 #include "capi_internal.h"
@@ -28,16 +39,26 @@ using namespace sva;
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64;
 
-constexpr int SB = 1024;        // threads
+constexpr int SB = 512;         // threads: two waves a SIMD, whose registers hold several weights in work
 constexpr int SW = SB / WAVE;
 constexpr int E = 8;            // consecutive elements of a thread
-constexpr int TILE = SB * E;    // elements that the workgroup takes at a time
+constexpr int STEP = WAVE * E;  // elements that a wave takes at a time,
+constexpr int STEPS = 4;        // this often one after another:
+constexpr int SHARE = STEP * STEPS;
+constexpr int GROUP = SW * SHARE;
+constexpr int LIGHT = 6, HEAVY = 2;  // steps under way of passes that do little, or much, with them
 constexpr int BINS = 2048;
 constexpr int CAP = 2048;       // elements of a bin that are sorted
+constexpr int PT = BINS / SB;    // bins, or elements of a list, of a thread
+static_assert(CAP == BINS, "");
 constexpr int64_t kMaxVocab = 1 << 20;
-constexpr int MAX_TILES = (int)(kMaxVocab / TILE);
-static_assert(MAX_TILES * SW <= BINS, "the waves' sums take the histogram's place");
+constexpr int SHARES = (int)(kMaxVocab / SHARE) + SW;
+static_assert(SHARES <= 2 * SB, "");
+constexpr int MANY = 8192;       // tokens that are listed
+constexpr u64 kRaw = 0x4330000000000000ull;  // the bits of 2^52
+constexpr int kFew = 256;       // top_k that the threads' largest bound
 
 struct SampleParams {
   const void* logits;
@@ -51,32 +72,39 @@ struct SampleParams {
   float temperature1, top_p1, min_p1;
   int64_t top_k1;
   int64_t* out;
-  int point;  // bits behind the fixed point
+  int point;       // bits behind the fixed point
+  int vocab_bits;  // 2^vocab_bits tokens at least
 };
 
 struct SampleLds {
-  double table[64];              // 2^(j / 64)
-  unsigned long long mass[BINS]; // also the waves' sums of the last pass
+  double table[256];  // 2^(j / 256 + point)
+  u64 hist[BINS];
   uint32_t count[BINS];
-  unsigned long long list[CAP];
-  unsigned long long scan[SW];
-  unsigned long long word[4];
+  u64 sums[SHARES];   // the kept weights of a share
+  u64 list[2][CAP];
+  uint32_t many[MANY];
+  u64 sorted[SB];
+  u64 scan[SW];
+  u64 word[6];
   float top[SW];
-  uint32_t n;
+  uint32_t n[3];
 };
 
+// A NaN is no token's, and infinity the largest number.
+SVA_DEV float number(float x) { return x == x ? fminf(x, 3.40282347e38f) : -INFINITY; }
+
 // Inclusive sum over the workgroup's threads in order; `total` of all.
-SVA_DEV unsigned long long upto_u64(unsigned long long v, SampleLds& s, unsigned long long& total) {
+SVA_DEV u64 upto_u64(u64 v, SampleLds& s, u64& total) {
   const int lane = lane_id(), w = (int)threadIdx.x / WAVE;
 #pragma unroll
   for (int k = 1; k < WAVE; k <<= 1) {
-    const unsigned long long x = __shfl_up(v, k, WAVE);
+    const u64 x = __shfl_up(v, k, WAVE);
     if (lane >= k) v += x;
   }
   __syncthreads();
   if (lane == WAVE - 1) s.scan[w] = v;
   __syncthreads();
-  unsigned long long before = 0;
+  u64 before = 0;
   total = 0;
 #pragma unroll
   for (int k = 0; k < SW; ++k) {
@@ -86,297 +114,800 @@ SVA_DEV unsigned long long upto_u64(unsigned long long v, SampleLds& s, unsigned
   return v + before;
 }
 
-template <int DT, bool VEC>
-struct Row {
-  const unsigned char* p;
-  int vocab;
-  float M;         // the largest logit
-  double rate;     // log2(e) / T
-  float per;       // bins below M for a logit's difference of 1
-  double one;      // 2^point
-  const double* table;
-
-  // elements at .. at + 7; those behind the row and NaN are -inf
-  SVA_DEV void load(int at, float (&x)[E]) const {
-    if (VEC && at + E <= vocab) {
-      if constexpr (DT == F32) {
-        const float4 a = *(const float4*)(p + (int64_t)at * 4), b = *(const float4*)(p + (int64_t)at * 4 + 16);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-      } else {
-        const u32x4 a = *(const u32x4*)(p + (int64_t)at * 2);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[2 * k] = elem_from_bits(a[k] & 0xFFFFu, DT), x[2 * k + 1] = elem_from_bits(a[k] >> 16, DT);
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < E; ++k) x[k] = at + k < vocab ? load_elem(p, at + k, DT) : -INFINITY;
-    }
-#pragma unroll
-    for (int k = 0; k < E; ++k) x[k] = x[k] == x[k] ? x[k] : -INFINITY;
-  }
-  // f(tile, first element, the elements), the next tile's under way
-  template <typename F>
-  SVA_DEV void each(F f) const {
-    const int first = (int)threadIdx.x * E;
-    float x[E], y[E];
-    load(first, x);
-    for (int tile = 0; tile * TILE < vocab; ++tile) {
-      const int at = tile * TILE + first;
-      if ((tile + 1) * TILE < vocab) load(at + TILE, y);
-      f(tile, at, x);
-#pragma unroll
-      for (int k = 0; k < E; ++k) x[k] = y[k];
-    }
-  }
-  // exp((x - M) / T) and its fixed-point number
-  SVA_DEV double weight(float x) const {
-    const double t = x == M ? 0.0 * rate : ((double)x - (double)M) * rate;
-    const double c = __builtin_fmax(t, -128.0);  // (a NaN: -128)
-    const double n = __builtin_rint(c * 64.0);
-    const double u = (c - n * 0.015625) * 0.69314718055994530942;
-    const int i = (int)n;
-    double e = __builtin_fma(u, 1.0 / 24.0, 1.0 / 6.0);
-    e = __builtin_fma(u, e, 0.5);
-    e = __builtin_fma(u, e, 1.0);
-    e = __builtin_fma(u, e, 1.0);
-    return __builtin_amdgcn_ldexp(e * table[i & 63], i >> 6);
-  }
-  SVA_DEV unsigned long long fixed(double w) const {
-    // (at most 2^46: behind 2^52 the integer stands in the low bits)
-    return (unsigned long long)__double_as_longlong(__builtin_fma(w, one, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-  }
-  SVA_DEV int bin(float x) const {
-    const float b = x == M ? 0.0f : (M - x) * per;
-    return (int)fminf(b, (float)(BINS - 1));
+// Eight elements as they lie in memory.
+template <int DT>
+struct Raw {
+  u32x4 w[DT == F32 ? 2 : 1];
+  SVA_DEV float operator[](int k) const {
+    if constexpr (DT == F32) return __uint_as_float(w[k / 4][k % 4]);
+    else return elem_from_bits(k & 1 ? w[0][k / 2] >> 16 : w[0][k / 2] & 0xFFFFu, DT);
   }
 };
 
-// A cut in the order of falling logits: composites of at least `thr` are kept.
-// MASS false: the first `want` elements.  MASS true: of the elements of at
-// least `from`, those with less than `share` of their sum before them (one at
-// least).
-template <bool MASS, typename R>
-SVA_DEV unsigned long long cut(const R& row, SampleLds& s, unsigned long long from, unsigned long long want, double share) {
-  const int tid = (int)threadIdx.x;
-  unsigned long long above = 0;  // counts or weights before the current range
-  int bin = -1;                  // the current range: elements of this bin whose key's bits from `bits` on are `prefix`
-  int bits = 32;
-  uint32_t prefix = 0;
-  auto inside = [&](float x, uint32_t key, int at) {
-    return composite(key, (uint32_t)at) >= from && (bin < 0 || row.bin(x) == bin) &&
-           (bits == 32 || key >> bits == prefix);
-  };
-  for (int level = 0;; ++level) {
-    for (int k = tid; k < BINS; k += SB) s.count[k] = 0u, s.mass[k] = 0ull;
-    __syncthreads();
-    const int next = bits >= 11 ? bits - 11 : 0;
-    row.each([&](int, int at, const float (&x)[E]) {
+template <int DT>
+struct Row {
+  static constexpr int ES = DT == F32 ? 4 : 2;
+  const unsigned char* p;  // a whole 16-byte word: element `skip` of it is the row's first
+  int skip, vocab, steps;
+  float M;                 // the largest logit
+  float ref, per;          // where the bins begin, and bins for a logit's difference of 1
+  double rate, off;        // x rate + off: 256ths of a binade below M
+  float T, least;          // logits below the least weigh nothing
+  u64 least_w;             // min_p
+  const double* table;
+
+  // elements at + k of the aligned window; what lies outside the row is -inf
+  SVA_DEV Raw<DT> load(int at) const {
+    Raw<DT> r;
+    if (at >= skip && at + E <= skip + vocab) {
+      const u32x4* q = (const u32x4*)(p + (int64_t)at * ES);
+      r.w[0] = q[0];
+      if constexpr (DT == F32) r.w[1] = q[1];
+    } else {
+      const uint32_t none = DT == F32 ? 0xFF800000u : (DT == BF16 ? 0xFF80u : 0xFC00u);
+      if (at >= skip + vocab) {
+#pragma unroll
+        for (int k = 0; k < 4 * (int)(sizeof(r.w) / sizeof(r.w[0])); ++k) r.w[k / 4][k % 4] = DT == F32 ? none : none << 16 | none;
+        return r;
+      }
 #pragma unroll
       for (int k = 0; k < E; ++k) {
-        const uint32_t key = f2key(x[k]);
-        if (at + k >= row.vocab || !inside(x[k], key, at + k)) continue;
-        const int i = level == 0 ? row.bin(x[k]) : (int)(key >> next) & ((1 << (bits - next)) - 1);
-        atomicAdd(&s.count[i], 1u);
-        if (MASS) atomicAdd(&s.mass[i], row.fixed(row.weight(x[k])));
+        const bool in = at + k >= skip && at + k < skip + vocab;
+        const uint32_t b = in ? load_elem_bits(p, at + k, DT) : none;
+        if constexpr (DT == F32) r.w[k / 4][k % 4] = b;
+        else r.w[0][k / 2] = k & 1 ? r.w[0][k / 2] | b << 16 : b;
       }
-    });
-    __syncthreads();
-    // falling order: bins of level 0 rise, keys fall
-    unsigned long long mine[2], total;
-    int at[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      at[k] = level == 0 ? 2 * tid + k : BINS - 1 - (2 * tid + k);
-      mine[k] = MASS ? s.mass[at[k]] : s.count[at[k]];
     }
-    const unsigned long long end = upto_u64(mine[0] + mine[1], s, total);
-    if (MASS && level == 0) {
-      const double t = __builtin_ceil((double)total * share);
-      want = t >= 1.0 ? (unsigned long long)t : 1ull;  // (a NaN: 1)
-      want = want < total ? want : total;
-    }
-    // the range in which the want-th unit lies
-    unsigned long long before = above + end - mine[0] - mine[1];
+    return r;
+  }
+  // the largest logit is known
+  SVA_DEV void begin(float largest) {
+    M = largest;
+    off = -(double)M * rate;
+    least = M - 55.4f * T;  // 2^-80
+  }
+  SVA_DEV bool plain() const { return T >= 1e-30f && __builtin_fabs(off) <= 268435456.0; }
+  SVA_DEV bool has(int token) const { return (uint32_t)token < (uint32_t)vocab; }
+  // this thread's elements of a step, in the window
+  static SVA_DEV int place(int step) {
+    const int tid = (int)threadIdx.x;
+    return step / STEPS * GROUP + tid / WAVE * SHARE + step % STEPS * STEP + tid % WAVE * E;
+  }
+  // f(step, the first one's token, elements), A steps under way (one turn of
+  // the loop takes A: registers that are loaded into do not move)
+  template <int A, typename F>
+  SVA_DEV void each(F f) const {
+    Raw<DT> r[A];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (before < want && before + mine[k] >= want) s.word[0] = before, s.word[1] = (unsigned long long)at[k];
-      before += mine[k];
-    }
-    __syncthreads();
-    above = s.word[0];
-    const int hit = (int)s.word[1];
-    const uint32_t count = s.count[hit];
-    __syncthreads();
-    if (level == 0) bin = hit;
-    else prefix = (bits == 32 ? 0u : prefix << (bits - next)) | (uint32_t)hit, bits = next;
-    if (count <= CAP) {
-      // sorted: the last one kept
-      if (tid == 0) s.n = 0u;
-      __syncthreads();
-      row.each([&](int, int at, const float (&x)[E]) {
+    for (int j = 0; j < A; ++j)
+      if (j < steps) r[j] = load(place(j));
+    for (int base = 0; base < steps; base += A) {
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-          const uint32_t key = f2key(x[k]);
-          if (at + k < row.vocab && inside(x[k], key, at + k)) s.list[atomicAdd(&s.n, 1u)] = composite(key, (uint32_t)(at + k));
+      for (int j = 0; j < A; ++j) {
+        const int step = base + j;
+        if (step < steps) {
+          const Raw<DT> x = r[j];
+          if (step + A < steps) r[j] = load(place(step + A));
+          f(step, place(step) - skip, x);
+          __builtin_amdgcn_sched_barrier(0);
         }
-      });
-      __syncthreads();
-      const int n = (int)s.n, padded = max(2, next_pow2(n));
-      for (int k = n + tid; k < padded; k += SB) s.list[k] = 0ull;
-      __syncthreads();
-      bitonic_sort_u64<SB>((uint64_t*)s.list, padded, true);
-      __syncthreads();
-      unsigned long long mine[2], total;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int i = 2 * tid + k;
-        mine[k] = i >= n ? 0ull : (MASS ? row.fixed(row.weight(key2f(composite_key(s.list[i])))) : 1ull);
       }
-      unsigned long long before = above + upto_u64(mine[0] + mine[1], s, total) - mine[0] - mine[1];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (before < want && before + mine[k] >= want) s.word[2] = s.list[2 * tid + k];
-        before += mine[k];
-      }
-      __syncthreads();
-      return s.word[2];
-    }
-    if (level > 0 && bits == 0) {
-      // more ties than can be sorted: of equal weights, the lowest tokens
-      const float x = key2f(prefix);
-      const unsigned long long each = MASS ? row.fixed(row.weight(x)) : 1ull;
-      const unsigned long long n = (want - above + each - 1) / each;  // (each > 0: the range holds the want-th unit)
-      const int token = locate(row, s, [&](float v, int at) { return f2key(v) == prefix && composite(prefix, (uint32_t)at) >= from ? 1ull : 0ull; },
-                               [&](unsigned long long) { return n - 1; });
-      return composite(prefix, (uint32_t)token);
     }
   }
+  SVA_DEV float at(int token) const { return load_elem(p, (int64_t)token + skip, DT); }
+  SVA_DEV float below(float x) const { return (ref - x) * per; }
+  // 2^(t / 256) in fixed point, with kRaw added
+  SVA_DEV u64 raw(double t) const {
+    const double y = t + 6755399441055744.0;  // the integer in the low bits
+    const int n = (int)__double_as_longlong(y);
+    const double r = t - (y - 6755399441055744.0);
+    constexpr double c = 0.69314718055994530942 / 256.0;
+    double e = __builtin_fma(r, c * c * c / 6.0, c * c / 2.0);
+    e = __builtin_fma(r, e, c);
+    e = __builtin_fma(r, e, 1.0);
+    union {
+      double d;
+      uint32_t w[2];
+    } two;
+    two.d = table[n & 255];
+    two.w[1] += (uint32_t)(n & ~255) << 12;
+    return (u64)__double_as_longlong(__builtin_fma(e, two.d, 4503599627370496.0));
+  }
+  // exp((x - M) / T) so.  x rate + off is off by 2^-53 of off, the same for all;
+  // a NaN counts as the least.  (One of eight 64-bit operations less than from
+  // x - M, and these take twice as long as others here.)
+  SVA_DEV u64 raw_weight(float x) const { return raw(__builtin_fma((double)fmaxf(x, least), rate, off)); }
+  SVA_DEV u64 weight(float x) const { return raw_weight(x) - kRaw; }
+};
+
+// The same for temperatures so far from the logits' size that off is too large,
+// or the least logit that counts is M itself.
+template <int DT>
+struct OddRow : Row<DT> {
+  SVA_DEV u64 weight(float x) const {
+    return this->raw(__builtin_fmax(((double)x - (double)this->M) * this->rate, -20480.0)) - kRaw;
+  }
+};
+
+template <typename R>
+SVA_DEV int bin_of(const R& row, float x) {
+  return (int)fmaxf(fminf(row.below(x), (float)(BINS - 1)), 0.0f);
 }
 
-// The first element up to which f(x, number) sums to more than pick(the whole
-// sum); -1 where the sum is 0.
-template <typename R, typename F, typename P>
-SVA_DEV int locate(const R& row, SampleLds& s, F f, P pick) {
-  const int tid = (int)threadIdx.x, lane = lane_id(), w = tid / WAVE;
-  unsigned long long* sums = s.mass;  // [tile][wave]
-  auto of8 = [&](int at, const float (&x)[E]) {
-    unsigned long long v = 0;
+// A thread's largest element, and the first step that has it.
+struct Largest {
+  float x = -INFINITY;
+  int step = 0;
+
+  template <typename X>
+  SVA_DEV void add(int at, const X& e) {
+    float y = e[0];
 #pragma unroll
-    for (int k = 0; k < E; ++k) v += at + k < row.vocab ? f(x[k], at + k) : 0ull;
-    return v;
-  };
+    for (int k = 1; k < E; ++k) y = fmaxf(y, e[k]);  // (a NaN is none)
+    step = y > x ? at : step;
+    x = fmaxf(x, y);
+  }
+};
+SVA_DEV float block_max(SampleLds& s, float x) {
+  x = wave_max(x);
   __syncthreads();
-  row.each([&](int tile, int at, const float (&x)[E]) {
-    unsigned long long v = of8(at, x);
-    if (__ballot(v != 0ull) != 0ull) {
+  if (lane_id() == 0) s.top[(int)threadIdx.x / WAVE] = x;
+  __syncthreads();
 #pragma unroll
-      for (int k = 1; k < WAVE; k <<= 1) v += __shfl_xor(v, k, WAVE);
+  for (int w = 0; w < SW; ++w) x = fmaxf(x, s.top[w]);
+  return fminf(x, 3.40282347e38f);
+}
+
+// Tokens that a pass lists in s.many: a thread keeps a bit for each of its
+// elements of eight steps, then their places come from one scan of the wave's
+// counts and one LDS atomic (for every step these took longer than the pass).
+struct Marks {
+  u64 bits = 0;
+
+  template <typename R>
+  SVA_DEV void add(const R& row, SampleLds& s, int step, uint32_t mask) {
+    bits |= (u64)mask << (8 * (step & 7));
+    if ((step & 7) == 7 || step == row.steps - 1) put(row, s, step & ~7);
+  }
+  template <typename R>
+  SVA_DEV void put(const R& row, SampleLds& s, int step) {
+    const uint32_t mine = (uint32_t)__popcll(bits);
+    if (__ballot(mine != 0u) == 0ull) return;
+    const uint32_t upto = wave_incl_scan(mine);
+    uint32_t i = 0;
+    if (lane_id() == WAVE - 1) i = atomicAdd(&s.n[2], upto);
+    i = (uint32_t)__builtin_amdgcn_readlane((int)i, WAVE - 1) + upto - mine;
+    for (; bits != 0ull; bits &= bits - 1, ++i) {
+      const int k = __builtin_ctzll(bits);
+      if (i < MANY) s.many[i] = (uint32_t)(R::place(step + k / E) + k % E - row.skip);
     }
-    if (lane == 0) sums[tile * SW + w] = v;
+  }
+};
+
+// The list's n elements in falling order: in s.sorted (n <= SB), or in place.
+SVA_DEV const u64* sort_list(SampleLds& s, u64* list, int n) {
+  const int tid = (int)threadIdx.x;
+  __syncthreads();
+  if (n > SB) {
+    const int padded = next_pow2(n);
+    for (int k = n + tid; k < padded; k += SB) list[k] = 0ull;
+    __syncthreads();
+    bitonic_sort_u64<SB>((uint64_t*)list, padded, true);
+    return list;
+  }
+  if (tid < n) {  // ranks by counting
+    const u64 mine = list[tid];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += list[j] > mine ? 1 : 0;
+    s.sorted[rank] = mine;
+  }
+  __syncthreads();
+  return s.sorted;
+}
+
+// What less than `share` of the whole sum comes to: elements with less than
+// this before them are kept.
+SVA_DEV u64 share_of(double share, u64 total) {
+  const double t = __builtin_ceil((double)total * share);
+  const u64 want = t >= 1.0 ? (u64)t : 1ull;  // (a NaN: 1)
+  return want < total ? want : total;
+}
+
+// Of n elements in falling order, with `above` of weight before them: how many
+// have less than `share` of `whole` (0: of theirs and `above`) before them; -1
+// where the last of these is none of the n.
+template <typename R>
+SVA_DEV int within_share(const R& row, SampleLds& s, const u64* sorted, int n, u64 above, u64 whole, double share) {
+  const int tid = (int)threadIdx.x;
+  u64 mine[PT], sum = 0, here;
+#pragma unroll
+  for (int k = 0; k < PT; ++k) {
+    mine[k] = PT * tid + k < n ? row.weight(key2f(composite_key(sorted[PT * tid + k]))) : 0ull;
+    sum += mine[k];
+  }
+  u64 before = above + upto_u64(sum, s, here) - sum;
+  const u64 want = share_of(share, whole ? whole : above + here);
+  if (want <= above || want > above + here) return -1;
+#pragma unroll
+  for (int k = 0; k < PT; ++k) {
+    if (PT * tid + k < n && before < want && before + mine[k] >= want) s.word[2] = (u64)(PT * tid + k + 1);
+    before += mine[k];
+  }
+  __syncthreads();
+  return (int)s.word[2];
+}
+
+// A step's weights v into its share's sum: of the wave together after the last.
+struct Share {
+  u64 sum = 0;
+
+  SVA_DEV void add(SampleLds& s, int step, u64 v) {
+    sum += v;
+    if (step % STEPS != STEPS - 1) return;
+    if (__ballot(sum != 0ull) != 0ull) {
+#pragma unroll
+      for (int k = 1; k < WAVE; k <<= 1) sum += __shfl_xor(sum, k, WAVE);
+    }
+    if (lane_id() == 0) s.sums[step / STEPS * SW + (int)threadIdx.x / WAVE] = sum;
+    sum = 0;
+  }
+};
+
+// The sums of f(x, token) by share (0 for what is no token, at -inf).  No branch
+// around an f: eight at once hide one another's latency (131072 weights: 48 us
+// where each stood behind its own condition).
+template <typename R, typename F>
+SVA_DEV void sum_shares(const R& row, SampleLds& s, F f) {
+  __syncthreads();
+  Share share;
+  row.template each<HEAVY>([&](int step, int at, const auto& x) {
+    u64 v = 0;
+#pragma unroll
+    for (int k = 0; k < E; ++k) v += f(x[k], at + k);
+    share.add(s, step, v);
   });
   __syncthreads();
-  const int n = (row.vocab + TILE - 1) / TILE * SW;
-  unsigned long long mine = 0, total;
-  constexpr int PER = MAX_TILES * SW / SB;
+}
+
+// The first token up to which f(x, token) sums to more than pick(the whole
+// sum), from the shares' sums; -1 where that is 0.
+template <typename R, typename F, typename P>
+SVA_DEV int find(const R& row, SampleLds& s, F f, P pick) {
+  const int tid = (int)threadIdx.x, lane = lane_id(), w = tid / WAVE;
+  constexpr int PER = (SHARES + SB - 1) / SB;
+  const int n = row.steps / STEPS * SW;
+  u64 mine = 0, total;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) mine += PER * tid + k < n ? sums[PER * tid + k] : 0ull;
-  unsigned long long before = upto_u64(mine, s, total) - mine;
+  for (int k = 0; k < PER; ++k) mine += PER * tid + k < n ? s.sums[PER * tid + k] : 0ull;
+  u64 before = upto_u64(mine, s, total) - mine;
   if (total == 0ull) return -1;
-  const unsigned long long target = pick(total);
+  const u64 target = pick(total);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     if (PER * tid + k >= n) continue;
-    const unsigned long long v = sums[PER * tid + k];
-    if (before <= target && before + v > target) s.word[0] = before, s.word[1] = (unsigned long long)(PER * tid + k);
+    const u64 v = s.sums[PER * tid + k];
+    if (before <= target && before + v > target) s.word[0] = before, s.word[1] = (u64)(PER * tid + k);
     before += v;
   }
   __syncthreads();
-  const int at0 = (int)s.word[1];
-  if (w == at0 % SW) {
-    const int at = at0 / SW * TILE + tid * E;
-    float x[E];
-    row.load(at, x);
-    unsigned long long v = of8(at, x), end = v;
-#pragma unroll
-    for (int k = 1; k < WAVE; k <<= 1) {
-      const unsigned long long y = __shfl_up(end, k, WAVE);
-      if (lane >= k) end += y;
-    }
-    unsigned long long before = s.word[0] + end - v;
+  // the share again, a step a wave
+  const int at = (int)s.word[1] * SHARE + w * STEP + lane * E;
+  u64 g[E], v = 0;
+  if (w < STEPS) {
+    const auto x = row.load(at);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-      const unsigned long long g = at + k < row.vocab ? f(x[k], at + k) : 0ull;
-      if (before <= target && before + g > target) s.word[3] = (unsigned long long)(at + k);
-      before += g;
+      g[k] = f(x[k], at + k - row.skip);
+      v += g[k];
+    }
+  }
+  u64 upto = s.word[0] + upto_u64(v, s, total) - v;
+  if (w < STEPS) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      if (upto <= target && upto + g[k] > target) s.word[3] = (u64)(at + k - row.skip);
+      upto += g[k];
     }
   }
   __syncthreads();
   return (int)s.word[3];
 }
 
-template <int DT, bool VEC>
+// A cut in the order of falling logits, with exact weights throughout:
+// composites of at least the answer are kept.  MASS false: the first `want`
+// elements.  MASS true: of the elements of at least `from`, those with less
+// than `share` of their sum before them (one at least).
+template <bool MASS, typename R>
+SVA_DEV u64 exact_cut(const R& row, SampleLds& s, u64 from, u64 want, double share) {
+  const int tid = (int)threadIdx.x;
+  u64 above = 0;  // counts or weights before the current range:
+  int bin = -1;   // elements of this bin whose key's bits from `bits` on are `prefix`
+  int bits = 32;
+  uint32_t prefix = 0;
+  auto inside = [&](float x, uint32_t key, int token) {
+    return row.has(token) && composite(key, (uint32_t)token) >= from && (bin < 0 || bin_of(row, x) == bin) &&
+           (bits == 32 || key >> bits == prefix);
+  };
+  for (int level = 0;; ++level) {
+    __syncthreads();
+    for (int k = tid; k < BINS; k += SB) s.count[k] = 0u, s.hist[k] = 0ull;
+    __syncthreads();
+    const int next = bits >= 11 ? bits - 11 : 0;
+    row.template each<HEAVY>([&](int, int at, const auto& x) {
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float v = number(x[k]);
+        const uint32_t key = f2key(v);
+        if (!inside(v, key, at + k)) continue;
+        const int i = level == 0 ? bin_of(row, v) : (int)(key >> next) & ((1 << (bits - next)) - 1);
+        atomicAdd(&s.count[i], 1u);
+        if (MASS) atomicAdd(&s.hist[i], row.weight(v));
+      }
+    });
+    __syncthreads();
+    // falling order: bins of level 0 rise, keys fall
+    u64 mine[PT], sum = 0, total;
+    int at[PT];
+#pragma unroll
+    for (int k = 0; k < PT; ++k) {
+      at[k] = level == 0 ? PT * tid + k : BINS - 1 - (PT * tid + k);
+      mine[k] = MASS ? s.hist[at[k]] : s.count[at[k]];
+      sum += mine[k];
+    }
+    u64 before = above + upto_u64(sum, s, total) - sum;
+    if (MASS && level == 0) want = share_of(share, total);
+    if (total == 0ull) return from;  // (no weight at all)
+    // the range in which the want-th unit lies
+#pragma unroll
+    for (int k = 0; k < PT; ++k) {
+      if (before < want && before + mine[k] >= want) s.word[0] = before, s.word[1] = (u64)at[k];
+      before += mine[k];
+    }
+    __syncthreads();
+    above = s.word[0];
+    const int hit = (int)s.word[1];
+    const uint32_t count = s.count[hit];
+    if (level == 0) bin = hit;
+    else prefix = (bits == 32 ? 0u : prefix << (bits - next)) | (uint32_t)hit, bits = next;
+    if (count <= CAP) {
+      __syncthreads();
+      if (tid == 0) s.n[0] = 0u;
+      __syncthreads();
+      row.template each<HEAVY>([&](int, int at, const auto& x) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          const float v = number(x[k]);
+          const uint32_t key = f2key(v);
+          if (inside(v, key, at + k)) s.list[0][atomicAdd(&s.n[0], 1u)] = composite(key, (uint32_t)(at + k));
+        }
+      });
+      __syncthreads();
+      const int n = (int)count;
+      const u64* sorted = sort_list(s, s.list[0], n);
+      sum = 0;
+#pragma unroll
+      for (int k = 0; k < PT; ++k) {
+        const int i = PT * tid + k;
+        mine[k] = i >= n ? 0ull : (MASS ? row.weight(key2f(composite_key(sorted[i]))) : 1ull);
+        sum += mine[k];
+      }
+      u64 upto = above + upto_u64(sum, s, total) - sum;
+#pragma unroll
+      for (int k = 0; k < PT; ++k) {
+        if (upto < want && upto + mine[k] >= want) s.word[2] = sorted[PT * tid + k];
+        upto += mine[k];
+      }
+      __syncthreads();
+      return s.word[2];
+    }
+    if (level > 0 && bits == 0) {
+      // more ties than are sorted: of equal weights, the lowest tokens
+      const u64 each = MASS ? row.weight(key2f(prefix)) : 1ull;
+      const u64 n = (want - above + each - 1) / each;  // (each > 0: the range holds the want-th unit)
+      const auto tie = [&](float x, int token) {
+        return f2key(number(x)) == prefix && row.has(token) && composite(prefix, (uint32_t)token) >= from ? 1ull : 0ull;
+      };
+      sum_shares(row, s, tie);
+      return composite(prefix, (uint32_t)find(row, s, tie, [&](u64) { return n - 1; }));
+    }
+  }
+}
+
+// What is asked of one row.
+struct Wish {
+  bool few, share;  // cut by top_k, by top_p
+  u64 top_k;
+  double top_p, u;
+};
+
+template <typename R>
+SVA_DEV int draw(const R& row, SampleLds& s, const Wish& wish, u64 thr) {
+  return find(
+      row, s,
+      [&](float x, int token) {
+        const u64 w = row.weight(number(x));
+        return w >= row.least_w && composite(f2key(number(x)), (uint32_t)token) >= thr ? w : 0ull;
+      },
+      [&](u64 total) {
+        const double t = __builtin_floor((double)total * wish.u);
+        const u64 v = t >= 0.0 ? (u64)__builtin_fmin(t, 9.0e18) : 0ull;
+        return v < total ? v : total - 1;
+      });
+}
+
+// No cut: every weight.
+template <typename R>
+SVA_DEV int draw_all(const R& row, SampleLds& s, const Wish& wish) {
+  __syncthreads();
+  Share share;
+  row.template each<HEAVY>([&](int step, int, const auto& x) {
+    u64 v = 0, w[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) w[k] = row.raw_weight(x[k]);
+    if (row.least_w) {
+#pragma unroll
+      for (int k = 0; k < E; ++k) v += w[k] - kRaw >= row.least_w ? w[k] - kRaw : 0ull;
+    } else {
+#pragma unroll
+      for (int k = 0; k < E; ++k) v += w[k];
+      v -= E * kRaw;
+    }
+    share.add(s, step, v);
+  });
+  __syncthreads();
+  return draw(row, s, wish, 0ull);
+}
+
+template <typename R>
+SVA_DEV int exact_draw(const R& row, SampleLds& s, const Wish& wish) {
+  u64 thr = 0ull;
+  if (wish.few) thr = exact_cut<false>(row, s, thr, wish.top_k, 0.0);
+  if (wish.share) thr = exact_cut<true>(row, s, thr, 0ull, wish.top_p);
+  sum_shares(row, s, [&](float x, int token) {
+    const u64 w = row.weight(number(x));
+    return w >= row.least_w && composite(f2key(number(x)), (uint32_t)token) >= thr ? w : 0ull;
+  });
+  return draw(row, s, wish, thr);
+}
+
+// The kept elements of a sorted list into the shares' sums.
+template <typename R>
+SVA_DEV void add_kept(const R& row, SampleLds& s, const u64* sorted, int n) {
+  for (int i = (int)threadIdx.x; i < n; i += SB) {
+    const u64 c = sorted[i], w = row.weight(key2f(composite_key(c)));
+    if (w >= row.least_w) atomicAdd(&s.sums[((int)composite_index(c) + row.skip) / SHARE], w);
+  }
+  __syncthreads();
+}
+
+// top_k of a few: as many of the threads' largest lie in the first bins up to
+// one, so that the cut does too: their elements are listed (-2: too many).
+template <typename R>
+SVA_DEV int draw_few(const R& row, SampleLds& s, const Wish& wish, float largest) {
+  const int tid = (int)threadIdx.x;
+  for (int k = tid; k < BINS; k += SB) s.count[k] = 0u;
+  for (int k = tid; k < row.steps / STEPS * SW; k += SB) s.sums[k] = 0ull;
+  if (tid == 0) s.n[2] = 0u, s.word[1] = ~0ull;
+  __syncthreads();
+  if (largest > -INFINITY) atomicAdd(&s.count[bin_of(row, largest)], 1u);
+  __syncthreads();
+  u64 mine = 0, total;
+#pragma unroll
+  for (int k = 0; k < PT; ++k) mine += s.count[PT * tid + k];
+  const u64 end = upto_u64(mine, s, total);
+  if (end - mine < wish.top_k && end >= wish.top_k) s.word[1] = (u64)(PT * tid + PT - 1);
+  __syncthreads();
+  if (s.word[1] == ~0ull) return -2;
+  const float most = s.word[1] >= BINS - 1 ? INFINITY : (float)((int)s.word[1] + 1);
+  if (most == INFINITY) return -2;
+  Marks marks;
+  row.template each<LIGHT>([&](int step, int, const auto& x) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int k = 0; k < E; ++k) mask |= row.below(x[k]) < most ? 1u << k : 0u;  // (no NaN, and no -inf)
+    marks.add(row, s, step, mask);
+  });
+  __syncthreads();
+  const int n = (int)s.n[2];
+  if (n > CAP) return -2;
+  for (int i = tid; i < n; i += SB) s.list[0][i] = composite(f2key(number(row.at((int)s.many[i]))), s.many[i]);
+  const u64* sorted = sort_list(s, s.list[0], n);
+  int kept = (int)wish.top_k;
+  if (wish.share) kept = within_share(row, s, sorted, kept, 0ull, 0ull, wish.top_p);
+  add_kept(row, s, sorted, kept);
+  return draw(row, s, wish, sorted[kept - 1]);
+}
+
+// Any cut, by a histogram of counts and fp32 weights in one word, exact weights
+// beside it (-1: no token at all, -2: it does not decide, -3: weights
+// cannot be taken so).  fp32 weights are rounded
+// to a unit of 2^-20 of the largest at least: a cut as `near` to the end of its
+// bin as their sums may be off takes the next one in.
+//
+// The bins begin above the largest of the first group, by as much as the rest
+// is not expected to pass (what does is in the first bin), so that the pass
+// that finds the largest of all is this one (256 rows of 131072: 13 us less).
+template <typename R>
+SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int bits, Largest& largest) {
+  const int tid = (int)threadIdx.x;
+  {
+    Largest some;
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) some.add(0, row.load(R::place(k)));
+    float top = block_max(s, some.x);
+    if (top == -INFINITY) {
+      row.template each<LIGHT>([&](int, int, const auto& x) { some.add(0, x); });
+      top = block_max(s, some.x);
+    }
+    row.ref = top + 256.0f / row.per;
+    largest = Largest();
+  }
+  const int low_bits = 63 - bits;  // (counts of up to 2^bits above them)
+  const u64 one = 1ull << low_bits, rest = one - 1;
+  const float unit = __builtin_amdgcn_ldexpf(1.0f, min(30, low_bits - 1 - bits));
+  const float hi_slope = (float)slope, lo_slope = (float)(slope - (double)hi_slope);
+  for (bool again = false;; again = true) {
+    for (int k = tid; k < BINS; k += SB) s.hist[k] = 0ull;
+    if (tid < 3) s.n[tid] = 0u;
+    if (tid == 0) s.word[4] = 0ull;
+    __syncthreads();
+    row.template each<HEAVY>([&](int step, int, const auto& x) {
+      if (!again) largest.add(step, x);
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float v = number(x[k]);
+        u64 add = one;
+        if (wish.share) {
+          const float d = fminf(v - row.ref, 0.0f);
+          add |= (uint32_t)__builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(d, hi_slope, d * lo_slope)), unit, 0.5f);
+        }
+        atomicAdd(&s.hist[bin_of(row, v)], add);
+      }
+    });
+    if (again) break;
+    row.begin(block_max(s, largest.x));
+    if (row.M == -INFINITY) return -1;
+    if (!row.plain()) return -3;
+    if (!wish.share || row.M <= row.ref) break;
+    row.ref = row.M;
+  }
+  __syncthreads();
+  if (tid == SB - 1) s.hist[BINS - 1] -= (u64)(row.steps / STEPS * GROUP - row.vocab) * one;  // (what is no token)
+  __syncthreads();
+  u64 mine[PT], first = 0, total;
+#pragma unroll
+  for (int k = 0; k < PT; ++k) first += mine[k] = s.hist[PT * tid + k];
+  first = upto_u64(first, s, total) - first;
+  int last = BINS;  // the bin of the top_k-th
+  u64 before_last = 0, sum = total & rest;
+  if (wish.few) {
+    u64 before = first;
+#pragma unroll
+    for (int k = 0; k < PT; ++k) {
+      if ((before >> low_bits) < wish.top_k && (before + mine[k]) >> low_bits >= wish.top_k)
+        s.word[0] = before, s.word[1] = (u64)(PT * tid + k);
+      before += mine[k];
+    }
+    __syncthreads();
+    last = (int)s.word[1];
+    before_last = (s.word[0] >> low_bits);
+    const u64 in = s.hist[last];
+    if ((in >> low_bits) > CAP) return -2;
+    sum = (s.word[0] & rest) +
+          (u64)((double)(in & rest) * (double)(wish.top_k - before_last) / (double)((in >> low_bits)));
+  }
+  int lo = last, hi = last;  // bins in which the cut may fall
+  if (wish.share) {
+    const u64 want = share_of(wish.top_p, sum > 0 ? sum : 1);
+    u64 before = first;
+#pragma unroll
+    for (int k = 0; k < PT; ++k) {
+      if ((before & rest) < want && ((before + mine[k]) & rest) >= want)
+        s.word[4] = (u64)(PT * tid + k), s.word[5] = before & rest;
+      before += mine[k];
+    }
+    __syncthreads();
+    lo = hi = min((int)s.word[4], last == BINS ? BINS - 1 : last);
+    const u64 near = sum >> 14, begin = s.word[5], end = begin + (s.hist[lo] & rest);
+    if (lo > 0 && want < begin + near) --lo;
+    if (hi < BINS - 1 && hi < last && want + near > end) ++hi;
+  }
+  const bool joined = hi == last;  // the bin of the top_k-th is among them
+  const int n_list = (int)((s.hist[lo] >> low_bits)) + (hi > lo ? (int)((s.hist[hi] >> low_bits)) : 0);
+  const int n_last = last < BINS ? (int)((s.hist[last] >> low_bits)) : 0;
+  if (n_list > CAP) return -2;
+  __syncthreads();
+  // The elements of these bins (list 0) and of the top_k-th's (list 1), and
+  // exact weights: `above` them, and of all before the top_k-th's bin, `whole`.
+  const bool need_whole = wish.share && !joined;
+  const float lo_f = lo == 0 ? -INFINITY : (float)lo, end_f = hi == BINS - 1 ? INFINITY : (float)(hi + 1);
+  const float last_f = last == BINS ? INFINITY : (float)last, behind_f = last >= BINS - 1 ? INFINITY : (float)(last + 1);
+  const bool by_list = wish.few && wish.top_k <= MANY - CAP;
+  if (by_list)
+    for (int k = tid; k < row.steps / STEPS * SW; k += SB) s.sums[k] = 0ull;
+  // (what is no token lies in the last bin)
+  const bool last_bin = hi == BINS - 1 || last == BINS - 1;
+  const auto in_lists = [&](float b) { return (b >= lo_f && b < end_f) || (b >= last_f && b < behind_f); };
+  const auto tokens = [&](int at) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int k = 0; k < E; ++k) mask |= row.has(at + k) ? 1u << k : 0u;
+    return mask;
+  };
+  __syncthreads();
+  u64 above = 0, whole = 0;
+  Marks marks;
+  if (by_list) {
+    // not many in all: listed, and the weights are theirs alone
+    row.template each<LIGHT>([&](int step, int at, const auto& x) {
+      uint32_t mask = 0;
+#pragma unroll
+      for (int k = 0; k < E; ++k) mask |= row.below(x[k]) < behind_f ? 1u << k : 0u;
+      if (last_bin) mask = tokens(at);
+      marks.add(row, s, step, mask);
+    });
+  } else if (last == BINS && !last_bin) {
+    // top_p alone: the whole sum, and what lies above the bins
+    Share share;
+    row.template each<HEAVY>([&](int step, int, const auto& x) {
+      u64 w[E], here = 0, kept = 0;
+      uint32_t mask = 0;
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float b = row.below(x[k]);  // (a NaN compares with nothing)
+        w[k] = row.raw_weight(x[k]);
+        whole += w[k];
+        mask |= b >= lo_f && b < end_f ? 1u << k : 0u;
+        w[k] = b < lo_f ? w[k] - kRaw : 0ull;
+        here += w[k];
+      }
+      whole -= E * kRaw;
+      above += kept = here;
+      if (row.least_w) {
+        kept = 0;
+#pragma unroll
+        for (int k = 0; k < E; ++k) kept += w[k] >= row.least_w ? w[k] : 0ull;
+      }
+      marks.add(row, s, step, mask);
+      share.add(s, step, kept);
+    });
+  } else {
+    Share share;
+    row.template each<HEAVY>([&](int step, int at, const auto& x) {
+      float v[E], b[E];
+      bool weigh = need_whole;
+      uint32_t mask = 0;
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        v[k] = number(x[k]);
+        b[k] = fminf(row.below(v[k]), (float)(BINS - 1));
+        weigh = weigh || b[k] < lo_f;
+        mask |= in_lists(b[k]) ? 1u << k : 0u;
+      }
+      u64 kept = 0;
+      if (__any(weigh)) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          const u64 w = row.weight(v[k]);
+          whole += b[k] < last_f ? w : 0ull;
+          above += b[k] < lo_f ? w : 0ull;
+          kept += b[k] < lo_f && w >= row.least_w ? w : 0ull;
+        }
+      }
+      if (last_bin) mask &= tokens(at);
+      marks.add(row, s, step, mask);
+      share.add(s, step, kept);
+    });
+  }
+  __syncthreads();
+  for (int i = tid, all = (int)s.n[2]; i < all; i += SB) {
+    const uint32_t token = s.many[i];
+    const float v = number(row.at((int)token)), b = fminf(row.below(v), (float)(BINS - 1));
+    const u64 c = composite(f2key(v), token);
+    if (b >= lo_f && b < end_f) s.list[0][atomicAdd(&s.n[0], 1u)] = c;
+    else if (b >= last_f) s.list[1][atomicAdd(&s.n[1], 1u)] = c;
+    if (by_list && b < last_f) {
+      const u64 w = row.weight(v);
+      whole += w;
+      if (b < lo_f) {
+        above += w;
+        if (w >= row.least_w) atomicAdd(&s.sums[((int)token + row.skip) / SHARE], w);
+      }
+    }
+  }
+  u64 sums[2];
+  upto_u64(above, s, sums[0]);
+  upto_u64(whole, s, sums[1]);
+  int n = n_list;
+  if (wish.few) {
+    const int of_last = (int)(wish.top_k - before_last);
+    if (joined) {
+      n -= n_last - of_last;
+    } else {
+      const u64* sorted = sort_list(s, s.list[1], n_last);
+      u64 w = 0, all;
+      for (int i = tid; i < of_last; i += SB) w += row.weight(key2f(composite_key(sorted[i])));
+      upto_u64(w, s, all);
+      sums[1] += all;
+    }
+  }
+  const u64* sorted = sort_list(s, s.list[0], n_list);
+  if (wish.share) n = within_share(row, s, sorted, n, sums[0], need_whole ? sums[1] : 0ull, wish.top_p);
+  if (n < 0) return -2;
+  add_kept(row, s, sorted, n);
+  return draw(row, s, wish, sorted[n - 1]);
+}
+
+template <int DT>
 __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
   __shared__ SampleLds s;
   const int tid = (int)threadIdx.x;
   const int64_t b = blockIdx.x;
-  Row<DT, VEC> row;
-  row.p = (const unsigned char*)p.logits + b * p.row_stride * (DT == F32 ? 4 : 2);
+  OddRow<DT> odd;
+  Row<DT>& row = odd;
+  const uintptr_t from = (uintptr_t)p.logits + b * p.row_stride * Row<DT>::ES;
+  row.p = (const unsigned char*)(from & ~(uintptr_t)15);
+  row.skip = (int)(from & 15) / Row<DT>::ES;
   row.vocab = p.vocab;
+  row.steps = (p.vocab + row.skip + GROUP - 1) / GROUP * STEPS;
   row.table = s.table;
-  if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
-  const float T = p.temperature ? p.temperature[b] : p.temperature1;
+  float T = p.temperature ? p.temperature[b] : p.temperature1;
+  T = T > 1e30f ? 1e30f : T;  // (all of them weigh the same)
   const int64_t k = p.top_k ? p.top_k[b] : p.top_k1;
   const float top_p = p.top_p ? p.top_p[b] : p.top_p1;
   const float min_p = fminf(p.min_p ? p.min_p[b] : p.min_p1, 1.0f);
-  const float u = p.uniforms[b];
+  Wish wish;
+  wish.u = p.uniforms[b];
+  wish.few = k > 0 && k < p.vocab;
+  wish.top_k = (u64)k;
+  wish.share = !(top_p >= 1.0f);
+  wish.top_p = top_p;
 
-  float M = -INFINITY;
-  row.each([&](int, int, const float (&x)[E]) {
-#pragma unroll
-    for (int i = 0; i < E; ++i) M = fmaxf(M, x[i]);
-  });
-  M = wave_max(M);
-  if (lane_id() == 0) s.top[tid / WAVE] = M;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < SW; ++w) M = fmaxf(M, s.top[w]);
-  row.M = M;
-  if (M == -INFINITY) {  // no token at all
-    if (tid == 0) p.out[b] = -1;
-    return;
+  row.T = T;
+  const double slope = 1.44269504088896340736 / (double)T;
+  row.rate = 256.0 * slope;
+  row.per = 64.0f / fmaxf(T, 0.25f);
+  row.least_w = (u64)__builtin_ceil((double)fmaxf(min_p, 0.0f) * __builtin_amdgcn_ldexp(1.0, p.point));
+  if (tid < 256) s.table[tid] = exp2((double)tid / 256.0 + (double)p.point);
+  const bool random = !(T <= 0.0f) && k != 1;
+  const bool few = random && wish.few && wish.top_k <= kFew;
+
+  Largest largest;
+  int token = -2;
+  if (!random || few || (!wish.few && !wish.share)) {
+    row.template each<LIGHT>([&](int step, int, const auto& x) { largest.add(step, x); });
+    row.begin(block_max(s, largest.x));
+    row.ref = row.M;
+    if (!random || row.M == -INFINITY) token = -1;
+    else if (!row.plain()) token = -3;
+    else if (few) token = draw_few(row, s, wish, fminf(largest.x, 3.40282347e38f));
+    else token = draw_all(row, s, wish);
   }
-  const auto largest = [&]() {
-    return locate(row, s, [&](float x, int) { return x == M ? 1ull : 0ull; }, [](unsigned long long) { return 0ull; });
-  };
-  int token = -1;
-  if (!(T <= 0.0f) && k != 1) {
-    row.rate = 1.44269504088896340736 / (double)T;
-    row.per = 64.0f / fmaxf(T, 0.25f);
-    row.one = __builtin_amdgcn_ldexp(1.0, p.point);
-    unsigned long long thr = 0ull;
-    if (k > 0 && k < p.vocab) thr = cut<false>(row, s, 0ull, (unsigned long long)k, 0.0);
-    if (!(top_p >= 1.0f)) thr = cut<true>(row, s, thr, 0ull, (double)top_p);
-    token = locate(
-        row, s,
-        [&](float x, int at) {
-          if (composite(f2key(x), (uint32_t)at) < thr) return 0ull;
-          const double w = row.weight(x);
-          return w >= (double)min_p ? row.fixed(w) : 0ull;
-        },
-        [&](unsigned long long total) {
-          const double t = __builtin_floor((double)total * (double)u);
-          const unsigned long long v = t >= 0.0 ? (unsigned long long)__builtin_fmin(t, 9.0e18) : 0ull;
-          return v < total ? v : total - 1;
-        });
+  if (token == -2) token = draw_cut(row, s, wish, slope, p.vocab_bits, largest);
+  if (token == -2) token = exact_draw(row, s, wish);
+  if (token == -3) token = exact_draw(odd, s, wish);
+  if (token < 0 && row.M > -INFINITY) {  // the largest, the lowest of equal ones
+    __syncthreads();
+    if (tid == 0) s.n[1] = 0xFFFFFFFFu;
+    __syncthreads();
+    if (fminf(largest.x, 3.40282347e38f) == row.M) {
+      const int at = row.place(largest.step);
+      const Raw<DT> x = row.load(at);
+      uint32_t first = 0;
+#pragma unroll
+      for (int i = E - 1; i >= 0; --i) first = number(x[i]) == row.M ? (uint32_t)(at + i - row.skip) : first;
+      atomicMin(&s.n[1], first);
+    }
+    __syncthreads();
+    token = (int)s.n[1];
   }
-  if (token < 0) token = largest();
   if (tid == 0) p.out[b] = token;
 }
 
 template <int DT>
-int launch(const SampleParams& p, int64_t rows, bool vec, hipStream_t stream) {
-  if (vec) hipLaunchKernelGGL((sample_kernel<DT, true>), dim3((unsigned)rows), dim3(SB), 0, stream, p);
-  else hipLaunchKernelGGL((sample_kernel<DT, false>), dim3((unsigned)rows), dim3(SB), 0, stream, p);
+int launch(const SampleParams& p, int64_t rows, hipStream_t stream) {
+  hipLaunchKernelGGL((sample_kernel<DT>), dim3((unsigned)rows), dim3(SB), 0, stream, p);
   SVA_CHECK_LAUNCH("sample_kernel");
   return SVA_OK;
 }
@@ -391,6 +922,7 @@ extern "C" int sva_sample_tokens(const void* logits, int dtype, int64_t row_stri
   SVA_REQUIRE(logits && uniforms && tokens, "sva_sample_tokens: null pointer");
   SVA_REQUIRE(dtype >= 0 && dtype <= 2, "sva_sample_tokens: bad dtype");
   SVA_REQUIRE(n_rows > 0 && n_rows < (1ll << 31) && vocab > 0 && row_stride >= 0, "sva_sample_tokens: bad sizes");
+  SVA_REQUIRE((uintptr_t)logits % (dtype == F32 ? 4 : 2) == 0, "sva_sample_tokens: logits are not aligned");
   SVA_UNSUPPORTED(vocab <= kMaxVocab, "sva_sample_tokens: %lld tokens (at most %lld)", (long long)vocab,
                   (long long)kMaxVocab);
   SampleParams p;
@@ -409,10 +941,9 @@ extern "C" int sva_sample_tokens(const void* logits, int dtype, int64_t row_stri
   p.out = tokens;
   int bits = 0;
   while ((1ll << bits) < vocab) ++bits;
-  p.point = std::min(46, 63 - bits - 1);
-  const int64_t es = dtype == F32 ? 4 : 2;
-  const bool vec = ((uintptr_t)logits & 15u) == 0 && row_stride * es % 16 == 0;
-  if (dtype == F32) return launch<F32>(p, n_rows, vec, (hipStream_t)stream);
-  if (dtype == BF16) return launch<BF16>(p, n_rows, vec, (hipStream_t)stream);
-  return launch<F16>(p, n_rows, vec, (hipStream_t)stream);
+  p.point = std::min(46, 62 - bits);
+  p.vocab_bits = bits;
+  if (dtype == F32) return launch<F32>(p, n_rows, (hipStream_t)stream);
+  if (dtype == BF16) return launch<BF16>(p, n_rows, (hipStream_t)stream);
+  return launch<F16>(p, n_rows, (hipStream_t)stream);
 }
