@@ -696,6 +696,8 @@ int sva_paged_attention(const void *q, int dtype, int64_t q_seq_stride, int64_t 
  *              -1: nothing was changed for this sequence, whose pages together
  *              with those asked for by the ones before it are not there, whose
  *              table is too short, or whose count is negative
+ * workspace: sva_pages_reserve_workspace_bytes(...) bytes, 16-byte aligned (0:
+ * none is needed, and it may be NULL; the same for sva_pages_fork).
  */
 size_t sva_pages_reserve_workspace_bytes(int64_t n_seq, int64_t n_pages);
 int sva_pages_reserve(int32_t *tables, int64_t table_stride, int64_t max_pages, int64_t *seq_lens, int64_t n_seq,

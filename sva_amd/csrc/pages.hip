@@ -151,42 +151,42 @@ SVA_DEV int64_t block_upto(int64_t v, int64_t* scratch, int64_t& total) {
   return v + before;
 }
 
-// Pages [0, pages) in order, 16 waves x 16 x 64 at a time: `pick(page, refs)`
-// says which count, `got(page, rank)` is told the rank of each of those; ends
-// behind the page of rank `enough` - 1 or soon after.  Returns how many counted.
+// 16 waves x 16 x 64 pages from `base` on: this thread's counts (behind the
+// end: of the last page).
 constexpr int PR = 16;  // pages a thread at a time
+SVA_DEV int64_t my_page(int64_t base) { return base + (int64_t)(threadIdx.x / WAVE) * (WAVE * PR) + lane_id(); }
+SVA_DEV void load_refs(const int32_t* refs, int64_t pages, int64_t base, int32_t (&r)[PR]) {
+#pragma unroll
+  for (int k = 0; k < PR; ++k) r[k] = refs[min(my_page(base) + k * WAVE, pages - 1)];
+}
+// Of these pages, those of which pick(page, refs) says so: got(page, rank) is
+// told their ranks from `found` on, which grows by their number.
 template <typename Pick, typename Got>
-SVA_DEV int64_t rank_pages(const int32_t* refs, int64_t pages, int64_t enough, int64_t* scratch, Pick pick, Got got) {
+SVA_DEV void rank_chunk(const int32_t (&r)[PR], int64_t pages, int64_t base, int64_t* scratch, int64_t& found, Pick pick,
+                        Got got) {
   const int lane = lane_id(), w = (int)threadIdx.x / WAVE;
-  int64_t found = 0;
-  for (int64_t base = 0; base < pages && found < enough; base += HB * PR) {
-    const int64_t mine = base + (int64_t)w * (WAVE * PR) + lane;
-    int32_t r[PR];
+  uint64_t mask[PR];
+  int count = 0;
 #pragma unroll
-    for (int k = 0; k < PR; ++k) r[k] = refs[min(mine + k * WAVE, pages - 1)];
-    uint64_t mask[PR];
-    int count = 0;
-#pragma unroll
-    for (int k = 0; k < PR; ++k) {
-      mask[k] = __ballot(mine + k * WAVE < pages && pick(mine + k * WAVE, r[k]));
-      count += (int)__popcll(mask[k]);
-    }
-    __syncthreads();
-    if (lane == 0) scratch[w] = count;
-    __syncthreads();
-    int64_t rank = found;
-#pragma unroll
-    for (int k = 0; k < HW; ++k) {
-      rank += k < w ? scratch[k] : 0;
-      found += scratch[k];
-    }
-#pragma unroll
-    for (int k = 0; k < PR; ++k) {
-      if (mask[k] >> lane & 1ull) got(mine + k * WAVE, rank + (int)__popcll(mask[k] & ((1ull << lane) - 1)));
-      rank += (int)__popcll(mask[k]);
-    }
+  for (int k = 0; k < PR; ++k) {
+    const int64_t page = my_page(base) + k * WAVE;
+    mask[k] = __ballot(page < pages && pick(page, r[k]));
+    count += (int)__popcll(mask[k]);
   }
-  return found;
+  __syncthreads();
+  if (lane == 0) scratch[w] = count;
+  __syncthreads();
+  int64_t rank = found;
+#pragma unroll
+  for (int k = 0; k < HW; ++k) {
+    rank += k < w ? scratch[k] : 0;
+    found += scratch[k];
+  }
+#pragma unroll
+  for (int k = 0; k < PR; ++k) {
+    if (mask[k] >> lane & 1ull) got(my_page(base) + k * WAVE, rank + (int)__popcll(mask[k] & ((1ull << lane) - 1)));
+    rank += (int)__popcll(mask[k]);
+  }
 }
 
 // What a sequence asks for: pages up to it (its own among them), the table
@@ -196,16 +196,27 @@ struct Ask {
   int32_t begin, leaves;
 };
 
+// Up to these sizes what the sequences ask for and get is kept in LDS.
+constexpr int64_t kFewSeqs = 1024, kFewPages = 8192;
+inline bool reserve_small(int64_t n_seq, int64_t n_pages) { return n_seq <= kFewSeqs && n_pages <= kFewPages; }
+
 // Room for counts[s] more rows behind every sequence, one workgroup: what each
 // asks for, in order; the free pages by rank; their way into the tables.  A
 // last page that others hold too is left to them where rows are to go into it:
 // the pair (it, the new one) is to be copied.  Bound by the latency of its
-// steps: the scan of refs ends with the last page that is wanted.
+// steps: the scan of refs, whose first chunk is under way from the start, ends
+// with the last page that is wanted.
+template <bool SMALL>
 __global__ void __launch_bounds__(HB) pages_reserve_kernel(HoldParams p, const int64_t* counts, int64_t each, Ask* asks,
                                                            int32_t* list, int64_t* first_rows, int32_t* src,
                                                            int32_t* dst) {
   __shared__ int64_t scratch[HW];
+  __shared__ Ask lds_asks[SMALL ? kFewSeqs : 1];
+  __shared__ int32_t lds_list[SMALL ? kFewPages : 1];
+  if (SMALL) asks = lds_asks, list = lds_list;
   const int tid = (int)threadIdx.x;
+  int32_t r[PR];
+  load_refs(p.refs, p.pages, 0, r);
   int64_t wanted = 0;
   for (int64_t s0 = 0; s0 < p.S; s0 += HB) {
     const int64_t s = s0 + tid;
@@ -228,13 +239,15 @@ __global__ void __launch_bounds__(HB) pages_reserve_kernel(HoldParams p, const i
     wanted += total;
     if (s < p.S) asks[s] = a;
   }
-  const int64_t found =
-      wanted == 0 ? 0
-                  : rank_pages(
-                        p.refs, p.pages, wanted, scratch, [](int64_t, int32_t r) { return r == 0; },
-                        [&](int64_t page, int64_t rank) {
-                          if (rank < wanted) list[rank] = (int32_t)page;
-                        });
+  int64_t found = 0;
+  for (int64_t base = 0; base < p.pages && found < wanted; base += HB * PR) {
+    if (base > 0) load_refs(p.refs, p.pages, base, r);
+    rank_chunk(
+        r, p.pages, base, scratch, found, [](int64_t, int32_t n) { return n == 0; },
+        [&](int64_t page, int64_t rank) {
+          if (rank < wanted) list[rank] = (int32_t)page;
+        });
+  }
   __syncthreads();
   // page r of the list: its sequence by bisection
   for (int64_t r = tid; r < (wanted < found ? wanted : found); r += HB) {
@@ -264,8 +277,8 @@ __global__ void __launch_bounds__(HB) pages_reserve_kernel(HoldParams p, const i
 }
 
 // Row s of the tables becomes a fork of row sources[s] (-1: of none, it is
-// freed; itself or no row: as it is).  First into `next`, since a source may
-// be replaced itself; the counts follow by integer atomics.
+// freed; itself or no row: as it is).  All are read before any is written, since
+// a source may be replaced itself; the counts follow by integer atomics.
 SVA_DEV bool forked(const HoldParams& p, const int64_t* sources, int64_t s, int64_t& from) {
   from = sources[s];
   return from != s && from >= -1 && from < p.S;
@@ -275,18 +288,44 @@ SVA_DEV int64_t held_by(const HoldParams& p, int64_t s) {
   return n < p.M ? n : p.M;
 }
 
-__global__ void __launch_bounds__(256) pages_fork_kernel(HoldParams p, const int64_t* sources, int32_t* next,
-                                                         int64_t* next_lens) {
-  const int64_t s = blockIdx.x, j = (int64_t)blockIdx.y * 256 + threadIdx.x;
+// Entry j of row s: what it becomes (counted), by `next`; whether row s changes.
+template <typename Next>
+SVA_DEV void fork_entry(const HoldParams& p, const int64_t* sources, int64_t s, int64_t j, Next next) {
   int64_t from;
-  if (j >= p.M || !forked(p, sources, s, from)) return;
-  if (j == 0) next_lens[s] = from < 0 ? 0 : p.lens[from];
+  if (!forked(p, sources, s, from)) return;
   int id = -1;
   if (from >= 0 && j < held_by(p, from)) id = p.tables[from * p.table_stride + j];
-  next[s * p.M + j] = id;
   if (is_page(p, id)) atomicAdd(p.refs + id, 1);
   const int old = j < held_by(p, s) ? p.tables[s * p.table_stride + j] : -1;
   if (is_page(p, old)) atomicSub(p.refs + old, 1);
+  next(id, from < 0 ? 0 : p.lens[from]);
+}
+
+// Tables of few entries: one workgroup, an entry a thread, the new ones in
+// registers meanwhile (4 x 33: 2.9 us, 4.3 in two launches; 64 x 33 as three
+// entries a thread 7.5, 6.1).
+constexpr int64_t kFewEntries = HB;
+__global__ void __launch_bounds__(HB) pages_fork_few_kernel(HoldParams p, const int64_t* sources) {
+  const int s = (int)threadIdx.x / (int)p.M, j = (int)threadIdx.x % (int)p.M;
+  int id = -1;
+  int64_t len = 0;
+  bool moved = false;
+  if (s < p.S) fork_entry(p, sources, s, j, [&](int page, int64_t n) { id = page, len = n, moved = true; });
+  __syncthreads();
+  if (!moved) return;
+  p.tables[s * p.table_stride + j] = id;
+  if (j == 0) p.lens[s] = len;
+}
+
+// Others: into `next` first, then back.
+__global__ void __launch_bounds__(256) pages_fork_kernel(HoldParams p, const int64_t* sources, int32_t* next,
+                                                         int64_t* next_lens) {
+  const int64_t s = blockIdx.x, j = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  if (j >= p.M) return;
+  fork_entry(p, sources, s, j, [&](int page, int64_t n) {
+    next[s * p.M + j] = page;
+    if (j == 0) next_lens[s] = n;
+  });
 }
 
 __global__ void __launch_bounds__(256) pages_forked_kernel(HoldParams p, const int64_t* sources, const int32_t* next,
@@ -301,23 +340,33 @@ __global__ void __launch_bounds__(256) pages_forked_kernel(HoldParams p, const i
 // The pages in use moved to the front: with U of them, the k-th one in use
 // from U on goes to the k-th free one below U.  One workgroup counts, ranks
 // and moves the refs; the tables follow, the pages themselves are copied by
-// the caller's pairs.  Bound by the latency of two scans of refs.
+// the caller's pairs.  Bound by the latency of the scans.
 __global__ void __launch_bounds__(HB) pages_compact_kernel(int32_t* refs, int64_t pages, int32_t* to, int32_t* src,
                                                            int32_t* dst, int64_t n_pairs, int32_t* used) {
   __shared__ int64_t scratch[HW];
-  const auto in_use = [](int64_t, int32_t r) { return r > 0; };
-  const int64_t U = rank_pages(
-      refs, pages, pages + 1, scratch,
-      [&](int64_t page, int32_t r) {
-        to[page] = (int32_t)page;  // (also of free pages, which a table may still name)
-        return r > 0;
-      },
-      [](int64_t, int64_t) {});
-  const int64_t moves = rank_pages(
-      refs, U, pages + 1, scratch, [](int64_t, int32_t r) { return r <= 0; },
-      [&](int64_t page, int64_t k) { dst[k] = (int32_t)page; });
-  rank_pages(
-      refs + U, pages - U, pages + 1, scratch, in_use, [&](int64_t page, int64_t k) { src[k] = (int32_t)(page + U); });
+  int64_t U = 0, holes = 0, moves = 0;
+  int32_t r[PR];
+  for (int64_t base = 0; base < pages; base += HB * PR) {
+    load_refs(refs, pages, base, r);
+    rank_chunk(
+        r, pages, base, scratch, U,
+        [&](int64_t page, int32_t n) {
+          to[page] = (int32_t)page;  // (also of free pages, which a table may still name)
+          return n > 0;
+        },
+        [](int64_t, int64_t) {});
+  }
+  for (int64_t base = 0; base < pages; base += HB * PR) {
+    if (pages > HB * PR) load_refs(refs, pages, base, r);
+    if (base < U)
+      rank_chunk(
+          r, pages, base, scratch, holes, [&](int64_t page, int32_t n) { return page < U && n <= 0; },
+          [&](int64_t page, int64_t k) { dst[k] = (int32_t)page; });
+    if (base + HB * PR > U)
+      rank_chunk(
+          r, pages, base, scratch, moves, [&](int64_t page, int32_t n) { return page >= U && n > 0; },
+          [&](int64_t page, int64_t k) { src[k] = (int32_t)page; });
+  }
   __syncthreads();
   for (int64_t k = threadIdx.x; k < n_pairs; k += HB) {
     if (k < moves) {
@@ -457,7 +506,7 @@ extern "C" int sva_pages_copy(void* pool, int64_t n_pages, int64_t page_stride_b
 }
 
 extern "C" size_t sva_pages_reserve_workspace_bytes(int64_t n_seq, int64_t n_pages) {
-  if (n_seq <= 0 || n_pages <= 0) return 0;
+  if (n_seq <= 0 || n_pages <= 0 || reserve_small(n_seq, n_pages)) return 0;
   return (size_t)n_seq * sizeof(Ask) + (size_t)n_pages * sizeof(int32_t);
 }
 
@@ -470,19 +519,23 @@ extern "C" int sva_pages_reserve(int32_t* tables, int64_t table_stride, int64_t 
   SVA_REQUIRE(sizes_ok(n_seq, max_pages, n_pages), "sva_pages_reserve: bad sizes");
   SVA_REQUIRE(page_rows_ok(page_rows), "sva_pages_reserve: %lld rows a page are no power of two from 16 to 1024",
               (long long)page_rows);
-  SVA_REQUIRE(workspace && ((uintptr_t)workspace & 15u) == 0 &&
-                  workspace_bytes >= sva_pages_reserve_workspace_bytes(n_seq, n_pages),
-              "sva_pages_reserve: a workspace of %zu bytes required", sva_pages_reserve_workspace_bytes(n_seq, n_pages));
+  const size_t need = sva_pages_reserve_workspace_bytes(n_seq, n_pages);
+  SVA_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need),
+              "sva_pages_reserve: a workspace of %zu bytes required", need);
+  const HoldParams p = hold(tables, table_stride, seq_lens, refs, n_seq, max_pages, n_pages, page_rows);
   Ask* asks = (Ask*)workspace;
-  hipLaunchKernelGGL(pages_reserve_kernel, dim3(1), dim3(HB), 0, (hipStream_t)stream,
-                     hold(tables, table_stride, seq_lens, refs, n_seq, max_pages, n_pages, page_rows), counts, count, asks,
-                     (int32_t*)(asks + n_seq), first_rows, src, dst);
+  if (need == 0)
+    hipLaunchKernelGGL((pages_reserve_kernel<true>), dim3(1), dim3(HB), 0, (hipStream_t)stream, p, counts, count, nullptr,
+                       nullptr, first_rows, src, dst);
+  else
+    hipLaunchKernelGGL((pages_reserve_kernel<false>), dim3(1), dim3(HB), 0, (hipStream_t)stream, p, counts, count, asks,
+                       (int32_t*)(asks + n_seq), first_rows, src, dst);
   SVA_CHECK_LAUNCH("pages_reserve_kernel");
   return SVA_OK;
 }
 
 extern "C" size_t sva_pages_fork_workspace_bytes(int64_t n_seq, int64_t max_pages) {
-  if (n_seq <= 0 || max_pages <= 0) return 0;
+  if (n_seq <= 0 || max_pages <= 0 || n_seq * max_pages <= kFewEntries) return 0;
   return (size_t)n_seq * sizeof(int64_t) + (size_t)n_seq * (size_t)max_pages * sizeof(int32_t);
 }
 
@@ -494,10 +547,15 @@ extern "C" int sva_pages_fork(int32_t* tables, int64_t table_stride, int64_t max
   SVA_REQUIRE(sizes_ok(n_seq, max_pages, n_pages), "sva_pages_fork: bad sizes");
   SVA_REQUIRE(page_rows_ok(page_rows), "sva_pages_fork: %lld rows a page are no power of two from 16 to 1024",
               (long long)page_rows);
-  SVA_REQUIRE(workspace && ((uintptr_t)workspace & 15u) == 0 &&
-                  workspace_bytes >= sva_pages_fork_workspace_bytes(n_seq, max_pages),
-              "sva_pages_fork: a workspace of %zu bytes required", sva_pages_fork_workspace_bytes(n_seq, max_pages));
+  const size_t need = sva_pages_fork_workspace_bytes(n_seq, max_pages);
+  SVA_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 15u) == 0 && workspace_bytes >= need),
+              "sva_pages_fork: a workspace of %zu bytes required", need);
   const HoldParams p = hold(tables, table_stride, seq_lens, refs, n_seq, max_pages, n_pages, page_rows);
+  if (need == 0) {
+    hipLaunchKernelGGL(pages_fork_few_kernel, dim3(1), dim3(HB), 0, (hipStream_t)stream, p, sources);
+    SVA_CHECK_LAUNCH("pages_fork_few_kernel");
+    return SVA_OK;
+  }
   int64_t* next_lens = (int64_t*)workspace;
   int32_t* next = (int32_t*)(next_lens + n_seq);
   const dim3 grid((unsigned)n_seq, (unsigned)((max_pages + 255) / 256));

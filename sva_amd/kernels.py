@@ -1128,16 +1128,18 @@ def _check_page_shape(page_rows: int, dim: int) -> None:
                          f"{page_rows} rows of {dim}")
 
 
-def _check_pool(pool: torch.Tensor) -> tuple[int, int, int, int, int]:
-    """(pages, G, P, D, elements between pages) of one layer's pool."""
+def _check_pool(pool: torch.Tensor, layers: bool = False) -> tuple[int, int, int, int, int]:
+    """(pages, G, P, D, elements between pages) of one layer's pool (of any number's, where `layers`)."""
 
-    if pool.dim() != 5 or pool.shape[1] != 2:
-        raise ValueError(f"a pool must be [pages, 2, G, P, D], got {tuple(pool.shape)}")
-    n, _, kv_heads, rows, dim = pool.shape
-    stride = pool.stride()
+    shape, stride = pool.shape, pool.stride()
+    if layers and len(shape) == 6:
+        shape, stride = shape[1:], stride[1:]
+    if len(shape) != 5 or shape[1] != 2:
+        raise ValueError(f"a pool must be [{'(layers,) ' if layers else ''}pages, 2, G, P, D], got {tuple(pool.shape)}")
+    n, _, kv_heads, rows, dim = shape
     if stride[4] != 1 or stride[3] != dim or stride[2] != rows * dim or stride[1] != kv_heads * rows * dim or \
             stride[0] < 2 * kv_heads * rows * dim:
-        raise ValueError(f"every page of a pool must be contiguous, got {tuple(pool.shape)} of strides {stride}")
+        raise ValueError(f"every page of a pool must be contiguous, got {tuple(pool.shape)} of strides {pool.stride()}")
     _check_page_shape(rows, dim)
     return n, kv_heads, rows, dim, stride[0]
 
@@ -1230,8 +1232,10 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, s
     _inference_only("paged_attention", q, pool)
     device = _same_device(q, pool, tables, seq_lens)
     dtype = dtype_code(q)
-    # tokens before heads: the model's projection takes the result without a copy
-    out = torch.empty(n_seq, q_len, heads, dim, device=device, dtype=out_dtype or q.dtype).transpose(1, 2)
+    if q_len == 1:
+        out = torch.empty(n_seq, heads, 1, dim, device=device, dtype=out_dtype or q.dtype)
+    else:  # tokens before heads: the model's projection takes the result without a copy
+        out = torch.empty(n_seq, q_len, heads, dim, device=device, dtype=out_dtype or q.dtype).transpose(1, 2)
     if out.numel() == 0:
         return out
     n_keys = entries * page_rows if n_keys is None else min(int(n_keys), entries * page_rows)
@@ -1279,17 +1283,17 @@ def pages_reserve(tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tens
     else:
         each, counts = int(counts), None
     device = _same_device(tables, seq_lens, refs, counts)
-    first_rows = torch.empty(n_seq, device=device, dtype=torch.int64)
-    src = torch.empty(n_seq, device=device, dtype=torch.int32)
-    dst = torch.empty_like(src)
+    first_rows = seq_lens.new_empty(n_seq)
+    src, dst = refs.new_empty((2, n_seq)).unbind()
     if n_seq == 0:
         return first_rows, src, dst
     if n_pages == 0 or entries == 0:
         return first_rows.fill_(-1), src.fill_(-1), dst.fill_(-1)
-    ws = torch.empty(lib().sva_pages_reserve_workspace_bytes(n_seq, n_pages), device=device, dtype=torch.uint8)
+    ws_bytes = lib().sva_pages_reserve_workspace_bytes(n_seq, n_pages)
+    ws = torch.empty(ws_bytes, device=device, dtype=torch.uint8) if ws_bytes else None
     _call(device, "sva_pages_reserve", tables.data_ptr(), table_stride, entries, seq_lens.data_ptr(), n_seq,
           refs.data_ptr(), n_pages, page_rows, ptr(counts), each, first_rows.data_ptr(), src.data_ptr(), dst.data_ptr(),
-          ws.data_ptr(), ws.numel())
+          ptr(ws), ws_bytes)
     return first_rows, src, dst
 
 
@@ -1305,9 +1309,10 @@ def pages_fork(tables: torch.Tensor, seq_lens: torch.Tensor, refs: torch.Tensor,
     device = _same_device(tables, seq_lens, refs, _seq_tensor("sources", sources, n_seq))
     if n_seq == 0 or n_pages == 0 or entries == 0:
         return
-    ws = torch.empty(lib().sva_pages_fork_workspace_bytes(n_seq, entries), device=device, dtype=torch.uint8)
+    ws_bytes = lib().sva_pages_fork_workspace_bytes(n_seq, entries)
+    ws = torch.empty(ws_bytes, device=device, dtype=torch.uint8) if ws_bytes else None
     _call(device, "sva_pages_fork", tables.data_ptr(), table_stride, entries, seq_lens.data_ptr(), n_seq,
-          refs.data_ptr(), n_pages, page_rows, sources.data_ptr(), ws.data_ptr(), ws.numel())
+          refs.data_ptr(), n_pages, page_rows, sources.data_ptr(), ptr(ws), ws_bytes)
 
 
 def pages_compact(tables: torch.Tensor, refs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -1318,9 +1323,8 @@ def pages_compact(tables: torch.Tensor, refs: torch.Tensor) -> tuple[torch.Tenso
 
     n_seq, entries, table_stride, n_pages = _check_holders(tables, None, refs, 16)
     device = _same_device(tables, refs)
-    src = torch.empty(n_pages // 2, device=device, dtype=torch.int32)
-    dst = torch.empty_like(src)
-    used = torch.empty(1, device=device, dtype=torch.int32)
+    src, dst = refs.new_empty((2, n_pages // 2)).unbind()
+    used = refs.new_empty(1)
     if n_pages == 0:
         return src, dst, used.zero_()
     if n_seq == 0 or entries == 0:  # (refs may still say that pages are in use)
@@ -1337,10 +1341,10 @@ def pages_copy(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None
     the pool are skipped.  A page must be in one pair alone, unless as the source
     of several."""
 
-    layers = pool if pool.dim() == 6 else pool.unsqueeze(0)
-    if layers.dim() != 6 or layers.shape[0] == 0:
-        raise ValueError(f"a pool must be [pages, 2, G, P, D] or [layers, pages, 2, G, P, D], got {tuple(pool.shape)}")
-    n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(layers[0])
+    n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(pool, layers=True)
+    n_layers, layer_stride = (pool.shape[0], pool.stride(0)) if pool.dim() == 6 else (1, 0)
+    if n_layers == 0:
+        raise ValueError("a pool of no layers")
     if src.dim() != 1 or src.dtype != torch.int32 or not src.is_contiguous() or dst.shape != src.shape or \
             dst.dtype != torch.int32 or not dst.is_contiguous():
         raise ValueError(f"src and dst must be int32 [pairs], got {src.dtype} {tuple(src.shape)} and {dst.dtype} "
@@ -1350,8 +1354,8 @@ def pages_copy(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None
     if src.numel() == 0 or n_pages == 0:
         return
     size = pool.element_size()
-    _call(device, "sva_pages_copy", pool.data_ptr(), n_pages, page_stride * size, layers.shape[0],
-          layers.stride(0) * size, 2 * kv_heads * page_rows * dim * size, src.data_ptr(), dst.data_ptr(), src.numel())
+    _call(device, "sva_pages_copy", pool.data_ptr(), n_pages, page_stride * size, n_layers,
+          layer_stride * size, 2 * kv_heads * page_rows * dim * size, src.data_ptr(), dst.data_ptr(), src.numel())
 
 
 # ---------------------------------------------------------------------------

@@ -72,7 +72,7 @@ class Cache:
 
 
 @pytest.mark.parametrize("seed,n_seq,entries,pages,P", [(1, 1, 3, 2, 16), (2, 5, 6, 17, 16), (3, 8, 4, 40, 32), (4, 40, 9, 200, 16),
-                                                        (5, 3, 300, 700, 16)])
+                                                        (5, 3, 300, 700, 16), (6, 3, 6000, 9000, 16), (7, 1500, 2, 2000, 16)])
 def test_random_steps(device, seed, n_seq, entries, pages, P):
     """Growth that is granted or not, forks of forks, swaps, frees and compactions, in any order."""
     rng = random.Random(seed)

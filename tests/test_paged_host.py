@@ -148,10 +148,10 @@ def test_c_entries_refuse():
                           ({26: 10}, "workspace"), ({17: 0}, "sizes"), ({11: 1 << 30, 13: 1 << 40}, "too many")):
         refused("sva_paged_attention", with_(attend, changes), text)
     refused("sva_paged_attention", with_(attend, {14: 70000}), "tokens", 3)
-    reserve = [p, 4, 4, p, 1, p, 4, 16, None, 1, p, p, p, p, 1 << 20, None]
+    reserve = [p, 4, 4, p, 1, p, 40000, 16, None, 1, p, p, p, p, 1 << 20, None]
     for changes, text in (({0: None}, "null"), ({2: 0}, "sizes"), ({7: 0}, "rows a page"), ({13: odd}, "workspace"), ({14: 8}, "workspace")):
         refused("sva_pages_reserve", with_(reserve, changes), text)
-    fork = [p, 4, 4, p, 1, p, 4, 16, p, p, 1 << 20, None]
+    fork = [p, 40000, 40000, p, 1, p, 4, 16, p, p, 1 << 20, None]
     for changes, text in (({8: None}, "null"), ({4: 0}, "sizes"), ({7: 100}, "rows a page"), ({10: 8}, "workspace")):
         refused("sva_pages_fork", with_(fork, changes), text)
     compact = [p, 4, 4, 1, p, 4, p, p, p, p, 1 << 20, None]
@@ -171,5 +171,6 @@ def test_workspaces():
     size = lib.sva_paged_attention_workspace_bytes
     assert size(0, 9, 3, 1, 64, 1, 100000) == size(1, 9, 2, 1, 64, 1, 100000) == size(1, 9, 3, 1, 64, 1, 256) == 0
     assert 256 < size(1, 9, 3, 1, 64, 0, 100000) < 1 << 24
-    assert lib.sva_pages_reserve_workspace_bytes(3, 10) >= 3 * 16 + 40
-    assert lib.sva_pages_fork_workspace_bytes(3, 10) >= 3 * 8 + 120 and lib.sva_pages_compact_workspace_bytes(7) >= 28
+    assert lib.sva_pages_reserve_workspace_bytes(3, 10) == 0 and lib.sva_pages_reserve_workspace_bytes(3, 10000) >= 3 * 16 + 40000
+    assert lib.sva_pages_reserve_workspace_bytes(2000, 10) >= 2000 * 16 + 40 and lib.sva_pages_fork_workspace_bytes(3, 10) == 0
+    assert lib.sva_pages_fork_workspace_bytes(3, 10000) >= 3 * 8 + 120000 and lib.sva_pages_compact_workspace_bytes(7) >= 28
