@@ -12,6 +12,8 @@ import importlib
 
 _EXPORTS = {
     "FourBitCache": "cache4",
+    "PagedCache": "paged",
+    "generate": "paged",
     "SVAArtifactBundle": "artifacts",
     "SVALayerArtifacts": "artifacts",
     "load_sva_artifact_bundle": "artifacts",

@@ -29,7 +29,7 @@ import torch
 from torch import nn
 from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
 
-from . import cache4, inverted, kernels
+from . import cache4, inverted, kernels, paged
 from .artifacts import SVAArtifactBundle, SVALayerArtifacts, load_sva_artifact_bundle
 from .stats import SVAStats
 
@@ -150,7 +150,12 @@ class SVALlamaAttention(nn.Module):
         v = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         cos, sin = position_embeddings
         q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        pages = paged.layer_of(past_key_values, self.layer_idx)
         held = cache4.layer_of(past_key_values, self.layer_idx)
+        if pages is not None:
+            kernels._inference_only("attention over a paged cache", q, k, v)
+            out = self._attention_paged(q, k, v, pages, attention_mask)
+            return self.o_proj(out.transpose(1, 2).contiguous().reshape(*input_shape, -1)), None
         if held is not None or (q.shape[2] > 1 and self.serving.prompt_attention == "dense"):
             kernels._inference_only("attention over a 4-bit cache" if held is not None else "prompt_attention", q, k, v)
         if held is not None:
@@ -293,6 +298,34 @@ class SVALlamaAttention(nn.Module):
 
         return kernels.prompt_attention(query, keys, values, k_len, self.scaling, mask=mask, seq_offsets=seq_offsets,
                                         seq_lens=seq_lens)
+
+    # query rows a KV head up to which pages are read in place: each 16 of them read every row again
+    _PAGED_ROWS = 64
+
+    def _attention_paged(self, query, key, value, held, attention_mask):
+        """Attention over every row of a cache held in pages (paged.PagedCache), to which the new rows key / value
+        [B, G, T, D] are written: no lookup.  A few tokens read the pages in place; a prompt takes its own rows, or, like
+        calls with a mask, the rows read back, by dense attention."""
+
+        kernels.require_device(query, key, value)
+        batch, _, q_len, _ = query.shape
+        start = held.length
+        held.append(key, value)
+        if attention_mask is None and (start > 0 or q_len == 1) and q_len * self.num_key_value_groups <= self._PAGED_ROWS:
+            return kernels.paged_attention(query, held.pool, held.cache.tables, held.cache.lens, self.scaling,
+                                           n_keys=held.length)
+        key, value = (key.contiguous(), value.contiguous()) if start == 0 else held.read()
+        k_len = key.shape[2]
+        mask = None if attention_mask is None else attention_mask[..., :q_len, :k_len]
+        if batch == 1:
+            return self._dense_prompt(query, key[0], value[0], k_len, mask)
+        # packed: the rows of KV head g and sequence b at b * G * N of g's, contiguous caches of N rows
+        rows = (batch - 1) * key.shape[1] * k_len + k_len
+        packed = [x.as_strided((x.shape[1], rows, x.shape[3]), (x.stride(1), x.stride(2), 1), x.storage_offset())
+                  for x in (key, value)]
+        lens = torch.full((batch,), k_len, device=query.device, dtype=torch.int64)
+        offsets = torch.arange(batch, device=query.device, dtype=torch.int64) * (key.shape[1] * k_len)
+        return self._dense_prompt(query, *packed, k_len, mask, offsets, lens)
 
     def _attention_cache4(self, query, key, value, held, attention_mask):
         """sva_attention over a cache held in 4 bits (cache4.FourBitCache):
