@@ -47,7 +47,7 @@ struct PagedParams {
   Pages c;
   const int64_t* lens;
   int64_t N;  // rows of a sequence behind this are not read
-  int H, G, Q, D, row_tiles, splits;
+  int n_seq, H, G, Q, D, row_tiles, splits;
   int chunk;  // keys per workgroup, a multiple of STEP
   float scaling;
   float* sums;  // join.h
@@ -159,9 +159,12 @@ __global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP)) paged_att
   __shared__ uint32_t odd_rows;
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
   const int m16 = lane & 15, qd = lane >> 4;
-  const int split = (int)blockIdx.x;
-  const int y = (int)blockIdx.y;
-  const int rt = y % p.row_tiles, g = y / p.row_tiles % p.G, b = y / (p.row_tiles * p.G);
+  // (the row tiles over the same keys are eight workgroups apart: on one XCD, whose L2 they share)
+  const uint32_t id = blockIdx.x, unit = id / (uint32_t)(kXcds * p.row_tiles) * kXcds + id % kXcds;
+  const int rt = (int)(id / kXcds % (uint32_t)p.row_tiles);
+  const int split = (int)(unit % (uint32_t)p.splits);
+  const int g = (int)(unit / (uint32_t)p.splits % (uint32_t)p.G), b = (int)(unit / (uint32_t)p.splits / (uint32_t)p.G);
+  if (b >= p.n_seq) return;
   const int grp = p.H / p.G;
   int64_t off;
   const int len = (int)seq_keys(p.lens, nullptr, p.N, p.N, b, off);
@@ -445,20 +448,26 @@ __global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP)) paged_att
   }
 }
 
-// Keys per workgroup: enough workgroups to fill the card, eight times as many
-// where sequences may differ in length (the last to end is then a small part
-// of the call: 32 sequences of up to 131072 keys 383 us with a quarter as many,
-// 330 with half, 297); at most 384 ranges (each costs a row of partial sums),
-// of at least 256 keys, or of 1024 where those fill the card already (4 tokens
-// of 8 x 32768 keys, 12 x 64: 64 us, 71 with 256).  A range of 128 KB is one
-// workgroup's business, whatever follows: a CU takes 50 GB/s, and a second
-// launch 3 us (500 keys of 9 x 64: 7.4 us in one range, 9.2 in two; 1000 10.8
-// in one, 9.2 in four).
+// Keys per workgroup.  A CU holds three workgroups of rows of up to 256 bytes
+// (K and V), two of 512, one of more.
+//  * A range of 128 KB is one workgroup's business, whatever follows: a CU takes
+//    50 GB/s, and a second launch 3 us (500 keys of 9 x 64: 7.4 us in one range,
+//    9.2 in two; 1000 10.8 in one, 9.2 in four).
+//  * One sequence: one round of the places of the CUs where that makes ranges of
+//    up to 1024 keys, else two (100000 keys of 9 x 64 fp32: 42 us in 471
+//    workgroups on 512 places, 53 in 294, 48 in 783).
+//  * Sequences that may differ in length: eight times the card's workgroups (the
+//    last to end is then a small part of the call: 32 sequences of up to 131072
+//    keys 297 us, 330 with a quarter as many), but ranges of 1024 keys where those
+//    fill it already (16 x 8192 keys of 16 x 128: 40 us, 48 with 384).
+// At most 384 ranges (each costs a row of partial sums), of at least 256 keys.
 int64_t chunk_keys(int64_t n_seq, int64_t groups, int64_t row_bytes, int64_t n_keys) {
   if (n_keys * row_bytes <= 131072) return (n_keys + STEP - 1) / STEP * STEP;
-  const int64_t want = std::min<int64_t>(384, std::max<int64_t>(1, (n_seq > 1 ? 8192 : 1024) / groups));
-  const int64_t least = std::max<int64_t>(2 * STEP, std::min<int64_t>(8 * STEP, n_keys * groups / 768));
-  return (std::max<int64_t>(least, (n_keys + want - 1) / want) + STEP - 1) / STEP * STEP;
+  const int64_t places = row_bytes <= 256 ? 768 : (row_bytes <= 512 ? 512 : 256), work = n_keys * groups;
+  const int64_t most = n_seq > 1 ? 8192 : (work <= 1024 * places ? places : 2 * places);
+  const int64_t want = std::min<int64_t>(384, std::max<int64_t>(1, most / groups));
+  const int64_t least = n_seq > 1 ? std::min<int64_t>(8 * STEP, work / (row_bytes <= 256 ? 768 : 256)) : 0;
+  return (std::max<int64_t>(std::max<int64_t>(least, 2 * STEP), (n_keys + want - 1) / want) + STEP - 1) / STEP * STEP;
 }
 
 int64_t row_tiles(int64_t H, int64_t G, int64_t Q) { return (H / G * Q + TR - 1) / TR; }
@@ -512,8 +521,6 @@ extern "C" int sva_paged_attention(const void* q, int dtype, int64_t q_seq_strid
                   n_seq * H * Q < (1ll << 31) && keys < (1ll << 31) - 1024,
               "sva_paged_attention: too many items or keys");
   const int64_t tiles = row_tiles(H, G, Q);
-  SVA_UNSUPPORTED(n_seq * G * tiles <= 65535, "sva_paged_attention: %lld tokens of %lld sequences in one call",
-                  (long long)Q, (long long)n_seq);
   const size_t need = sva_paged_attention_workspace_bytes(n_seq, H, G, Q, D, dtype, keys);
   SVA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "sva_paged_attention: workspace of %zu bytes required",
               need);
@@ -533,6 +540,7 @@ extern "C" int sva_paged_attention(const void* q, int dtype, int64_t q_seq_strid
   p.c.bits = page_bits(page_rows);
   p.lens = seq_lens;
   p.N = keys;
+  p.n_seq = (int)n_seq;
   p.H = (int)H;
   p.G = (int)G;
   p.Q = (int)Q;
@@ -548,7 +556,10 @@ extern "C" int sva_paged_attention(const void* q, int dtype, int64_t q_seq_strid
   p.o_bs = out_seq_stride;
   p.o_hs = out_head_stride;
   p.o_ts = out_tok_stride;
-  const dim3 grid((unsigned)p.splits, (unsigned)(n_seq * G * tiles));
+  const int64_t units = n_seq * G * p.splits, blocks = (units + kXcds - 1) / kXcds * kXcds * tiles;
+  SVA_UNSUPPORTED(blocks < (1ll << 31), "sva_paged_attention: %lld tokens of %lld sequences in one call", (long long)Q,
+                  (long long)n_seq);
+  const dim3 grid((unsigned)blocks);
   int rc;
   if (dtype == F32) rc = launch<F32>(p, grid, (hipStream_t)stream);
   else if (dtype == BF16) rc = launch<BF16>(p, grid, (hipStream_t)stream);

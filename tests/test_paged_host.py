@@ -147,7 +147,6 @@ def test_c_entries_refuse():
                           ({18: 4}, "head_dim"), ({8: 17}, "rows a page"), ({5: odd}, "16-byte"), ({25: None}, "workspace"),
                           ({26: 10}, "workspace"), ({17: 0}, "sizes"), ({11: 1 << 30, 13: 1 << 40}, "too many")):
         refused("sva_paged_attention", with_(attend, changes), text)
-    refused("sva_paged_attention", with_(attend, {14: 70000}), "tokens", 3)
     reserve = [p, 4, 4, p, 1, p, 40000, 16, None, 1, p, p, p, p, 1 << 20, None]
     for changes, text in (({0: None}, "null"), ({2: 0}, "sizes"), ({7: 0}, "rows a page"), ({13: odd}, "workspace"), ({14: 8}, "workspace")):
         refused("sva_pages_reserve", with_(reserve, changes), text)
