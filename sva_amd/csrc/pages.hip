@@ -28,22 +28,24 @@ struct RowsParams {
   int64_t n_rows;
   int G, chunks;  // 16-byte chunks of a row
   int es;
+  uint32_t blocks;  // of one head's K or V
 };
 
 // One 16-byte chunk of a row a thread, a head's rows one after another as they
-// lie in the page; y: (sequence, head, K or V).  WRITE: into the pages, else
+// lie in the page, `blocks` workgroups for each (sequence, head, K or V).  WRITE: into the pages, else
 // out of them (rows without a page read as 0).  VEC: rows in memory are whole
 // aligned 16-byte words.  Bound by memory where there are many rows, by the
 // latency of page number and row where there are few.
 template <bool WRITE, bool VEC>
 __global__ void __launch_bounds__(256) page_rows_kernel(RowsParams p) {
-  const int kv = (int)blockIdx.y & 1, g = (int)(blockIdx.y >> 1) % p.G, b = (int)(blockIdx.y >> 1) / p.G;
+  const uint32_t y = blockIdx.x / p.blocks;
+  const int kv = (int)(y & 1), g = (int)((y >> 1) % (uint32_t)p.G), b = (int)((y >> 1) / (uint32_t)p.G);
   const int64_t first = p.first_rows[b];
   unsigned char* rows = (kv ? p.values : p.keys) + b * p.kv_bs + g * p.kv_hs;
   const int64_t rowb = (int64_t)p.chunks * 16;
   const int64_t inside = (((int64_t)(kv * p.G + g)) << p.c.bits) * rowb;
   const int64_t total = p.n_rows * p.chunks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+  for (int64_t i = (int64_t)(blockIdx.x % p.blocks) * 256 + threadIdx.x; i < total; i += (int64_t)p.blocks * 256) {
     const int64_t t = (uint64_t)i / (uint32_t)p.chunks;
     const int ch = (int)(i - t * p.chunks);
     const int64_t n = first + t;
@@ -427,8 +429,7 @@ int rows(const char* name, const void* keys, const void* values, int kv_dtype, i
   SVA_REQUIRE(((uintptr_t)pool & 15u) == 0 && page_stride * es % 16 == 0 && page_stride >= 2 * G * page_rows * D,
               "%s: pages are not 16-byte aligned blocks of 2 x G x rows x head_dim elements", name);
   SVA_REQUIRE(n_pages < (1ll << 31) && max_pages < (1ll << 31) && n_rows < (1ll << 40), "%s: too many pages or rows", name);
-  SVA_UNSUPPORTED(n_seq <= 32767 && G <= 32767 && n_seq * G <= 32767, "%s: %lld sequences of %lld heads in one call", name,
-                  (long long)n_seq, (long long)G);
+  SVA_REQUIRE(n_seq < (1ll << 31) && G < (1ll << 20), "%s: too many sequences or heads", name);
   RowsParams p;
   p.c.pool = (unsigned char*)const_cast<void*>(pool);
   p.c.page_bytes = page_stride * es;
@@ -450,7 +451,12 @@ int rows(const char* name, const void* keys, const void* values, int kv_dtype, i
   const bool vec = (((uintptr_t)keys | (uintptr_t)values) & 15u) == 0 && p.kv_bs % 16 == 0 && p.kv_hs % 16 == 0 &&
                    p.kv_rs % 16 == 0;
   SVA_REQUIRE(WRITE || vec, "%s: outputs are not 16-byte aligned rows", name);
-  const dim3 grid((unsigned)std::min<int64_t>((n_rows * p.chunks + 255) / 256, 4096), (unsigned)(2 * n_seq * G));
+  // (4096 workgroups for a head, fewer where that would be more than a grid holds)
+  const int64_t heads = 2 * n_seq * G;
+  const int64_t blocks = std::min<int64_t>({(n_rows * p.chunks + 255) / 256, 4096, ((1ll << 31) - 1) / heads});
+  SVA_UNSUPPORTED(blocks > 0, "%s: %lld sequences of %lld heads in one call", name, (long long)n_seq, (long long)G);
+  p.blocks = (uint32_t)blocks;
+  const dim3 grid((unsigned)(blocks * heads));
   if (vec) hipLaunchKernelGGL((page_rows_kernel<WRITE, true>), grid, dim3(256), 0, (hipStream_t)stream, p);
   else hipLaunchKernelGGL((page_rows_kernel<WRITE, false>), grid, dim3(256), 0, (hipStream_t)stream, p);
   SVA_CHECK_LAUNCH("page_rows_kernel");

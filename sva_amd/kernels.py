@@ -1323,10 +1323,11 @@ def pages_compact(tables: torch.Tensor, refs: torch.Tensor) -> tuple[torch.Tenso
 
     n_seq, entries, table_stride, n_pages = _check_holders(tables, None, refs, 16)
     device = _same_device(tables, refs)
-    src, dst = refs.new_empty((2, n_pages // 2)).unbind()
+    pairs = n_pages // 2
+    src, dst = refs.new_empty((2, max(1, pairs))).unbind()
     used = refs.new_empty(1)
-    if n_pages == 0:
-        return src, dst, used.zero_()
+    if pairs == 0:  # (no page, or one, which stays where it is)
+        return src[:0], dst[:0], used.copy_((refs > 0).sum()) if n_pages else used.zero_()
     if n_seq == 0 or entries == 0:  # (refs may still say that pages are in use)
         tables, n_seq, entries, table_stride = torch.full((1, 1), -1, device=device, dtype=torch.int32), 1, 1, 1
     ws = torch.empty(lib().sva_pages_compact_workspace_bytes(n_pages), device=device, dtype=torch.uint8)

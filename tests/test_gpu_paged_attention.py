@@ -221,6 +221,28 @@ def test_write_and_read(device, G, D, P, dtype, T):
     assert torch.equal(again.view(torch.uint8), pool.view(torch.uint8))
 
 
+def test_many_sequences(device):
+    """More (sequence, head) pairs than a grid's second dimension holds."""
+    from sva_amd import kernels
+
+    n, G, D, P = 20000, 4, 8, 16
+    gen = torch.Generator(device=device).manual_seed(2)
+    pool = kernels.pages_alloc(n, G, P, D, device, F32)
+    tables = torch.randperm(n, device=device, generator=gen).int()[:, None]
+    lens = torch.arange(n, device=device) % P + 1
+    keys, values = (torch.randn(n, G, P, D, device=device, generator=gen) for _ in range(2))
+    kernels.paged_write(keys, values, pool, tables, torch.zeros(n, device=device, dtype=torch.int64))
+    back = kernels.paged_read(pool, tables, torch.zeros(n, device=device, dtype=torch.int64), P)
+    assert torch.equal(back[0], keys) and torch.equal(back[1], values)
+    q = torch.randn(n, G, 1, D, device=device, generator=gen)
+    got = kernels.paged_attention(q, pool, tables, lens, 0.3)
+    s = (q.double() @ keys.double().transpose(-1, -2) * 0.3).masked_fill(torch.arange(P, device=device) >= lens[:, None, None, None],
+                                                                        -float("inf"))
+    want = torch.softmax(s, -1) @ values.double()
+    # scores of 8 products and 16 weights and sums: (2 (8 + 4) + 16 + 16) 2^-24 of at most 16 values' size, scores under 30
+    assert (got.double() - want).abs().max() <= 30 * 56 * 2.0 ** -24 * values.abs().max()
+
+
 def test_beyond_32_bits(device):
     """Pages, and elements between pages, past 2^32."""
     from sva_amd import kernels

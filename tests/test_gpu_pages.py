@@ -193,6 +193,9 @@ def test_empty_pools(device):
     assert k.pages_reserve(tables, lens, none, 1, 16)[0].tolist() == [-1, -1]
     k.pages_fork(tables, lens, none, ints(device, [1, 0]), 16)
     assert k.pages_compact(tables, none)[2].tolist() == [0]
+    for n in (0, 3):  # one page
+        src, dst, used = k.pages_compact(tables, ints(device, [n], torch.int32))
+        assert used.tolist() == [min(n, 1)] and src.shape == dst.shape == (0,)
     refs = ints(device, [0, 1, 0], torch.int32)
     assert k.pages_compact(tables[:0], refs)[2].tolist() == [1] and refs.tolist() == [1, 0, 0]
 

@@ -139,7 +139,7 @@ def test_c_entries_refuse():
                           ({9: 264}, "head_dim"), ({14: 24}, "rows a page"), ({14: 8}, "rows a page"), ({11: odd}, "16-byte"),
                           ({13: 2 * 16 * 64 - 8}, "16-byte"), ({12: 0}, "sizes"), ({6: 0}, "sizes")):
         refused("sva_paged_write", with_(write, changes), text)
-    refused("sva_paged_write", with_(write, {6: 40000}), "sequences", 3)
+    refused("sva_paged_write", with_(write, {6: 1 << 30, 8: 4, 12: 4, 13: 2 * 4 * 16 * 64}), "sequences", 3)
     read = [p, 4, 2 * 16 * 64, 16, p, 4, 4, p, 1, 1, 1, 64, p, p, 1, 64, 64, 64, None]
     refused("sva_paged_read", with_(read, {12: odd}), "16-byte")
     attend = [p, 1, 64, 64, 64, p, 4, 2 * 16 * 64, 16, p, 4, 4000, p, 64000, 1, 1, 1, 1, 64, one, p, 1, 64, 64, 64, p, 1 << 20, None]
