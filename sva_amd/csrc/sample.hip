@@ -83,7 +83,7 @@ struct SampleLds {
   u64 sums[SHARES];   // the kept weights of a share
   u64 list[2][CAP];
   uint32_t many[MANY];
-  u64 scan[SW];
+  u64 scan[2 * SW];
   u64 word[8];
   float top[SW];
   uint32_t n[3];
@@ -92,14 +92,31 @@ struct SampleLds {
 // A NaN is no token's, and infinity the largest number.
 SVA_DEV float number(float x) { return x == x ? fminf(x, 3.40282347e38f) : -INFINITY; }
 
+// x moved N lanes up within its DPP row (0 moves in).
+template <int N>
+SVA_DEV u64 row_shr_u64(u64 x) {
+  return (u64)row_shr0<N>((uint32_t)x) | (u64)row_shr0<N>((uint32_t)(x >> 32)) << 32;
+}
+SVA_DEV u64 readlane_u64(u64 x, int lane) {
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
+         (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32;
+}
+// Inclusive sum over the wave (all lanes active).
+SVA_DEV u64 wave_upto_u64(u64 v) {
+  v += row_shr_u64<1>(v);
+  v += row_shr_u64<2>(v);
+  v += row_shr_u64<4>(v);
+  v += row_shr_u64<8>(v);
+  const u64 a = readlane_u64(v, 15), b = a + readlane_u64(v, 31), c = b + readlane_u64(v, 47);
+  const int row = lane_id() >> 4;
+  return v + (row == 0 ? 0ull : (row == 1 ? a : (row == 2 ? b : c)));
+}
+SVA_DEV u64 wave_sum_u64(u64 v) { return readlane_u64(wave_upto_u64(v), WAVE - 1); }
+
 // Inclusive sum over the workgroup's threads in order; `total` of all.
 SVA_DEV u64 upto_u64(u64 v, SampleLds& s, u64& total) {
   const int lane = lane_id(), w = (int)threadIdx.x / WAVE;
-#pragma unroll
-  for (int k = 1; k < WAVE; k <<= 1) {
-    const u64 x = __shfl_up(v, k, WAVE);
-    if (lane >= k) v += x;
-  }
+  v = wave_upto_u64(v);
   __syncthreads();
   if (lane == WAVE - 1) s.scan[w] = v;
   __syncthreads();
@@ -111,6 +128,16 @@ SVA_DEV u64 upto_u64(u64 v, SampleLds& s, u64& total) {
     total += s.scan[k];
   }
   return v + before;
+}
+// Both summed over the workgroup.
+SVA_DEV void sum_both(u64& a, u64& b, SampleLds& s) {
+  const u64 x = wave_sum_u64(a), y = wave_sum_u64(b);
+  __syncthreads();
+  if (lane_id() == 0) s.scan[(int)threadIdx.x / WAVE] = x, s.scan[SW + (int)threadIdx.x / WAVE] = y;
+  __syncthreads();
+  a = b = 0;
+#pragma unroll
+  for (int k = 0; k < SW; ++k) a += s.scan[k], b += s.scan[SW + k];
 }
 
 // Eight elements as they lie in memory.
@@ -386,10 +413,7 @@ struct Share {
   SVA_DEV void add(SampleLds& s, int step, u64 v) {
     sum += v;
     if (step % STEPS != STEPS - 1) return;
-    if (__ballot(sum != 0ull) != 0ull) {
-#pragma unroll
-      for (int k = 1; k < WAVE; k <<= 1) sum += __shfl_xor(sum, k, WAVE);
-    }
+    sum = wave_sum_u64(sum);
     if (lane_id() == 0) s.sums[step / STEPS * SW + (int)threadIdx.x / WAVE] = sum;
     sum = 0;
   }
@@ -857,9 +881,7 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
       }
     }
   }
-  u64 sums[2];
-  upto_u64(above, s, sums[0]);
-  upto_u64(whole, s, sums[1]);
+  sum_both(above, whole, s);
   int n = n_list;
   if (wish.few) {
     const int of_last = (int)(wish.top_k - before_last);
@@ -870,11 +892,11 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
       u64 w = 0, all;
       for (int i = tid; i < of_last; i += SB) w += row.weight(key2f(composite_key(sorted[i])));
       upto_u64(w, s, all);
-      sums[1] += all;
+      whole += all;
     }
   }
   const u64* sorted = sort_list(s, s.list[0], n_list);
-  if (wish.share) n = within_share(row, s, sorted, n, sums[0], need_whole ? sums[1] : 0ull, wish.top_p);
+  if (wish.share) n = within_share(row, s, sorted, n, above, need_whole ? whole : 0ull, wish.top_p);
   if (n < 0) return -2;
   add_kept(row, s, sorted, n);
   return draw(row, s, wish, sorted[n - 1]);
@@ -912,11 +934,11 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
   row.least_w = (u64)__builtin_ceil((double)fmaxf(min_p, 0.0f) * __builtin_amdgcn_ldexp(1.0, p.point));
   if (tid < 256) s.table[tid] = exp2((double)tid / 256.0 + (double)p.point);
   const bool random = !(T <= 0.0f) && k != 1;
-  const bool few = random && wish.few && wish.top_k <= kFew;
+  const bool cut = random && (wish.few || wish.share), few = cut && wish.few && wish.top_k <= kFew;
 
   Largest largest;
   int token = -2;
-  if (!random || few || (!wish.few && !wish.share)) {
+  if (!cut || few) {
     row.template each<LIGHT>([&](int step, int, const auto& x) { largest.add(step, x); });
     row.begin(block_max(s, largest.x));
     row.ref = row.M;
