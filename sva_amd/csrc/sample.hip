@@ -18,7 +18,7 @@
 //    names the bin in which the cut falls.  (top_k of a few: the bin that top_k
 //    of the threads' largest reach bounds the cut, no histogram is needed);
 //  * for the exact weights above that bin (and of the whole row, for top_p),
-//    summed by shares of 2048 elements, and the bin's elements, which are sorted
+//    summed by shares of 2048 (short rows: 512) elements, and the bin's elements, which are sorted
 //    in LDS: exact weights decide the cut.
 // The share in which the answer lies is gone over again.  What the histogram
 // cannot decide (a bin of more elements than are sorted, logits or a temperature
@@ -44,17 +44,18 @@ typedef unsigned long long u64;
 constexpr int SB = 512;         // threads: two waves a SIMD, whose registers hold several weights in work
 constexpr int SW = SB / WAVE;
 constexpr int E = 8;            // consecutive elements of a thread
-constexpr int STEP = WAVE * E;  // elements that a wave takes at a time,
-constexpr int STEPS = 4;        // this often one after another:
-constexpr int SHARE = STEP * STEPS;
-constexpr int GROUP = SW * SHARE;
+constexpr int STEP = WAVE * E;  // elements that a wave takes at a time, 2^turns times one after another: a share
+constexpr int STEP_BITS = 9;
+static_assert(STEP == 1 << STEP_BITS, "");
+constexpr int TURNS = 2;        // rows of more than kSpread elements; 0: all waves have something of a short row
+constexpr int kSpread = 16384;
 constexpr int LIGHT = 6, HEAVY = 2;  // steps under way of passes that do little, or much, with them
 constexpr int BINS = 2048;
 constexpr int CAP = 2048;       // elements of a bin that are sorted
 constexpr int PT = BINS / SB;    // bins, or elements of a list, of a thread
 static_assert(CAP == BINS, "");
 constexpr int64_t kMaxVocab = 1 << 20;
-constexpr int SHARES = (int)(kMaxVocab / SHARE) + SW;
+constexpr int SHARES = (int)(kMaxVocab >> (STEP_BITS + TURNS)) + SW;
 static_assert(SHARES <= 2 * SB, "");
 constexpr int MANY = 8192;       // tokens that are listed
 constexpr u64 kRaw = 0x4330000000000000ull;  // the bits of 2^52
@@ -154,7 +155,7 @@ template <int DT>
 struct Row {
   static constexpr int ES = DT == F32 ? 4 : 2;
   const unsigned char* p;  // a whole 16-byte word: element `skip` of it is the row's first
-  int skip, vocab, steps;
+  int skip, vocab, steps, turns;
   float M;                 // the largest logit
   float ref, per;          // where the bins begin, and bins for a logit's difference of 1
   double rate, off;        // x rate + off: 256ths of a binade below M
@@ -195,10 +196,12 @@ struct Row {
   SVA_DEV bool plain() const { return T >= 1e-30f && __builtin_fabs(off) <= 268435456.0; }
   SVA_DEV bool has(int token) const { return (uint32_t)token < (uint32_t)vocab; }
   // this thread's elements of a step, in the window
-  static SVA_DEV int place(int step) {
-    const int tid = (int)threadIdx.x;
-    return step / STEPS * GROUP + tid / WAVE * SHARE + step % STEPS * STEP + tid % WAVE * E;
+  SVA_DEV int place(int step) const {
+    const int tid = (int)threadIdx.x, turn = step & ((1 << turns) - 1);
+    return ((((step >> turns) * SW + tid / WAVE) << turns) + turn) * STEP + tid % WAVE * E;
   }
+  SVA_DEV int shares() const { return (steps >> turns) * SW; }
+  SVA_DEV int share_of(int token) const { return (token + skip) >> (STEP_BITS + turns); }
   // f(step, the first one's token, elements), A steps under way (one turn of
   // the loop takes A: registers that are loaded into do not move)
   template <int A, typename F>
@@ -305,7 +308,7 @@ struct Marks {
     i = (uint32_t)__builtin_amdgcn_readlane((int)i, WAVE - 1) + upto - mine;
     for (; bits != 0ull; bits &= bits - 1, ++i) {
       const int k = __builtin_ctzll(bits);
-      if (i < MANY) s.many[i] = (uint32_t)(R::place(step + k / E) + k % E - row.skip);
+      if (i < MANY) s.many[i] = (uint32_t)(row.place(step + k / E) + k % E - row.skip);
     }
   }
 };
@@ -410,11 +413,12 @@ SVA_DEV int within_share(const R& row, SampleLds& s, const u64* sorted, int n, u
 struct Share {
   u64 sum = 0;
 
-  SVA_DEV void add(SampleLds& s, int step, u64 v) {
+  template <typename R>
+  SVA_DEV void add(const R& row, SampleLds& s, int step, u64 v) {
     sum += v;
-    if (step % STEPS != STEPS - 1) return;
+    if ((~step & ((1 << row.turns) - 1)) != 0) return;
     sum = wave_sum_u64(sum);
-    if (lane_id() == 0) s.sums[step / STEPS * SW + (int)threadIdx.x / WAVE] = sum;
+    if (lane_id() == 0) s.sums[(step >> row.turns) * SW + (int)threadIdx.x / WAVE] = sum;
     sum = 0;
   }
 };
@@ -430,7 +434,7 @@ SVA_DEV void sum_shares(const R& row, SampleLds& s, F f) {
     u64 v = 0;
 #pragma unroll
     for (int k = 0; k < E; ++k) v += f(x[k], at + k);
-    share.add(s, step, v);
+    share.add(row, s, step, v);
   });
   __syncthreads();
 }
@@ -441,7 +445,7 @@ template <typename R, typename F, typename P>
 SVA_DEV int find(const R& row, SampleLds& s, F f, P pick) {
   const int tid = (int)threadIdx.x, lane = lane_id(), w = tid / WAVE;
   constexpr int PER = (SHARES + SB - 1) / SB;
-  const int n = row.steps / STEPS * SW;
+  const int n = row.shares();
   u64 mine = 0, total;
 #pragma unroll
   for (int k = 0; k < PER; ++k) mine += PER * tid + k < n ? s.sums[PER * tid + k] : 0ull;
@@ -457,9 +461,10 @@ SVA_DEV int find(const R& row, SampleLds& s, F f, P pick) {
   }
   __syncthreads();
   // the share again, a step a wave
-  const int at = (int)s.word[1] * SHARE + w * STEP + lane * E;
+  const int at = (((int)s.word[1] << row.turns) + w) * STEP + lane * E;
+  const bool mine_too = w >> row.turns == 0;
   u64 g[E], v = 0;
-  if (w < STEPS) {
+  if (mine_too) {
     const auto x = row.load(at);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
@@ -468,7 +473,7 @@ SVA_DEV int find(const R& row, SampleLds& s, F f, P pick) {
     }
   }
   u64 upto = s.word[0] + upto_u64(v, s, total) - v;
-  if (w < STEPS) {
+  if (mine_too) {
 #pragma unroll
     for (int k = 0; k < E; ++k) {
       if (upto <= target && upto + g[k] > target) s.word[3] = (u64)(at + k - row.skip);
@@ -618,7 +623,7 @@ SVA_DEV int draw_all(const R& row, SampleLds& s, const Wish& wish) {
       for (int k = 0; k < E; ++k) v += w[k];
       v -= E * kRaw;
     }
-    share.add(s, step, v);
+    share.add(row, s, step, v);
   });
   __syncthreads();
   return draw(row, s, wish, 0ull);
@@ -641,7 +646,7 @@ template <typename R>
 SVA_DEV void add_kept(const R& row, SampleLds& s, const u64* sorted, int n) {
   for (int i = (int)threadIdx.x; i < n; i += SB) {
     const u64 c = sorted[i], w = row.weight(key2f(composite_key(c)));
-    if (w >= row.least_w) atomicAdd(&s.sums[((int)composite_index(c) + row.skip) / SHARE], w);
+    if (w >= row.least_w) atomicAdd(&s.sums[row.share_of((int)composite_index(c))], w);
   }
   __syncthreads();
 }
@@ -652,7 +657,7 @@ template <typename R>
 SVA_DEV int draw_few(const R& row, SampleLds& s, const Wish& wish, float largest) {
   const int tid = (int)threadIdx.x;
   for (int k = tid; k < BINS; k += SB) s.count[k] = 0u;
-  for (int k = tid; k < row.steps / STEPS * SW; k += SB) s.sums[k] = 0ull;
+  for (int k = tid; k < row.shares(); k += SB) s.sums[k] = 0ull;
   if (tid == 0) s.n[2] = 0u, s.word[1] = ~0ull;
   __syncthreads();
   if (largest > -INFINITY) atomicAdd(&s.count[bin_of(row, largest)], 1u);
@@ -699,7 +704,7 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
   {
     Largest some;
 #pragma unroll
-    for (int k = 0; k < STEPS; ++k) some.add(0, row.load(R::place(k)));
+    for (int k = 0; k < 1 << TURNS; ++k) some.add(0, row.load(row.place(k)));
     float top = block_max(s, some.x);
     if (top == -INFINITY) {
       row.template each<LIGHT>([&](int, int, const auto& x) { some.add(0, x); });
@@ -738,7 +743,7 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
     row.ref = row.M;
   }
   __syncthreads();
-  if (tid == SB - 1) s.hist[BINS - 1] -= (u64)(row.steps / STEPS * GROUP - row.vocab) * one;  // (what is no token)
+  if (tid == SB - 1) s.hist[BINS - 1] -= (u64)(row.steps * SB * E - row.vocab) * one;  // (what is no token)
   __syncthreads();
   u64 mine[PT], first = 0, total;
 #pragma unroll
@@ -790,7 +795,7 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
   const float last_f = last == BINS ? INFINITY : (float)last, behind_f = last >= BINS - 1 ? INFINITY : (float)(last + 1);
   const bool by_list = wish.few && wish.top_k <= MANY - CAP;
   if (by_list)
-    for (int k = tid; k < row.steps / STEPS * SW; k += SB) s.sums[k] = 0ull;
+    for (int k = tid; k < row.shares(); k += SB) s.sums[k] = 0ull;
   // (what is no token lies in the last bin)
   const bool last_bin = hi == BINS - 1 || last == BINS - 1;
   const auto in_lists = [&](float b) { return (b >= lo_f && b < end_f) || (b >= last_f && b < behind_f); };
@@ -835,7 +840,7 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
         for (int k = 0; k < E; ++k) kept += w[k] >= row.least_w ? w[k] : 0ull;
       }
       marks.add(row, s, step, mask);
-      share.add(s, step, kept);
+      share.add(row, s, step, kept);
     });
   } else {
     Share share;
@@ -862,7 +867,7 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
       }
       if (last_bin) mask &= tokens(at);
       marks.add(row, s, step, mask);
-      share.add(s, step, kept);
+      share.add(row, s, step, kept);
     });
   }
   __syncthreads();
@@ -877,7 +882,7 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
       whole += w;
       if (b < lo_f) {
         above += w;
-        if (w >= row.least_w) atomicAdd(&s.sums[((int)token + row.skip) / SHARE], w);
+        if (w >= row.least_w) atomicAdd(&s.sums[row.share_of((int)token)], w);
       }
     }
   }
@@ -913,7 +918,9 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
   row.p = (const unsigned char*)(from & ~(uintptr_t)15);
   row.skip = (int)(from & 15) / Row<DT>::ES;
   row.vocab = p.vocab;
-  row.steps = (p.vocab + row.skip + GROUP - 1) / GROUP * STEPS;
+  row.turns = p.vocab > kSpread ? TURNS : 0;
+  const int group = SB * E << row.turns;
+  row.steps = ((p.vocab + row.skip + group - 1) / group) << row.turns;
   row.table = s.table;
   float T = p.temperature ? p.temperature[b] : p.temperature1;
   T = T > 1e30f ? 1e30f : T;  // (all of them weigh the same)
