@@ -14,21 +14,21 @@
 //
 // A row is one workgroup's, which reads it twice, the first time from memory:
 //  * for M and each thread's largest; where a cut is asked for, for a histogram
-//    over 2048 bins of x too, of counts and fp32 weights in one 64-bit word: it
-//    names the bin in which the cut falls.  (top_k of a few: the bin that top_k
-//    of the threads' largest reach bounds the cut, no histogram is needed);
+//    over 2048 bins of x too, of counts or fp32 weights: it names the bin in
+//    which the cut falls.  (top_k of a few: the bin that top_k of the threads'
+//    largest reach bounds the cut, no histogram is needed);
 //  * for the exact weights above that bin (and of the whole row, for top_p),
-//    summed by shares of 2048 (short rows: 512) elements, and the bin's elements, which are sorted
-//    in LDS: exact weights decide the cut.
+//    summed by shares of 2048 elements (short rows: 512), and the bin's elements,
+//    which are sorted in LDS: exact weights decide the cut.
 // The share in which the answer lies is gone over again.  What the histogram
 // cannot decide (a bin of more elements than are sorted, logits or a temperature
 // at the ends of their range) is done over again with exact weights throughout,
-// bins narrowed by the bits of x.
-// What bounds it (256 rows of 131072 bf16 logits; 67 MB): the read for greedy
+// bins narrowed by the bits of x (constant rows: 0.3 to 0.6 ms).
+// What bounds it (256 rows of 131072 bf16 logits, 67 MB): the read for greedy
 // rows, 17 us; the 64-bit operations of the weights, 28 us a pass, in rows
-// without a cut (44); for top_p the histogram's exponentials and LDS atomics
-// too, 25 (84 to 95).  One row of 49152 fp32 logits, top_k 50, top_p 0.95: 14.6,
-// two passes of one CU over 192 KB and a dozen short steps between barriers.
+// without a cut (41); for top_p the histogram's exponentials and LDS atomics
+// too, 25 (86).  One row of 49152 fp32 logits, top_k 50, top_p 0.95: 14 us, two
+// passes of one CU over 192 KB and a dozen short steps between barriers.
 #include <algorithm>
 
 #include "capi_internal.h"
@@ -689,53 +689,69 @@ SVA_DEV int draw_few(const R& row, SampleLds& s, const Wish& wish, float largest
   return draw(row, s, wish, sorted[kept - 1]);
 }
 
-// Any cut, by a histogram of counts and fp32 weights in one word, exact weights
-// beside it (-1: no token at all, -2: it does not decide, -3: weights
-// cannot be taken so).  fp32 weights are rounded
-// to a unit of 2^-20 of the largest at least: a cut as `near` to the end of its
-// bin as their sums may be off takes the next one in.
+// Any cut, by a histogram of counts (top_k) and fp32 weights (top_p), exact
+// weights beside it (-1: no token at all, -2: it does not decide, -3: weights
+// cannot be taken so, -4: nothing is cut off).  A cut as `near` to the end of its
+// bin as the fp32 sums may be off takes the next one in.
 //
-// The bins begin above the largest of the first group, by as much as the rest
-// is not expected to pass (what does is in the first bin), so that the pass
-// that finds the largest of all is this one (256 rows of 131072: 13 us less).
+// The bins begin above the largest of the row's first elements, by as much as
+// the rest is not expected to pass (if it does, the pass is done again), so that
+// the pass that finds the largest of all is this one (256 rows of 131072: 13 us
+// less).
 template <typename R>
-SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int bits, Largest& largest) {
+SVA_DEV int draw_cut(R& row, SampleLds& s, Wish& wish, double slope, int bits, Largest& largest) {
   const int tid = (int)threadIdx.x;
+  float top;
+  uint32_t weighty = 0;
   {
     Largest some;
 #pragma unroll
     for (int k = 0; k < 1 << TURNS; ++k) some.add(0, row.load(row.place(k)));
-    float top = block_max(s, some.x);
+    top = block_max(s, some.x);
     if (top == -INFINITY) {
       row.template each<LIGHT>([&](int, int, const auto& x) { some.add(0, x); });
       top = block_max(s, some.x);
     }
-    row.ref = top + 256.0f / row.per;
+    row.ref = top + 512.0f / row.per;
     largest = Largest();
   }
-  const int low_bits = 63 - bits;  // (counts of up to 2^bits above them)
-  const u64 one = 1ull << low_bits, rest = one - 1;
-  const float unit = __builtin_amdgcn_ldexpf(1.0f, min(30, low_bits - 1 - bits));
+  const double unit = __builtin_amdgcn_ldexp(1.0, min(51, 62 - bits));  // of a weight of 1, at ref; 2^bits of them fit
   const float hi_slope = (float)slope, lo_slope = (float)(slope - (double)hi_slope);
   for (bool again = false;; again = true) {
-    for (int k = tid; k < BINS; k += SB) s.hist[k] = 0ull;
+    for (int k = tid; k < BINS; k += SB) s.hist[k] = 0ull, s.count[k] = 0u;
     if (tid < 3) s.n[tid] = 0u;
-    if (tid == 0) s.word[4] = 0ull;
+    if (tid == 0) s.word[4] = s.word[5] = 0ull;
     __syncthreads();
     row.template each<HEAVY>([&](int step, int, const auto& x) {
       if (!again) largest.add(step, x);
 #pragma unroll
       for (int k = 0; k < E; ++k) {
         const float v = number(x[k]);
-        u64 add = one;
+        const int bin = bin_of(row, v);
+        if (wish.few) {
+          if (bin < BINS - 1) atomicAdd(&s.count[bin], 1u);
+          weighty += (v - top) * hi_slope > -60.0f ? 1u : 0u;
+        }
         if (wish.share) {
           const float d = fminf(v - row.ref, 0.0f);
-          add |= (uint32_t)__builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(d, hi_slope, d * lo_slope)), unit, 0.5f);
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(d, hi_slope, d * lo_slope));
+          const u64 fixed = (u64)__double_as_longlong(__builtin_fma((double)w, unit, 4503599627370496.0)) - kRaw;
+          atomicAdd(&s.hist[fixed != 0ull ? bin : tid], fixed);  // (0 anywhere: not all in one word)
         }
-        atomicAdd(&s.hist[bin_of(row, v)], add);
       }
     });
     if (again) break;
+    if (wish.few) {
+      u64 all = weighty, none = 0;
+      sum_both(all, none, s);
+      if (all <= wish.top_k) {  // (what top_k cuts off weighs nothing)
+        wish.few = false;
+        if (!wish.share) {
+          row.begin(block_max(s, largest.x));
+          return row.plain() ? -4 : -3;
+        }
+      }
+    }
     row.begin(block_max(s, largest.x));
     if (row.M == -INFINITY) return -1;
     if (!row.plain()) return -3;
@@ -743,29 +759,36 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
     row.ref = row.M;
   }
   __syncthreads();
-  if (tid == SB - 1) s.hist[BINS - 1] -= (u64)(row.steps * SB * E - row.vocab) * one;  // (what is no token)
-  __syncthreads();
-  u64 mine[PT], first = 0, total;
+  u64 mass[PT], first = 0, sum = 0;  // weights before this thread's bins, of all
+  if (wish.share) {
 #pragma unroll
-  for (int k = 0; k < PT; ++k) first += mine[k] = s.hist[PT * tid + k];
-  first = upto_u64(first, s, total) - first;
+    for (int k = 0; k < PT; ++k) first += mass[k] = s.hist[PT * tid + k];
+    first = upto_u64(first, s, sum) - first;
+  }
   int last = BINS;  // the bin of the top_k-th
-  u64 before_last = 0, sum = total & rest;
+  u64 before_last = 0;
   if (wish.few) {
-    u64 before = first;
+    u64 count[PT], before = 0, all, weight = first;
+#pragma unroll
+    for (int k = 0; k < PT; ++k) before += count[k] = s.count[PT * tid + k];
+    before = upto_u64(before, s, all) - before;
+    if (tid == SB - 1) {  // (the last bin holds the rest: masked logits by the thousand would meet in one word)
+      count[PT - 1] = (u64)row.vocab - all;
+      s.count[BINS - 1] = (uint32_t)count[PT - 1];
+    }
 #pragma unroll
     for (int k = 0; k < PT; ++k) {
-      if ((before >> low_bits) < wish.top_k && (before + mine[k]) >> low_bits >= wish.top_k)
-        s.word[0] = before, s.word[1] = (u64)(PT * tid + k);
-      before += mine[k];
+      if (before < wish.top_k && before + count[k] >= wish.top_k)
+        s.word[0] = before, s.word[1] = (u64)(PT * tid + k), s.word[2] = weight;
+      before += count[k];
+      if (wish.share) weight += mass[k];
     }
     __syncthreads();
     last = (int)s.word[1];
-    before_last = (s.word[0] >> low_bits);
-    const u64 in = s.hist[last];
-    if ((in >> low_bits) > CAP) return -2;
-    sum = (s.word[0] & rest) +
-          (u64)((double)(in & rest) * (double)(wish.top_k - before_last) / (double)((in >> low_bits)));
+    before_last = s.word[0];
+    if (s.count[last] > CAP) return -2;
+    if (wish.share)
+      sum = s.word[2] + (u64)((double)s.hist[last] * (double)(wish.top_k - before_last) / (double)s.count[last]);
   }
   int lo = last, hi = last;  // bins in which the cut may fall
   if (wish.share) {
@@ -773,20 +796,18 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
     u64 before = first;
 #pragma unroll
     for (int k = 0; k < PT; ++k) {
-      if ((before & rest) < want && ((before + mine[k]) & rest) >= want)
-        s.word[4] = (u64)(PT * tid + k), s.word[5] = before & rest;
-      before += mine[k];
+      if (before < want && before + mass[k] >= want) s.word[4] = (u64)(PT * tid + k), s.word[5] = before;
+      before += mass[k];
     }
     __syncthreads();
     lo = hi = min((int)s.word[4], last == BINS ? BINS - 1 : last);
-    const u64 near = sum >> 14, begin = s.word[5], end = begin + (s.hist[lo] & rest);
+    const u64 near = sum >> 14, begin = s.word[5], end = begin + s.hist[lo];
     if (lo > 0 && want < begin + near) --lo;
     if (hi < BINS - 1 && hi < last && want + near > end) ++hi;
   }
   const bool joined = hi == last;  // the bin of the top_k-th is among them
-  const int n_list = (int)((s.hist[lo] >> low_bits)) + (hi > lo ? (int)((s.hist[hi] >> low_bits)) : 0);
-  const int n_last = last < BINS ? (int)((s.hist[last] >> low_bits)) : 0;
-  if (n_list > CAP) return -2;
+  const int n_last = wish.few ? (int)s.count[last] : 0;
+  if (wish.few && s.count[lo] + (hi > lo ? s.count[hi] : 0u) > CAP) return -2;
   __syncthreads();
   // The elements of these bins (list 0) and of the top_k-th's (list 1), and
   // exact weights: `above` them, and of all before the top_k-th's bin, `whole`.
@@ -871,12 +892,17 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
     });
   }
   __syncthreads();
+  if (s.n[2] > MANY) return -2;
   for (int i = tid, all = (int)s.n[2]; i < all; i += SB) {
     const uint32_t token = s.many[i];
     const float v = number(row.at((int)token)), b = fminf(row.below(v), (float)(BINS - 1));
     const u64 c = composite(f2key(v), token);
-    if (b >= lo_f && b < end_f) s.list[0][atomicAdd(&s.n[0], 1u)] = c;
-    else if (b >= last_f) s.list[1][atomicAdd(&s.n[1], 1u)] = c;
+    if (b >= lo_f && b < end_f) {
+      const uint32_t place = atomicAdd(&s.n[0], 1u);
+      if (place < CAP) s.list[0][place] = c;
+    } else if (b >= last_f) {
+      s.list[1][atomicAdd(&s.n[1], 1u)] = c;
+    }
     if (by_list && b < last_f) {
       const u64 w = row.weight(v);
       whole += w;
@@ -887,6 +913,8 @@ SVA_DEV int draw_cut(R& row, SampleLds& s, const Wish& wish, double slope, int b
     }
   }
   sum_both(above, whole, s);
+  const int n_list = (int)s.n[0];
+  if (n_list > CAP) return -2;
   int n = n_list;
   if (wish.few) {
     const int of_last = (int)(wish.top_k - before_last);
@@ -955,6 +983,7 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
     else token = draw_all(row, s, wish);
   }
   if (token == -2) token = draw_cut(row, s, wish, slope, p.vocab_bits, largest);
+  if (token == -4) token = draw_all(row, s, wish);
   if (token == -2) token = exact_draw(row, s, wish);
   if (token == -3) token = exact_draw(odd, s, wish);
   if (token < 0 && row.M > -INFINITY) {  // the largest, the lowest of equal ones

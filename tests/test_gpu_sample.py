@@ -89,6 +89,35 @@ def test_cuts_far_below_the_largest(device, top_k, top_p, T):
     compare(device, x, rng.random(8), torch.float32, top_k=top_k, top_p=top_p, temperature=T)
 
 
+@pytest.mark.parametrize("mask", [-np.inf, float(np.finfo(np.float32).min), -1e9])
+@pytest.mark.parametrize("V,kept", [(3000, 40), (40000, 900), (40000, 9000)])
+def test_masked_vocabularies(device, V, kept, mask):
+    """Most tokens masked, the first ones of the row among them; top_k of more tokens than are left."""
+    rng = np.random.default_rng(V + kept)
+    x = normal(rng, 6, V)
+    for b in range(6):
+        x[b, rng.permutation(V)[:V - kept]] = mask
+        x[b, :V // 2 if b % 2 else 0] = mask
+    u = rng.random(6)
+    for params in ({}, {"top_p": 0.9}, {"top_k": 300}, {"top_k": 8000}, {"top_k": 8000, "top_p": 0.8}, {"min_p": 0.01},
+                   {"top_k": 10000, "top_p": 0.999, "temperature": 0.4}, {"top_k": 20, "top_p": 0.7}):
+        compare(device, x, u, torch.float32, **params)
+
+
+@pytest.mark.parametrize("T", [0.1, 1.0, 8.0])
+@pytest.mark.parametrize("V", [16384, 16385, 60000])
+def test_the_largest_come_last(device, V, T):
+    """Rows whose first thousands of logits are far below the others, or rise to the end."""
+    rng = np.random.default_rng(V)
+    x = normal(rng, 8, V)
+    x[:4, :15000] -= 60.0
+    x[4:6].sort(axis=1)
+    x[6:, -5:] += 40.0
+    for dtype in (torch.float32, torch.bfloat16):
+        for params in ({"top_p": 0.9}, {"top_k": 700}, {"top_k": 700, "top_p": 0.6}, {"top_k": 7000, "min_p": 0.001}, {}):
+            compare(device, x, rng.random(8), dtype, temperature=T, **params)
+
+
 def test_values_that_are_not_finite(device):
     rng = np.random.default_rng(5)
     V = 9000
