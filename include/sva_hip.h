@@ -642,8 +642,9 @@ int sva_prompt_attention(const void *q, int dtype, int64_t q_seq_stride, int64_t
 
 /*
  * Writes rows of K and V: token t of sequence b goes to row first_rows[b] + t
- * ([n_seq] int64 on the device); rows without a page, and below 0, are
- * skipped.  No two of a call's tokens may name one row.
+ * ([n_seq] int64 on the device); rows without a page are skipped, and so is a
+ * sequence whose first row is below 0.  No two of a call's tokens may name one
+ * row.
  *   keys / values  (b, g, t, d) at b*kv_seq_stride + g*kv_head_stride +
  *                  t*kv_row_stride + d, of the pool's dtype
  */
@@ -654,7 +655,8 @@ int sva_paged_write(const void *keys, const void *values, int kv_dtype, int64_t 
 
 /*
  * Rows first_rows[b] + t, laid out as sva_paged_write takes them (16-byte
- * aligned rows); rows without a page read as 0.
+ * aligned rows); rows without a page, and all of a sequence whose first row is
+ * below 0, read as 0.
  */
 int sva_paged_read(const void *pool, int64_t n_pages, int64_t page_stride, int64_t page_rows, const int32_t *tables,
                    int64_t table_stride, int64_t max_pages, const int64_t *first_rows, int64_t n_seq, int64_t n_rows,

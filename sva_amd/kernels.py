@@ -1158,7 +1158,8 @@ def paged_write(keys: torch.Tensor, values: torch.Tensor, pool: torch.Tensor, ta
     """Writes keys / values [n_seq, G, T, D] (or [G, T, D]) of the pool's dtype
     into their pages: token t of sequence b into row first_rows[b] + t (int64
     [n_seq] on the device, as pages_reserve gives it, or ints).  Rows without a
-    page, and below 0, are skipped; no two tokens may name one row."""
+    page are skipped, and so is a sequence whose first row is below 0 (that was
+    given no room); no two tokens may name one row."""
 
     n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(pool)
     if keys.dim() == 3:
@@ -1191,7 +1192,8 @@ def _page_first_rows(first_rows, n_seq: int, device: torch.device) -> torch.Tens
 
 def paged_read(pool: torch.Tensor, tables: torch.Tensor, first_rows, n_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows first_rows[b] + t, t < n_rows, of every sequence as keys and values
-    [n_seq, G, n_rows, D]; rows without a page read as 0."""
+    [n_seq, G, n_rows, D]; rows without a page, and all of a sequence whose
+    first row is below 0, read as 0."""
 
     n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(pool)
     n_seq, entries, table_stride = _check_tables(tables)

@@ -110,6 +110,27 @@ def test_many_sequences_and_pages(device):
     assert [t[:-(-n // 16)] for t, n in zip(c.tables.tolist(), c.lens.tolist())] == model.held
 
 
+def test_rows_of_sequences_without_room(device):
+    """A sequence that was given no room writes none of its rows, the second token no more than the first."""
+    from sva_amd import kernels as k
+
+    pool = torch.randn(4, 2, 1, 16, 8, device=device)
+    tables, lens = ints(device, [[2, -1, -1, -1], [0, -1, -1, -1]], torch.int32), ints(device, [9, 3])
+    refs = ints(device, [1, 0, 1, 0], torch.int32)
+    first, src, dst = k.pages_reserve(tables, lens, refs, ints(device, [50, 5]), 16)  # three pages, of two; none
+    assert first.tolist() == [-1, 3] and lens.tolist() == [9, 8]
+    keys = torch.randn(2, 1, 5, 8, device=device)
+    want = pool.clone()
+    want[0, 0, 0, 3:8], want[0, 1, 0, 3:8] = keys[1, 0], -keys[1, 0]
+    k.paged_write(keys, -keys, pool, tables, first)
+    assert torch.equal(pool, want)
+    got = k.paged_read(pool, tables, first, 5)
+    assert (got[0][0] == 0).all() and (got[1][0] == 0).all() and torch.equal(got[0][1], keys[1])
+    for far in (2 ** 63 - 2, -2 ** 63):
+        k.paged_write(keys, -keys, pool, tables, [far, far])
+        assert torch.equal(pool, want) and (k.paged_read(pool, tables, [far, far], 5)[0] == 0).all()
+
+
 def test_a_full_pool(device):
     """All pages or none: a sequence whose pages are not there changes nothing, one that needs none goes on."""
     c = Cache(device, 4, 8, 6, 16)
