@@ -241,7 +241,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, num_samples: i
     """`num_samples` continuations of each prompt of input_ids [B, T], drawn by kernels.sample_tokens over a paged cache:
     tokens [B * num_samples, T + new], the samples of a prompt one after another.  The prompts are run once, their pages
     shared by the samples.  Sequences that have ended go on as eos_token_id; all having ended, the rest is left out.
-    cache: rows before input_ids (of B sequences), extended in place."""
+    cache: rows before input_ids (of B sequences), extended in place.  A token -1 says that its logits were all NaN or
+    -inf; the sequence goes on from token 0."""
 
     if max_new_tokens < 1 or num_samples < 1:
         raise ValueError(f"{num_samples} samples of {max_new_tokens} tokens")
@@ -261,5 +262,5 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, num_samples: i
         out.append(token[:, None])
         if step + 1 == max_new_tokens or (eos_token_id is not None and bool(ended.all())):
             break
-        logits = model(input_ids=token[:, None], past_key_values=cache, use_cache=True).logits[:, -1]
+        logits = model(input_ids=token[:, None].clamp_min(0), past_key_values=cache, use_cache=True).logits[:, -1]
     return torch.cat(out, 1)

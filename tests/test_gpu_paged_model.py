@@ -150,6 +150,26 @@ def test_beams(device, patched, monkeypatch):
     assert torch.equal(got, want) and len(calls) == (2 * 24 if patched else 0)
 
 
+def test_generate_from_nothing(device):
+    """Logits that are all NaN: -1, and what the model is given next is a token of it."""
+    from sva_amd import generate
+
+    model, _ = setup(device)
+    ids = tokens(device, 2, 9)
+    given = []
+    inner = model.forward
+
+    def forward(input_ids, **kw):
+        given.append(input_ids.tolist())
+        out = inner(input_ids=input_ids.clamp(0, 63), **kw)
+        out.logits = torch.full_like(out.logits, float("nan"))
+        return out
+
+    model.forward = forward
+    assert generate(model, ids, 3).tolist() == [row + [-1, -1, -1] for row in ids.tolist()]
+    assert given == [ids.tolist(), [[0], [0]], [[0], [0]]]
+
+
 def test_generate(device):
     """Samples of prompts drawn token by token as the definition draws them from the model's own logits."""
     from sva_amd import PagedCache, generate
