@@ -40,6 +40,8 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int SB = 512;         // threads: two waves a SIMD, whose registers hold several weights in work
 constexpr int SW = SB / WAVE;
@@ -61,6 +63,16 @@ constexpr int MANY = 8192;       // tokens that are listed
 constexpr u64 kRaw = 0x4330000000000000ull;  // the bits of 2^52
 constexpr int kFew = 256;       // top_k that the threads' largest bound
 
+// bf16 has few values, each its own bin, in falling order: 64 binades of either
+// sign from 2^-55 to 510, 0 and what is smaller, and what is at most -510.  (32
+// binades, from 2^-23, leave out an element of one row in two hundred.)
+constexpr int VALUES = 16384;
+constexpr int VALUE0 = (127 - 55) << 7;  // the bits of 2^-55
+constexpr int PV = VALUES / SB;          // bins of a thread
+constexpr int VROWS = VALUES / WAVE;
+static_assert(PV == 32 && 2 * VROWS <= SHARES, "");
+constexpr float kLow = -510.0f;
+
 struct SampleParams {
   const void* logits;
   int64_t row_stride;
@@ -79,11 +91,18 @@ struct SampleParams {
 
 struct SampleLds {
   double table[256];  // 2^(j / 256 + point)
-  u64 hist[BINS];
-  uint32_t count[BINS];
+  union {
+    struct {
+      u64 hist[BINS];
+      uint32_t count[BINS];
+      u64 list[2][CAP];
+      uint32_t many[MANY];
+    };
+    uint32_t counts[VALUES];  // draw_values
+    u64 weights[VALUES];
+  };
   u64 sums[SHARES];   // the kept weights of a share
-  u64 list[2][CAP];
-  uint32_t many[MANY];
+  u64 ties[SHARES];
   u64 scan[2 * SW];
   u64 word[8];
   float top[SW];
@@ -147,8 +166,9 @@ struct Raw {
   u32x4 w[DT == F32 ? 2 : 1];
   SVA_DEV float operator[](int k) const {
     if constexpr (DT == F32) return __uint_as_float(w[k / 4][k % 4]);
-    else return elem_from_bits(k & 1 ? w[0][k / 2] >> 16 : w[0][k / 2] & 0xFFFFu, DT);
+    else return elem_from_bits(bits(k), DT);
   }
+  SVA_DEV uint32_t bits(int k) const { return k & 1 ? w[0][k / 2] >> 16 : w[0][k / 2] & 0xFFFFu; }  // of 16-bit elements
 };
 
 template <int DT>
@@ -689,6 +709,198 @@ SVA_DEV int draw_few(const R& row, SampleLds& s, const Wish& wish, float largest
   return draw(row, s, wish, sorted[kept - 1]);
 }
 
+// The bins of two elements, 16 bits each.
+SVA_DEV uint32_t value_bins(uint32_t two) {
+  s16x2 i = __builtin_bit_cast(s16x2, two & 0x7FFF7FFFu) - (short)VALUE0;
+  i = __builtin_elementwise_min(__builtin_elementwise_max(i, s16x2{0, 0}), s16x2{VALUES / 2 - 1, VALUES / 2 - 1});
+  const u16x2 minus = __builtin_bit_cast(u16x2, two) >> (unsigned short)15;
+  return __builtin_bit_cast(uint32_t, i) ^ (__builtin_bit_cast(uint32_t, minus) + (VALUES / 2 - 1) * 0x10001u);
+}
+SVA_DEV float bin_value(int bin) {
+  const bool minus = bin >= VALUES / 2;
+  const int i = minus ? bin - VALUES / 2 : VALUES / 2 - 1 - bin;
+  return __uint_as_float((uint32_t)((i == 0 ? 0 : i + VALUE0) | (minus ? 0x8000 : 0)) << 16);
+}
+
+// Sums of the rows of 64 bins, in order: the row in which they come to `want` of
+// the whole sum (VROWS: none), and what is before it.  Every wave gets the same.
+template <typename W>
+SVA_DEV int row_of(const u64* rows, W want, u64& wanted, u64& before) {
+  constexpr int PER = VROWS / WAVE;
+  const int lane = lane_id();
+  u64 v[PER], sum = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) sum += v[k] = rows[PER * lane + k];
+  const u64 upto = wave_upto_u64(sum);
+  wanted = want(readlane_u64(upto, WAVE - 1));
+  u64 at = upto - sum, mine = 0;
+  int row = -1;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const bool here = at < wanted && at + v[k] >= wanted;
+    row = here ? PER * lane + k : row;
+    mine = here ? at : mine;
+    at += v[k];
+  }
+  const u64 found = __ballot(row >= 0);
+  if (found == 0ull) return VROWS;
+  const int from = __builtin_ctzll(found);
+  before = readlane_u64(mine, from);
+  return __builtin_amdgcn_readlane(row, from);
+}
+
+// bf16, any cut: one pass counts the values.  Counts and exact weights of the
+// values are the row's: they name the value at which the cut falls, and how many
+// of the tokens that have it are kept.  A second pass takes the weights from a
+// table, 0 for what is cut off.  -2: a logit of at least 510, or between 0 and
+// 2^-55, or one of at most -510 that weighs something.
+template <typename R>
+SVA_DEV int draw_values(R& row, SampleLds& s, const Wish& wish) {
+  const int tid = (int)threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  constexpr u64 kTie = 1ull << 58;  // (a thread's weights of a share come to 2^51)
+  for (int k = tid; k < VALUES / 4; k += SB) ((u32x4*)s.counts)[k] = u32x4{0u, 0u, 0u, 0u};
+  if (tid == 0) s.n[0] = 0u, s.n[1] = VALUES, s.n[2] = 0u, s.word[4] = ~0ull;
+  __syncthreads();
+  u16x2 small = {0xFFFF, 0xFFFF};
+  row.template each<LIGHT>([&](int, int, const auto& x) {
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
+      small = __builtin_elementwise_min(small, __builtin_bit_cast(u16x2, x.w[0][k] & 0x7FFF7FFFu) - (unsigned short)1);
+      const uint32_t two = value_bins(x.w[0][k]), lo = two & 0xFFFFu, hi = two >> 16;
+      if (lo < VALUES - 1) atomicAdd(&s.counts[lo], 1u);  // (masked logits would meet in one word)
+      if (hi < VALUES - 1) atomicAdd(&s.counts[hi], 1u);
+    }
+  });
+  if (min(small[0], small[1]) < VALUE0) s.n[2] = 1u;
+  __syncthreads();
+  // A wave's bins: every eighth row of 64.  Most are empty: loops over the others
+  // are not unrolled (this code runs once, and waits for its instructions).
+  const int bin0 = wave * WAVE + lane;
+  u64 total = 0, none = 0;
+  int first = VALUES;
+  uint32_t used = 0;  // bit k: row k * SW + wave
+#pragma unroll
+  for (int k = PV - 1; k >= 0; --k) {
+    const uint32_t n = s.counts[bin0 + SB * k];
+    total += n;
+    const u64 any = __ballot(n != 0u);
+    used |= any ? 1u << k : 0u;
+    first = any ? bin0 - lane + SB * k + (int)__builtin_ctzll(any) : first;
+  }
+  if (lane == 0 && first < VALUES) atomicMin(&s.n[1], (uint32_t)first);
+  if (lane < PV) s.ties[lane * SW + wave] = s.ties[VROWS + lane * SW + wave] = 0ull;
+  sum_both(total, none, s);
+  const int top = (int)s.n[1];
+  if (s.n[2] != 0u || top == 0 || top == VALUES) return -2;
+  row.begin(bin_value(top));
+  if (!row.plain() || (total < (u64)row.vocab && !(row.least >= kLow))) return -2;
+  const auto weight = [&](int k) { return row.raw_weight(bin_value(bin0 + SB * k)) - kRaw; };
+  const auto rows_upto = [&](int cut) {  // those of this wave
+    const int n = cut >= wave ? (cut - wave) / SW + 1 : 0;
+    return n >= PV ? used : used & ((1u << n) - 1u);
+  };
+  int cut = VROWS;     // the last row of which something is kept,
+  uint32_t kept = 0;   // and of this lane's bin in it: how many are,
+  u64 want, before;
+  if (wish.few) {
+#pragma unroll 1
+    for (uint32_t m = used; m != 0u; m &= m - 1) {
+      const int k = __builtin_ctz(m);
+      const u64 sum = wave_sum_u64(s.counts[bin0 + SB * k]);
+      if (lane == 0) s.ties[k * SW + wave] = sum;
+    }
+    __syncthreads();
+    cut = row_of(s.ties, [&](u64) { return wish.top_k; }, want, before);
+    if (cut < VROWS) {
+      const uint32_t n = s.counts[cut * WAVE + lane];
+      const u64 above = before + wave_upto_u64(n) - n, left = want > above ? want - above : 0ull;
+      kept = (u64)n < left ? n : (uint32_t)left;
+    }
+  }
+  if (wish.share) {
+    const int last = cut;
+#pragma unroll 1
+    for (uint32_t m = rows_upto(last); m != 0u; m &= m - 1) {
+      const int k = __builtin_ctz(m);
+      const u64 sum = wave_sum_u64((k * SW + wave == last ? kept : s.counts[bin0 + SB * k]) * weight(k));
+      if (lane == 0) s.ties[VROWS + k * SW + wave] = sum;
+    }
+    __syncthreads();
+    cut = row_of(s.ties + VROWS, [&](u64 all) { return share_of(wish.top_p, all); }, want, before);
+    kept = cut == last ? kept : s.counts[cut * WAVE + lane];
+    const u64 each = row.raw_weight(bin_value(cut * WAVE + lane)) - kRaw;
+    const u64 mass = kept * each, above = before + wave_upto_u64(mass) - mass;
+    if (above >= want) {
+      kept = 0u;
+    } else if (above + mass >= want) {
+      const u64 rest = want - above;
+      u64 n = (u64)((double)rest / (double)each);  // (at most 2^20: off by one at most)
+      if (n * each < rest) ++n;
+      if (n * each < rest) ++n;
+      if (n > 1 && (n - 1) * each >= rest) --n;
+      kept = (uint32_t)n;
+    }
+  }
+  const bool whole = cut < VROWS && kept == s.counts[cut * WAVE + lane];  // all of the bin
+  const uint32_t live = rows_upto(cut);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < PV; ++k)
+    if (!(live >> k & 1u)) s.weights[bin0 + SB * k] = 0ull;
+#pragma unroll 1
+  for (uint32_t m = live; m != 0u; m &= m - 1) {
+    const int k = __builtin_ctz(m), bin = bin0 + SB * k;
+    u64 w = weight(k);
+    w = w >= row.least_w && bin < VALUES - 1 ? w : 0ull;
+    if (k * SW + wave == cut) {
+      const bool part = kept != 0u && !whole;
+      if (part) s.word[4] = (u64)bin, s.word[5] = kept, s.word[6] = w;
+      const u64 some = __ballot(kept != 0u);
+      if (lane == 63 - (int)__builtin_clzll(some)) s.n[0] = (uint32_t)bin;
+      w = part ? kTie : (kept != 0u ? w : 0ull);
+    }
+    s.weights[bin] = w;
+  }
+  __syncthreads();
+  const int part = (int)s.word[4];
+  const u64 of_part = s.word[5], w_part = s.word[6];
+  u64 here = 0;
+  row.template each<LIGHT>([&](int step, int, const auto& x) {
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
+      const uint32_t two = value_bins(x.w[0][k]);
+      here += s.weights[two & 0xFFFFu];
+      here += s.weights[two >> 16];
+    }
+    if ((~step & ((1 << row.turns) - 1)) != 0) return;
+    const int share = (step >> row.turns) * SW + wave;
+    const u64 v = wave_sum_u64(here & (kTie - 1));
+    if (lane == 0) s.sums[share] = v;
+    if (part >= 0) {
+      const u64 same = wave_sum_u64(here / kTie);
+      if (lane == 0) s.ties[share] = same;
+    }
+    here = 0;
+  });
+  __syncthreads();
+  u64 thr = cut < VROWS ? composite(f2key(bin_value((int)s.n[0])), (uint32_t)row.vocab) : 0ull;
+  if (part >= 0) {
+    // which tokens of that value: the first ones
+    const uint32_t key = f2key(bin_value(part));
+    const auto tie = [&](float x, int token) { return f2key(x) == key && row.has(token) ? 1ull : 0ull; };
+    for (int k = tid; k < row.shares(); k += SB) s.hist[k] = s.sums[k], s.sums[k] = s.ties[k];
+    __syncthreads();
+    const int end = find(row, s, tie, [&](u64) { return of_part - 1; });
+    thr = composite(key, (uint32_t)end);
+    const int share = (int)s.word[1];
+    for (int k = tid; k < row.shares(); k += SB)
+      s.sums[k] = s.hist[k] + w_part * (k < share ? s.ties[k] : (k == share ? of_part - s.word[0] : 0ull));
+    __syncthreads();
+  }
+  const int token = draw(row, s, wish, thr);
+  return token < 0 ? -2 : token;
+}
+
 // Any cut, by a histogram of counts (top_k) and fp32 weights (top_p), exact
 // weights beside it (-1: no token at all, -2: it does not decide, -3: weights
 // cannot be taken so, -4: nothing is cut off).  A cut as `near` to the end of its
@@ -981,6 +1193,9 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
     else if (!row.plain()) token = -3;
     else if (few) token = draw_few(row, s, wish, fminf(largest.x, 3.40282347e38f));
     else token = draw_all(row, s, wish);
+  }
+  if constexpr (DT == BF16) {
+    if (token == -2 && p.vocab > kSpread) token = draw_values(row, s, wish);
   }
   if (token == -2) token = draw_cut(row, s, wish, slope, p.vocab_bits, largest);
   if (token == -4) token = draw_all(row, s, wish);
