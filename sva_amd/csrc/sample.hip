@@ -70,6 +70,7 @@ constexpr int VALUES = 16384;
 constexpr int VALUE0 = (127 - 55) << 7;  // the bits of 2^-55
 constexpr int PV = VALUES / SB;          // bins of a thread
 constexpr int VROWS = VALUES / WAVE;
+constexpr int ZERO = VALUES / 2 - 1;     // -0: the next
 static_assert(PV == 32 && 2 * VROWS <= SHARES, "");
 constexpr float kLow = -510.0f;
 
@@ -773,6 +774,8 @@ SVA_DEV int draw_values(R& row, SampleLds& s, const Wish& wish) {
   });
   if (min(small[0], small[1]) < VALUE0) s.n[2] = 1u;
   __syncthreads();
+  if (tid == 0) s.counts[ZERO] += s.counts[ZERO + 1], s.counts[ZERO + 1] = 0u;  // (-0 equals 0)
+  __syncthreads();
   // A wave's bins: every eighth row of 64.  Most are empty: loops over the others
   // are not unrolled (this code runs once, and waits for its instructions).
   const int bin0 = wave * WAVE + lane;
@@ -861,6 +864,8 @@ SVA_DEV int draw_values(R& row, SampleLds& s, const Wish& wish) {
     }
     s.weights[bin] = w;
   }
+  __syncthreads();
+  if (tid == 0) s.weights[ZERO + 1] = s.weights[ZERO];
   __syncthreads();
   const int part = (int)s.word[4];
   const u64 of_part = s.word[5], w_part = s.word[6];

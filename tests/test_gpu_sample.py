@@ -78,6 +78,59 @@ def test_ties(device, top_k, top_p, dtype):
         compare(device, x, u, dtype, near=0.0 if x.min() == x.max() else None, top_k=top_k, top_p=top_p)
 
 
+@pytest.mark.parametrize("top_k,top_p,min_p", [(5000, 1.0, 0.0), (0, 0.5, 0.0), (7000, 0.3, 0.0), (12500, 1.0, 0.0),
+                                               (12500, 0.8, 0.1), (0, 0.9, 0.3), (19990, 0.99999, 0.0), (300, 0.5, 0.0)])
+@pytest.mark.parametrize("V", [20000, 100003])
+def test_few_values(device, V, top_k, top_p, min_p):
+    """bf16 rows of a few values, -0 beside 0: the cut falls among thousands of equal logits."""
+    rng = np.random.default_rng(V + top_k)
+    values = [[0.0, -0.0, 1.0, -2.0], [0.0, -0.0], [-0.0, -1.0, -3.0], [2.0, 3.0, 3.015625], [-5.0, -5.03125, -100.0]]
+    x = np.stack([rng.choice(np.array(v, np.float32), V) for v in values for _ in range(3)])
+    # (the 300 largest are equal in every row: they weigh 1 each, half of their sum is 150 exactly, and 300 times a number
+    # of 24 bits is exact in 64: no border is unclear)
+    compare(device, x, rng.random(len(x)), torch.bfloat16, near=0.0 if top_k == 300 else None, top_k=top_k, top_p=top_p,
+            min_p=min_p)
+
+
+@pytest.mark.parametrize("T", [0.05, 1.0, 12.0, 500.0])
+def test_values_at_the_ends_of_bf16(device, T):
+    """bf16 logits of 510 and more, of less than 2^-55, of -510 and less that weigh something, and far below."""
+    rng = np.random.default_rng(5)
+    V = 30001
+    x = normal(rng, 14, V)
+    x[0] += 507.0
+    x[1, 20] = 1e30
+    x[2, ::3] *= 1e-20
+    x[3, ::2] = 0.0
+    x[4, ::2] *= 2.0 ** -54
+    x[5] -= 508.0
+    x[6] -= 511.0
+    x[7, ::2] = -509.0
+    x[8, ::2] = -512.0
+    x[9, 1:] = -np.inf
+    x[10, ::2] = np.nan
+    x[11, 5::7] = -np.nan
+    x[12, 9000] = np.inf
+    x[13] *= 1e4
+    u = rng.random(14)
+    for params in ({"top_p": 0.9}, {"top_k": 6000}, {"top_k": 14000, "top_p": 0.99}, {"top_p": 0.7, "min_p": 0.01}):
+        compare(device, x, u, torch.bfloat16, temperature=T, **params)
+
+
+@pytest.mark.parametrize("mask", [-np.inf, float(np.finfo(np.float32).min) * 0.99, -1e4])
+@pytest.mark.parametrize("V,kept", [(40000, 900), (130001, 9000)])
+def test_masked_bf16(device, V, kept, mask):
+    rng = np.random.default_rng(V + kept)
+    x = normal(rng, 6, V)
+    for b in range(6):
+        x[b, rng.permutation(V)[:V - kept]] = mask
+        x[b, :V // 2 if b % 2 else 0] = mask
+    u = rng.random(6)
+    for params in ({"top_p": 0.9}, {"top_k": 300}, {"top_k": 8000}, {"top_k": 8000, "top_p": 0.8},
+                   {"top_k": 10000, "top_p": 0.999, "temperature": 0.4}, {"top_p": 0.9, "temperature": 20.0}):
+        compare(device, x, u, torch.bfloat16, **params)
+
+
 @pytest.mark.parametrize("top_k,top_p,T", [(5000, 1.0, 1.0), (0, 0.7, 1.0), (9000, 0.9, 1.0), (3000, 0.5, 0.01), (0, 0.999, 30.0)])
 def test_cuts_far_below_the_largest(device, top_k, top_p, T):
     """One logit far above the others, so that a cut lies where the first bins say nothing; and logits far apart."""
