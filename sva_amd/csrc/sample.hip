@@ -23,12 +23,16 @@
 // The share in which the answer lies is gone over again.  What the histogram
 // cannot decide (a bin of more elements than are sorted, logits or a temperature
 // at the ends of their range) is done over again with exact weights throughout,
-// bins narrowed by the bits of x (constant rows: 0.3 to 0.6 ms).
+// bins narrowed by the bits of x (256 constant rows of fp16: 0.6 to 1.1 ms).
+// Long bf16 rows have few values for their tokens: draw_values counts them, and
+// takes weights once for a value, not for a token.
 // What bounds it (256 rows of 131072 bf16 logits, 67 MB): the read for greedy
 // rows, 17 us; the 64-bit operations of the weights, 28 us a pass, in rows
-// without a cut (41); for top_p the histogram's exponentials and LDS atomics
-// too, 25 (86).  One row of 49152 fp32 logits, top_k 50, top_p 0.95: 14 us, two
-// passes of one CU over 192 KB and a dozen short steps between barriers.
+// without a cut (42); for top_p (45) the two passes, 16 us each, bin numbers
+// and LDS as long as the read, and between and behind them a dozen short steps.
+// fp16 and fp32, top_p: the histogram's exponentials and LDS atomics, 25 us, and
+// a pass of weights (80).  One row of 49152 fp32 logits, top_k 50, top_p 0.95: 14
+// us, two passes of one CU over 192 KB and a dozen short steps between barriers.
 #include <algorithm>
 
 #include "capi_internal.h"
@@ -1200,6 +1204,8 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
     else token = draw_all(row, s, wish);
   }
   if constexpr (DT == BF16) {
+    // (64 rows of 20000, top_p 0.9: 22 us, 27 by the histogram; 8 of 4000: its steps between the passes alone take
+    // as long as what they save)
     if (token == -2 && p.vocab > kSpread) token = draw_values(row, s, wish);
   }
   if (token == -2) token = draw_cut(row, s, wish, slope, p.vocab_bits, largest);
