@@ -65,6 +65,8 @@ struct PagedType {
   static constexpr int ES = DT == F32 ? 4 : 2;
   using elem = typename std::conditional<DT == BF16, __bf16, _Float16>::type;
   using frag = typename std::conditional<DT == BF16, bf16x8, f16x8>::type;
+  // weights are 2^kBelow at a new reference; in a range's sums too, whoever takes them
+  static constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;
   // waves per SIMD that the registers are kept to (four for the narrowest send 20 registers through scratch memory: 32
   // sequences of up to 131072 keys, 9 x 64 bf16, 416 us against 297)
   static constexpr int waves(int dp) { return dp * ES <= 128 ? 3 : (dp * ES <= 256 ? 2 : 1); }
@@ -83,8 +85,9 @@ SVA_DEV f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 }
 
 // One query row again over keys [k0, end), key by key, by one wave: lanes take
-// 64 keys' scores, then the row's elements.  Finite V whose sums are too large:
-// once more, weights and sums 2^-60 of themselves.
+// 64 keys' scores, then the row's elements.  Weights are those of the tiles, as
+// other ranges' sums join these.  Finite V whose sums are too large: once more,
+// weights and sums 2^-60 of themselves.
 template <int DT, int DP>
 SVA_DEV void attend_again(const PagedParams& p, int64_t qa, int b, int g, int k0, int end, float sl, float (&acc)[DP / 64],
                           float& m, float& z) {
@@ -112,7 +115,8 @@ SVA_DEV void attend_again(const PagedParams& p, int64_t qa, int b, int g, int k0
       }
       const float mn = fmaxf(m, wave_max(sc));
       const float corr = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sl);
-      const float e = page >= 0 ? __builtin_amdgcn_exp2f((sc - (mn == -INFINITY ? 0.0f : mn)) * sl) * down : 0.0f;
+      const float below = __builtin_fmaf(sc - (mn == -INFINITY ? 0.0f : mn), sl, PagedType<DT>::kBelow);
+      const float e = page >= 0 ? __builtin_amdgcn_exp2f(below) * down : 0.0f;
       m = mn;
       z = z * corr + wave_sum(e);
 #pragma unroll
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP)) paged_att
   constexpr int PS = DP + 3;               // a query row's m, z and sums of one wave
   constexpr int VB = WIDE ? 0 : AW * TK * VS, PB = AW * TR * PS * 4;
   constexpr float kMost = DT == F16 ? 32768.0f : 65536.0f;  // a lane's weights of a tile may sum to
-  constexpr float kBelow = DT == F16 ? 8.0f : 0.0f;         // weights are 2^8 at a new reference
+  constexpr float kBelow = Type::kBelow;
   constexpr float kLarge = 0x1p110f;                        // all ranges' sums of less stay finite together
   __shared__ __align__(16) unsigned char lds[VB > PB ? VB : PB];
   __shared__ uint32_t odd_rows;

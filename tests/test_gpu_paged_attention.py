@@ -148,6 +148,52 @@ def test_what_is_not_seen_reaches_nothing(device, dtype):
             assert (got[:, :, 3].float() == bad).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_a_range_done_again_joins_the_others(device, dtype):
+    """Several ranges, of which one holds what takes its sums out of the finite numbers: its share stays as large as it is."""
+    from sva_amd import kernels
+
+    lens, H, G, D, P = [3000, 2100], 4, 2, 64, 16
+    pool, tables, seq_lens, kv, gen = make(device, lens, G, D, P, dtype)
+    q = normal(gen, (2, H, 5, D), dtype, device)
+    clean, want = pool.clone(), kernels.paged_attention(q, pool, tables, seq_lens, 0.3)
+    check(want, q, kv, lens, 0.3)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for b, n in enumerate(lens):  # the last row: seen by token 4 alone
+            pool[int(tables[b, (n - 1) // P]), :, :, (n - 1) % P] = bad
+        got = kernels.paged_attention(q, pool, tables, seq_lens, 0.3)
+        for b, n in enumerate(lens):
+            for h in range(H):
+                allowed = np.arange(n) <= n - 5 + np.arange(4)[:, None]
+                check_attention(got[b, h, :4], q[b, h, :4], kv[b][0, h // 2], kv[b][1, h // 2], allowed, 0.3)
+    # an infinite element of V is one of the output; the others are as they were
+    pool.copy_(clean)
+    pool[int(tables[0, 1500 // P]), 1, :, 1500 % P, 7] = float("inf")
+    got = kernels.paged_attention(q, pool, tables, seq_lens, 0.3)
+    assert torch.isinf(got[0, :, :, 7]).all()
+    rest = torch.arange(D, device=device) != 7
+    for h in range(H):
+        allowed = np.arange(3000) <= 2995 + np.arange(5)[:, None]
+        whole = torch.where(rest, got[0, h], want[0, h])
+        check_attention(whole, q[0, h], kv[0][0, h // 2], kv[0][1, h // 2], allowed, 0.3)
+    # rows without a page, page 0 (which is read in their place) of NaN
+    pool.copy_(clean)
+    tables[0, 60] = -1
+    zero = (tables == 0).nonzero()
+    for b, at in zero.tolist():
+        tables[b, at] = -1
+    pool[0] = float("nan")
+    gone = {0: [60], 1: []}
+    for b, at in zero.tolist():
+        gone[b].append(at)
+    got = kernels.paged_attention(q, pool, tables, seq_lens, 0.3)
+    for b, n in enumerate(lens):
+        there = ~np.isin(np.arange(n) // P, gone[b])
+        for h in range(H):
+            allowed = (np.arange(n) <= n - 5 + np.arange(5)[:, None]) & there
+            check_attention(got[b, h], q[b, h], kv[b][0, h // 2], kv[b][1, h // 2], allowed, 0.3)
+
+
 def test_an_infinite_key_takes_or_leaves_all(device):
     """Scores of -inf weigh nothing, of one +inf make the row NaN, as in softmax."""
     from sva_amd import kernels
