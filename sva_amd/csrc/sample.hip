@@ -185,7 +185,8 @@ struct Row {
   float ref, per;          // where the bins begin, and bins for a logit's difference of 1
   double rate, off;        // x rate + off: 256ths of a binade below M
   float T, least;          // logits below the least weigh nothing
-  u64 least_w;             // min_p
+  float min_p;
+  u64 least_w;             // min_p of the largest weight
   const double* table;
 
   // elements at + k of the aligned window; what lies outside the row is -inf
@@ -212,12 +213,15 @@ struct Row {
     }
     return r;
   }
-  // the largest logit is known
+  // the largest logit is known (and the table).  Its weight is not a whole 2^point: `off` is rounded, and M = 50 at T =
+  // 0.2 weighs 2^46 - 1.  What is kept by min_p = 1 weighs as much as it does.
   SVA_DEV void begin(float largest) {
     M = largest;
     off = -(double)M * rate;
     least = M - 55.4f * T;  // 2^-80
+    least_w = min_p > 0.0f && plain() ? share_of_largest(weight(M)) : 0ull;
   }
+  SVA_DEV u64 share_of_largest(u64 w) const { return (u64)__builtin_ceil((double)min_p * (double)w); }
   SVA_DEV bool plain() const { return T >= 1e-30f && __builtin_fabs(off) <= 268435456.0; }
   SVA_DEV bool has(int token) const { return (uint32_t)token < (uint32_t)vocab; }
   // this thread's elements of a step, in the window
@@ -281,6 +285,7 @@ struct OddRow : Row<DT> {
   SVA_DEV u64 weight(float x) const {
     return this->raw(__builtin_fmax(((double)x - (double)this->M) * this->rate, -20480.0)) - kRaw;
   }
+  SVA_DEV void begin_odd() { this->least_w = this->share_of_largest(weight(this->M)); }
 };
 
 template <typename R>
@@ -1187,7 +1192,7 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
   const double slope = 1.44269504088896340736 / (double)T;
   row.rate = 256.0 * slope;
   row.per = 64.0f / fmaxf(T, 0.25f);
-  row.least_w = (u64)__builtin_ceil((double)fmaxf(min_p, 0.0f) * __builtin_amdgcn_ldexp(1.0, p.point));
+  row.min_p = fmaxf(min_p, 0.0f);
   if (tid < 256) s.table[tid] = exp2((double)tid / 256.0 + (double)p.point);
   const bool random = !(T <= 0.0f) && k != 1;
   const bool cut = random && (wish.few || wish.share), few = cut && wish.few && wish.top_k <= kFew;
@@ -1211,7 +1216,10 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
   if (token == -2) token = draw_cut(row, s, wish, slope, p.vocab_bits, largest);
   if (token == -4) token = draw_all(row, s, wish);
   if (token == -2) token = exact_draw(row, s, wish);
-  if (token == -3) token = exact_draw(odd, s, wish);
+  if (token == -3) {
+    odd.begin_odd();
+    token = exact_draw(odd, s, wish);
+  }
   if (token < 0 && row.M > -INFINITY) {  // the largest, the lowest of equal ones
     __syncthreads();
     if (tid == 0) s.n[1] = 0xFFFFFFFFu;

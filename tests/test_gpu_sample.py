@@ -263,3 +263,22 @@ def test_in_a_graph_and_on_another_stream(device):
         x.mul_(1.01)
         graph.replay()
         assert torch.equal(out, kernels.sample_tokens(x, u, top_p=0.9, top_k=10000)), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [0.05, 0.1, 0.2, 0.7])
+@pytest.mark.parametrize("V", [3, 3000, 20000])
+def test_only_what_weighs_as_much_as_the_largest(device, V, T, dtype):
+    """min_p = 1 with tied largest logits, of any size against the temperature: all of them are kept, and nothing else."""
+    rng = np.random.default_rng(V)
+    B = 48
+    x = np.minimum(normal(rng, B, V), 4.0)
+    top = 5.0 + np.concatenate([np.arange(B - 4) * 1.375, [12.875, 13.75, 25.5, 45.0]]).astype(np.float32)  # 17.875, 18.75, 30.5, 50
+    for b in range(B):
+        x[b, rng.permutation(V)[:2 if V == 3 else 2 + 5 * b]] = top[b]
+    u = rng.random(B)
+    for params in ({}, {"top_p": 0.9}, {"top_k": max(1, V // 2)}, {"top_k": 40}, {"top_k": 600, "top_p": 0.47}):
+        got = compare(device, x, u, dtype, temperature=T, min_p=1.0, **params)
+        assert all(x[b, g] == top[b] for b, g in enumerate(got))
+    odd = np.where(np.arange(B) % 2, np.float32(1e-32), np.float32(T))  # too cold for the usual weights
+    compare(device, x, u, dtype, temperature=odd, min_p=1.0)
