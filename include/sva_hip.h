@@ -667,7 +667,8 @@ int sva_paged_read(const void *pool, int64_t n_pages, int64_t page_stride, int64
  * Attention of the last Q tokens of every sequence over its rows: token t sees
  * row n iff n <= seq_lens[b] - Q + t and the row has a page; a token that sees
  * none gives 0.  n_keys is at least every length; the part of a sequence behind
- * it, or behind max_pages pages, is not read.  What an unseen row holds, NaN
+ * it, or behind max_pages pages, is not read (tokens keep their places: one
+ * behind that part sees every row before it).  What an unseen row holds, NaN
  * and infinities included, reaches no output.
  *   q        of the pool's dtype, (b, h, t, d) at b*q_seq_stride +
  *            h*q_head_stride + t*q_tok_stride + d

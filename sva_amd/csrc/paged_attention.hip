@@ -1,11 +1,11 @@
 // Attention of a few tokens over a KV cache in pages (pages.h).
 //
 // out[h, t] = sum_n p[n] V[n] / sum_n p[n], p[n] = exp(s (q[h, t] . K[n]) - m)
-// over the rows n <= len - Q + t of the sequence, in one pass over its pages
-// with a running reference m.  Each wave takes 32-key tiles on its own, K and
-// V of the next ones under way in registers; the query rows (token, head of
-// the KV group) of a workgroup are 16 at a time, so that a tile serves all of
-// them: S^T = K Q^T and O^T = V^T P^T on 16x16 matrix instructions.
+// over the rows n <= len - Q + t of the sequence that are read, in one pass over
+// its pages with a running reference m.  Each wave takes 32-key tiles on its
+// own, K and V of the next ones under way in registers; the query rows (token,
+// head of the KV group) of a workgroup are 16 at a time, so that a tile serves
+// all of them: S^T = K Q^T and O^T = V^T P^T on 16x16 matrix instructions.
 //  * 16 aligned keys lie in one page: a tile is two halves whose addresses are
 //    scalars.  Page numbers come 64 at a time, one a lane, 32 tiles ahead.
 //  * S^T leaves a lane with scores of one query row that are its share of the
@@ -178,6 +178,9 @@ __global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP)) paged_att
   const int ranges = tile_ranges(len, p.chunk);
   if (split >= ranges) return;
   const int k0 = split * p.chunk, k1 = k0 + min(p.chunk, len - k0);
+  // rows that the first token sees: of the length itself, also where not all of it is read
+  const int64_t seen = min(max(p.lens[b], (int64_t)0), (int64_t)1 << 40) - p.Q + 1;
+  auto seen_by = [&](int t) { return (int)max(min(seen + t, (int64_t)k1), (int64_t)0); };  // of keys below k1
   const int dim = PAD ? p.D : DP;
   const uint32_t rowb = (uint32_t)dim * ES;
 
@@ -221,8 +224,8 @@ __global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP)) paged_att
       bq[j] = x;
     }
   }
-  const int lim = live ? min(k1 - 1, len - p.Q + tok) : -1;  // the last key this query row may see here
-  const int full = min(k1, len - p.Q + rt * TR / grp + 1);   // keys below are seen by every row
+  const int lim = live ? seen_by(tok) - 1 : -1;  // the last key this query row may see here
+  const int full = seen_by(rt * TR / grp);       // keys below are seen by every row
   const float sl = score_scale(p.scaling);
   float top = -3.40282347e38f, z = 0.0f;  // weights are 2^((score - top) sl + kBelow)
   f32x4 o[NO];
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(AW * WAVE, PagedType<DT>::waves(DP)) paged_att
     const int t = gr / grp, h = g * grp + gr % grp;
     float acc[DP / 64], m, zz;
     attend_again<DT, DP>(p, (int64_t)b * p.q_bs + (int64_t)h * p.q_hs + (int64_t)t * p.q_ts, b, g, k0,
-                         min(k1, len - p.Q + t + 1), sl, acc, m, zz);
+                         seen_by(t), sl, acc, m, zz);
 #pragma unroll
     for (int k = 0; k < DP / 64; ++k)
       if (lane + 64 * k < p.D) put(row, lane + 64 * k, acc[k], m, zz);

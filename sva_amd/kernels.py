@@ -1220,7 +1220,8 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor, s
     rows in pages: token t of q [n_seq, H, Q, D] (of the pool's dtype) sees row
     n iff n <= seq_lens[b] - Q + t and the row has a page (0 where it sees
     none).  seq_lens int64 [n_seq] on the device; n_keys: at least the longest
-    (rows behind it are not read; default: all that the tables can hold).
+    (rows behind it are not read, and no token changes its place for it;
+    default: all that the tables can hold).
     Inference only: no gradient."""
 
     n_pages, kv_heads, page_rows, dim, page_stride = _check_pool(pool)

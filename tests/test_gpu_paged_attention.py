@@ -194,6 +194,28 @@ def test_a_range_done_again_joins_the_others(device, dtype):
             check_attention(got[b, h], q[b, h], kv[b][0, h // 2], kv[b][1, h // 2], allowed, 0.3)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,cut", [(100, 50), (100, 97), (3000, 2600), (3000, 2998)])
+def test_sequences_longer_than_what_is_read(device, n, cut, dtype):
+    """Rows behind n_keys, or behind the table, are not read; a token still sees every row up to its own place before."""
+    from sva_amd import kernels
+
+    H, G, D, P, Q = 4, 2, 64, 16, 5
+    pool, tables, seq_lens, kv, gen = make(device, [n], G, D, P, dtype)
+    q = normal(gen, (1, H, Q, D), dtype, device)
+    short = tables[:, :cut // P]
+    for got, rows in ((kernels.paged_attention(q, pool, tables, seq_lens, 0.2, n_keys=cut), cut),
+                      (kernels.paged_attention(q, pool, short, seq_lens, 0.2), cut // P * P)):
+        for h in range(H):
+            allowed = np.arange(rows) <= n - Q + np.arange(Q)[:, None]
+            check_attention(got[0, h], q[0, h], kv[0][0, h // 2, :rows], kv[0][1, h // 2, :rows], allowed, 0.2)
+    # lengths past any table, and none
+    far = kernels.paged_attention(q, pool, tables, torch.tensor([2 ** 62], device=device), 0.2, n_keys=cut)
+    for h in range(H):
+        check_attention(far[0, h], q[0, h], kv[0][0, h // 2, :cut], kv[0][1, h // 2, :cut], np.ones((Q, cut), bool), 0.2)
+    assert (kernels.paged_attention(q, pool, tables, torch.tensor([-2 ** 63], device=device), 0.2, n_keys=cut) == 0).all()
+
+
 def test_an_infinite_key_takes_or_leaves_all(device):
     """Scores of -inf weigh nothing, of one +inf make the row NaN, as in softmax."""
     from sva_amd import kernels
