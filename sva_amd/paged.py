@@ -163,16 +163,21 @@ class PagedCache(Cache):
     # ------------------------------------------------------------------ sequences
     def fork(self, sources) -> None:
         """The batch becomes forks of its sequences: new sequence i of `sources` (int64 tensor, or ints; any number of
-        them, each a sequence's) shares the pages of sequence sources[i].  Those that are not named are freed."""
+        them, each a sequence's) shares the pages of sequence sources[i].  Those that are not named are freed.  The
+        numbers are looked at by the host, which waits for those that are on the device."""
 
         if self.pool is None:
             return
-        device, old = self.tables.device, self.tables.shape[0]
         sources = torch.as_tensor(sources, dtype=torch.int64).flatten()
-        if sources.device.type == "cpu" and not bool(((sources >= 0) & (sources < old)).all()):
-            raise ValueError(f"forks of {sources.tolist()} from a paged cache of {old} sequences")
-        sources = sources.to(device)  # (on the device they are not looked at: others leave a sequence as it was)
-        new = sources.shape[0]
+        host, old = sources.cpu(), self.tables.shape[0]
+        if not bool(((host >= 0) & (host < old)).all()):
+            raise ValueError(f"forks of {host.tolist()} from a paged cache of {old} sequences")
+        self._fork(sources.to(self.tables.device))
+
+    def _fork(self, sources: torch.Tensor) -> None:
+        """The same for int64 numbers on the device that are known to be sequences'."""
+
+        old, new = self.tables.shape[0], sources.shape[0]
         if new > old:
             self.tables = torch.cat([self.tables, self.tables.new_full((new - old, self.tables.shape[1]), -1)])
             self.lens = torch.cat([self.lens, self.lens.new_zeros(new - old)])
@@ -189,11 +194,11 @@ class PagedCache(Cache):
 
     def batch_repeat_interleave(self, repeats: int) -> None:
         if self.pool is not None:
-            self.fork(torch.arange(self.tables.shape[0], device=self.tables.device).repeat_interleave(repeats))
+            self._fork(torch.arange(self.tables.shape[0], device=self.tables.device).repeat_interleave(repeats))
 
     def batch_select_indices(self, indices: torch.Tensor) -> None:
         if self.pool is not None:
-            self.fork(torch.arange(self.tables.shape[0], device=self.tables.device)[indices])
+            self.fork(torch.arange(self.tables.shape[0])[torch.as_tensor(indices).cpu()])
 
     def crop(self, tokens_to_remove: int) -> None:
         """Drops the last -tokens_to_remove rows (a positive number: rows behind it)."""
@@ -205,9 +210,12 @@ class PagedCache(Cache):
         if self.pool is None or keep == self.length:
             return
         gone = self.tables[:, self._pages(keep):self._pages(self.length)]
-        self.refs.index_add_(0, gone.flatten().long(), torch.full((gone.numel(),), -1, device=gone.device, dtype=torch.int32))
+        pages = gone.flatten().long()
+        there = (pages >= 0) & (pages < self.refs.shape[0])  # (a sequence that kernels.pages_fork freed has none)
+        if self.refs.shape[0] > 0:
+            self.refs.index_add_(0, torch.where(there, pages, 0), -there.int())
         gone.fill_(-1)
-        self.lens.fill_(keep)
+        self.lens.clamp_(max=keep)
         self.length, self.first_rows = keep, None
 
     def compact(self, release: bool = False) -> None:

@@ -226,3 +226,29 @@ def test_refusals(device):
     for bad in ([0, 2], [-1]):
         with pytest.raises(ValueError, match="forks"):
             cache.fork(bad)
+
+
+def test_forks_of_no_sequence_are_refused(device):
+    """Numbers on the device are looked at too, and nothing changes: the cache goes on, and a crop finds its pages."""
+    from sva_amd import PagedCache
+
+    model, bundle = setup(device)
+    ids = tokens(device, 2, 60)
+    cache = PagedCache(model.config)
+    feed(model, cache, ids, 0, 40)
+    held = cache.tables.clone(), cache.lens.clone(), cache.refs.clone()
+    for bad in ([0, 2], [-1, 0], [0, 1, -1], [1, 0, 5], [2 ** 40, 0]):
+        for call in (cache.fork, cache.reorder_cache):
+            with pytest.raises(ValueError, match="forks"):
+                call(torch.tensor(bad, device=device))
+    for bad in ([0, 2], [-3]):
+        with pytest.raises(IndexError):
+            cache.batch_select_indices(torch.tensor(bad, device=device))
+    assert all(torch.equal(a, b) for a, b in zip(held, (cache.tables, cache.lens, cache.refs)))
+    cache.batch_select_indices(torch.tensor([False, True], device=device))
+    cache.batch_repeat_interleave(2)
+    cache.crop(-15)
+    assert int(cache.refs.sum()) == 2 * 2 and cache.lens.tolist() == [25, 25]
+    rows = torch.cat([ids[1:, :25], ids[1:, 40:]], 1).expand(2, -1)
+    got = feed(model, cache, rows, 25, 45)
+    near(got, feed(model, DynamicCache(), rows, 0, 45)[:, -20:])

@@ -173,3 +173,38 @@ def test_workspaces():
     assert lib.sva_pages_reserve_workspace_bytes(3, 10) == 0 and lib.sva_pages_reserve_workspace_bytes(3, 10000) >= 3 * 16 + 40000
     assert lib.sva_pages_reserve_workspace_bytes(2000, 10) >= 2000 * 16 + 40 and lib.sva_pages_fork_workspace_bytes(3, 10) == 0
     assert lib.sva_pages_fork_workspace_bytes(3, 10000) >= 3 * 8 + 120000 and lib.sva_pages_compact_workspace_bytes(7) >= 28
+
+
+@pytest.mark.parametrize("keep,refs,lens", [(40, [1, 2, 2, 0], [40, 0, 40]), (33, [1, 2, 2, 0], [33, 0, 33]),
+                                            (32, [1, 2, 0, 0], [32, 0, 32]), (20, [1, 2, 0, 0], [20, 0, 20]), (0, [0, 0, 0, 0], [0, 0, 0])])
+def test_crop_of_a_batch_with_a_freed_sequence(keep, refs, lens):
+    """A sequence that kernels.pages_fork freed names no page: a crop counts none for it and leaves its length."""
+    from transformers import LlamaConfig
+
+    from sva_amd import PagedCache
+
+    cache = PagedCache(LlamaConfig(hidden_size=64, num_attention_heads=1, num_key_value_heads=1, num_hidden_layers=1))
+    cache._begin(3, torch.zeros(3, 1, 45, 64))
+    cache.pool = torch.zeros(1, 4, 2, 1, 16, 64)
+    cache.tables = torch.tensor([[0, 1, 2, -1], [-1, -1, -1, -1], [0, 1, 2, -1]], dtype=torch.int32)
+    cache.tables[2, 0] = 2 ** 31 - 1  # (an entry outside the pool names no page either)
+    cache.refs = torch.tensor([1, 2, 2, 0], dtype=torch.int32)
+    cache.lens = torch.tensor([45, 0, 45])
+    cache.length = cache.layers[0].length = 45
+    cache.crop(keep - 45)
+    assert cache.refs.tolist() == refs and cache.lens.tolist() == lens and cache.get_seq_length() == keep
+    held = -(-keep // 16)
+    assert (cache.tables[:, held:] == -1).all() and (held == 0 or cache.tables[0, :held].tolist() == [0, 1, 2][:held])
+
+
+def test_crop_of_a_cache_without_pages():
+    from transformers import LlamaConfig
+
+    from sva_amd import PagedCache
+
+    cache = PagedCache(LlamaConfig(hidden_size=64, num_attention_heads=1, num_key_value_heads=1, num_hidden_layers=1))
+    cache._begin(1, torch.zeros(1, 1, 20, 64))
+    cache.tables = torch.full((1, 2), -1, dtype=torch.int32)
+    cache.length = cache.layers[0].length = 20
+    cache.crop(-20)
+    assert cache.length == 0 and cache.lens.tolist() == [0]
