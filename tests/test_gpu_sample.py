@@ -282,3 +282,34 @@ def test_only_what_weighs_as_much_as_the_largest(device, V, T, dtype):
         assert all(x[b, g] == top[b] for b, g in enumerate(got))
     odd = np.where(np.arange(B) % 2, np.float32(1e-32), np.float32(T))  # too cold for the usual weights
     compare(device, x, u, dtype, temperature=odd, min_p=1.0)
+
+
+def test_masked_and_absent_logits_take_no_longer(device):
+    """A share of the sum (top_p) at temperatures whose reciprocal fp32 rounds up, or down: rows that do not fill their
+    last step, and rows masked with -inf or the lowest number, are cut in the same number of passes.  (A row that is done
+    over again takes several times as long; the factor leaves room for the cards' noise alone.)"""
+    from sva_amd import kernels
+
+    gen = torch.Generator(device=device).manual_seed(2)
+
+    def time(x, T):
+        u = torch.rand(x.shape[0], device=device, generator=gen)
+        kernels.sample_tokens(x, u, temperature=T, top_p=0.9)
+        best = float("inf")
+        for _ in range(15):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(4):
+                kernels.sample_tokens(x, u, temperature=T, top_p=0.9)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    for V, mask in ((50001, None), (49152, -float("inf")), (49152, torch.finfo(torch.float32).min)):
+        x = torch.randn(64, V, device=device, generator=gen) * 2.0
+        if mask is not None:
+            x[:, torch.randperm(V, device=device, generator=gen)[:V // 2]] = mask
+        want = time(x, 1.0)
+        for T in (0.7, 0.8, 0.9):
+            assert time(x, T) < 2.0 * want, (V, mask, T)
