@@ -1202,7 +1202,8 @@ __global__ void __launch_bounds__(SB) sample_kernel(SampleParams p) {
 
   Largest largest;
   int token = -2;
-  if (!cut || few) {
+  // (T under 4.3e-39 puts 1 / (T ln 2) past fp32, in which draw_cut counts what weighs something; none so cold is plain)
+  if (!cut || few || !(T >= 1e-30f)) {
     row.template each<LIGHT>([&](int step, int, const auto& x) { largest.add(step, x); });
     row.begin(block_max(s, largest.x));
     row.ref = row.M;

@@ -313,3 +313,17 @@ def test_masked_and_absent_logits_take_no_longer(device):
         want = time(x, 1.0)
         for T in (0.7, 0.8, 0.9):
             assert time(x, T) < 2.0 * want, (V, mask, T)
+
+
+@pytest.mark.parametrize("T", [1e-39, 1e-44, 1e-36, 1e-31])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_cuts_of_ties_at_any_temperature(device, T, dtype):
+    """top_k among equal largest logits where 1 / temperature is past fp32."""
+    V = 30000
+    x = np.full((6, V), -2.0, np.float32)
+    x[3:] = 0.5
+    x[3:, ::3] = 1.25
+    u = np.array([0.0, 0.3, 0.77, 0.1, 0.5, 0.99], np.float32)
+    # (equal weights of 2^45 each: sums and borders are exact)
+    for params in ({"top_k": 300}, {"top_k": 5000}, {"top_k": 5000, "top_p": 0.5}, {"top_k": 40}):
+        compare(device, x, u, dtype, temperature=T, near=0.0, **params)
