@@ -15,6 +15,8 @@ gradient are refused (run the model under ``torch.no_grad()``).
 
 from __future__ import annotations
 
+import inspect
+
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
 
@@ -255,7 +257,9 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, num_samples: i
     if max_new_tokens < 1 or num_samples < 1:
         raise ValueError(f"{num_samples} samples of {max_new_tokens} tokens")
     cache = PagedCache(model.config) if cache is None else cache
-    logits = model(input_ids=input_ids, past_key_values=cache, use_cache=True).logits[:, -1]
+    # (a prompt's other logits, 2 T V bytes of them in bf16, are not asked for where the model can leave them out)
+    last = {"logits_to_keep": 1} if "logits_to_keep" in inspect.signature(model.forward).parameters else {}
+    logits = model(input_ids=input_ids, past_key_values=cache, use_cache=True, **last).logits[:, -1]
     if num_samples > 1:
         cache.batch_repeat_interleave(num_samples)
         logits = logits.repeat_interleave(num_samples, 0)

@@ -252,3 +252,24 @@ def test_forks_of_no_sequence_are_refused(device):
     rows = torch.cat([ids[1:, :25], ids[1:, 40:]], 1).expand(2, -1)
     got = feed(model, cache, rows, 25, 45)
     near(got, feed(model, DynamicCache(), rows, 0, 45)[:, -20:])
+
+
+@pytest.mark.parametrize("batch,samples", [(1, 1), (2, 3)])
+def test_generate_takes_the_last_logits_alone(device, batch, samples):
+    """Nothing but the last token of a prompt goes through the output layer; a model that takes no such wish gives all."""
+    from sva_amd import generate
+
+    model, bundle = setup(device)
+    ids = tokens(device, batch, 50)
+    seen = []
+    hook = model.lm_head.register_forward_pre_hook(lambda m, args: seen.append(tuple(args[0].shape[:2])))
+    with patch_llama_attention(model, bundle):
+        got = generate(model, ids, 3, num_samples=samples, temperature=0.0)
+        assert seen == [(batch, 1), (batch * samples, 1), (batch * samples, 1)]
+        seen.clear()
+        inner = model.forward
+        model.forward = lambda input_ids, past_key_values, use_cache: inner(input_ids=input_ids, past_key_values=past_key_values,
+                                                                            use_cache=use_cache)
+        assert torch.equal(generate(model, ids, 3, num_samples=samples, temperature=0.0), got)
+        assert seen == [(batch, 50), (batch * samples, 1), (batch * samples, 1)]
+    hook.remove()
